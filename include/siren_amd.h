@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define SIREN_ABI_VERSION 7
+#define SIREN_ABI_VERSION 8
 
 enum {
     SIREN_OK = 0,
@@ -410,6 +410,55 @@ int32_t siren_forward_laplace_store(const siren_cfg* cfg, const float* ws, const
                                     float* gx, float* lap, float* tws, void* stream);
 int32_t siren_laplace_backward_stored(const siren_cfg* cfg, const float* ws, const float* x, int64_t n,
                                       const float* glap, float* tws, float* gx, float* gparams, void* stream);
+
+/* ---- 8-bit training: block-scaled operands ---------------------------------------------------------------------
+ * A tensor in 8 bits is e4m3 (format 0; e5m2: format 1) values with one power-of-two scale for each block of 128,
+ * held as its exponent byte: value * 2^(byte - 127). The scale is the smallest with which the block's largest finite
+ * magnitude is at most 448 (57344) times the scale, byte >= 1; a value is rounded once, to the nearest, ties to even;
+ * NaN and infinities become NaN (e5m2 keeps infinities). Layout of a (rows, cols) tensor quantised along its columns:
+ *   values (rows, C), C = cols rounded up to a multiple of 128, the padding zero
+ *   scales (R, S) bytes, S = C / 128 rounded up to a multiple of 4; R = rows (one scale per 1 x 128) or, with tiles,
+ *   rows / 128 rounded up (one per 128 x 128)
+ * dtype of unquantised tensors: 0 fp32, 1 bf16, 2 fp16. Values, outputs and workspaces 16-byte aligned, scales 4. */
+
+/* x (rows, cols) of row stride ld -> q, s: quantised along the columns; qt, st: the transpose (cols, rows), quantised
+ * along the rows, laid out as a (cols, rows) tensor. Either pair may be NULL. mult (rows, cols) bf16, contiguous,
+ * nullable: x is multiplied by it first. colsum (cols) fp32, nullable: the column sums of what is quantised, before
+ * rounding (a bias's gradient), through colsum_ws of ceil(rows / 128) * cols floats. With rows == 0 nothing is
+ * written. */
+int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, const void* mult,
+                           int32_t format, int32_t tiles, void* q, void* s, void* qt, void* st, float* colsum_ws,
+                           float* colsum, void* stream);
+
+/* out (m, n) = act(a b^T + bias) of a (m, k) and b (n, k) quantised along k, sums in 32 bits. a may be e4m3 or e5m2,
+ * b is e4m3. act 0: none, 1: sin(omega z), with deriv (m, n) bf16, nullable, = omega cos(omega z). bias (n) fp32,
+ * nullable. ws: siren_fp8_matmul_ws_bytes(m, n, k) bytes. */
+int32_t siren_fp8_matmul_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes);
+int32_t siren_fp8_matmul(const void* a, const void* sa, int64_t m, int32_t a_tiles, int32_t a_format, const void* b,
+                         const void* sb, int64_t n, int32_t b_tiles, int64_t k, const float* bias, int32_t act,
+                         float omega, void* out, int32_t dtype, void* deriv, void* ws, void* stream);
+
+/* y (m, n) = act(x w^T + bias), the layer of siren_fp8_quantize (rows of x, e4m3) and siren_fp8_matmul in one call:
+ * x (m, k) of row stride ld, w (n, k) in 8 bits with tiles, y in x's dtype. ws: siren_fp8_linear_ws_bytes. */
+int32_t siren_fp8_linear_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes);
+int32_t siren_fp8_linear(const void* x, int32_t dtype, int64_t m, int64_t k, int64_t ld, const void* w, const void* sw,
+                         int64_t n, const float* bias, int32_t act, float omega, void* y, void* ws, void* stream);
+
+/* torch.nn.utils.clip_grad_norm_(max_norm) + torch.optim.AdamW.step over count tensors (HOST arrays of their device
+ * pointers, element counts and dtypes; a gradient has its parameter's dtype; a NULL gradient leaves its tensor and
+ * state as they are; no two tensors overlap):
+ *   c = min(1, max_norm / (||g|| + 1e-6)) over all gradients (no clip when max_norm <= 0)
+ *   m = m + (1 - b1)(c g - m), v = b2 v + (1 - b2)(c g)^2, p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+ * The states are flat: tensor i's begins at the sum of the earlier tensors' element counts, each rounded up to a
+ * multiple of 128. state_bits 32: exp_avg, exp_avg_sq fp32. state_bits 8: e4m3 codes of m and of sqrt(v), with one
+ * scale byte per 128 in scale_avg / scale_avg_sq (255: the block is NaN), rounded at random by splitmix64 of (seed, t,
+ * element). step: DEVICE int64, the number of steps before this one; the call adds 1, t is the sum. scratch:
+ * siren_adamw_scratch_bytes(count) bytes of this call's own; its float at byte 32 receives ||g|| (0 without max_norm). */
+int32_t siren_adamw_scratch_bytes(int64_t count, int64_t* bytes);
+int32_t siren_adamw_step(int64_t count, void* const* params, const void* const* grads, const int64_t* numels,
+                         const int32_t* dtypes, int32_t state_bits, void* exp_avg, void* exp_avg_sq, void* scale_avg,
+                         void* scale_avg_sq, int64_t* step, double lr, double beta1, double beta2, double eps,
+                         double weight_decay, double max_norm, uint64_t seed, void* scratch, void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,7 +11,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('SIREN_AMD_LIB', os.path.join(_HERE, 'libsiren_amd.so'))
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 # Error codes (include/siren_amd.h)
 SIREN_OK, SIREN_EINVAL, SIREN_EUNSUPPORTED, SIREN_EHIP = 0, 1, 2, 3
@@ -30,6 +30,8 @@ class SirenUnsupported(RuntimeError):
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
+_I32 = ctypes.c_int32
+_F64 = ctypes.c_double
 _CFG = ctypes.POINTER(SirenCfg)
 
 # name -> argtypes; every entry point returns int32 status
@@ -97,6 +99,15 @@ _SIGS = {
     'siren_second_order_batched': [_CFG, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P],
     'siren_hvp_backward_batched_ws_floats': [_CFG, _I64, _I64, ctypes.POINTER(_I64)],
     'siren_hvp_backward_batched': [_CFG, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    'siren_fp8_quantize': [_P, _I32, _I64, _I64, _I64, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _P],
+    'siren_fp8_matmul_ws_bytes': [_I64, _I64, _I64, ctypes.POINTER(_I64)],
+    'siren_fp8_matmul': [_P, _P, _I64, _I32, _I32, _P, _P, _I64, _I32, _I64, _P, _I32, ctypes.c_float, _P, _I32, _P, _P,
+                         _P],
+    'siren_fp8_linear_ws_bytes': [_I64, _I64, _I64, ctypes.POINTER(_I64)],
+    'siren_fp8_linear': [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _I32, ctypes.c_float, _P, _P, _P],
+    'siren_adamw_scratch_bytes': [_I64, ctypes.POINTER(_I64)],
+    'siren_adamw_step': [_I64, _P, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _F64, _F64, _F64, _F64, _F64, _F64,
+                         ctypes.c_uint64, _P, _P],
 }
 EXPORTED = ('siren_abi_version', 'siren_last_error') + tuple(_SIGS)
 

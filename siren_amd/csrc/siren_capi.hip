@@ -1,5 +1,7 @@
 // siren_capi.hip — the C ABI of libsiren_amd.so (include/siren_amd.h): validation, workspace sizing and
 // dispatch to the kernel launchers (launch.h; one translation unit per kernel family).
+#include "adamw.h"
+#include "fp8.h"
 #include "hess_kernel.hpp"
 #include "launch.h"
 #include "siren_common.h"
@@ -1655,6 +1657,171 @@ int32_t siren_backward_stored_batched(const siren_cfg* cfg, const float* ws, con
                                            gx + b * n * d, gparams + b * P, stream))
             return rc;
     return SIREN_OK;
+}
+
+// ---- 8-bit training: block quantisation, products of 8-bit operands, AdamW over many tensors ------------------------
+namespace {
+bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+
+int check_fp8_type(int32_t dtype) {
+    return dtype >= siren::FP8_F32 && dtype <= siren::FP8_F16 ? SIREN_OK : fail(SIREN_EINVAL, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+}
+int check_fp8_product(int64_t m, int64_t n, int64_t k) {
+    if (m < 0 || n < 0 || k < 1) return fail(SIREN_EINVAL, "fp8 product: need m, n >= 0 and k >= 1");
+    if (siren::fp8_blocks(k) > kMaxGrid || siren::fp8_blocks(m) > kMaxGrid / std::max<int64_t>(1, siren::fp8_blocks(n)))
+        return fail(SIREN_EINVAL, "fp8 product: too many tiles");
+    return SIREN_OK;
+}
+int check_fp8_act(int32_t act, float omega, const void* deriv) {
+    if (act != siren::FP8_ACT_NONE && act != siren::FP8_ACT_SINE) return fail(SIREN_EINVAL, "fp8 product: act is 0 (none) or 1 (sine)");
+    if (act == siren::FP8_ACT_SINE && !std::isfinite(omega)) return fail(SIREN_EINVAL, "fp8 product: omega must be finite");
+    if (deriv != nullptr && act != siren::FP8_ACT_SINE) return fail(SIREN_EINVAL, "fp8 product: deriv belongs to the sine");
+    return SIREN_OK;
+}
+int check_fp8_operands(const void* a, const void* sa, const void* b, const void* sb, const float* bias, const void* out,
+                       const void* deriv) {
+    if (a == nullptr || sa == nullptr || b == nullptr || sb == nullptr || out == nullptr)
+        return fail(SIREN_EINVAL, "fp8 product: NULL pointer");
+    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(sa, 4) || !aligned(sb, 4) || !aligned(out, 16) ||
+        !aligned(deriv, 16) || !aligned(bias, 4))
+        return fail(SIREN_EINVAL, "fp8 product: values and out must be 16-byte aligned, scales and bias 4-byte aligned");
+    return SIREN_OK;
+}
+int check_fp8_source(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld) {
+    if (rows > 1 && ld < cols) return fail(SIREN_EINVAL, "fp8: need a row stride of at least the columns");
+    if (x == nullptr || !aligned(x, dtype == siren::FP8_F32 ? 4 : 2))
+        return fail(SIREN_EINVAL, "fp8: x is NULL or not aligned to its type");
+    return SIREN_OK;
+}
+}  // namespace
+
+int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, const void* mult,
+                           int32_t format, int32_t tiles, void* q, void* s, void* qt, void* st, float* colsum_ws,
+                           float* colsum, void* stream) {
+    if (int rc = check_fp8_type(dtype)) return rc;
+    if (rows < 0 || cols < 0 || (format != 0 && format != 1))
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: need rows, cols >= 0 and format 0 (e4m3) or 1 (e5m2)");
+    if (siren::fp8_blocks(cols) > kMaxGrid / std::max<int64_t>(1, siren::fp8_blocks(rows)))
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: too many tiles");
+    if ((q == nullptr) != (s == nullptr) || (qt == nullptr) != (st == nullptr))
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: values and scales go together");
+    if (colsum != nullptr && colsum_ws == nullptr) return fail(SIREN_EINVAL, "siren_fp8_quantize: colsum needs colsum_ws");
+    if (rows == 0 || cols == 0) return SIREN_OK;
+    if (int rc = check_fp8_source(x, dtype, rows, cols, ld)) return rc;
+    if (q == nullptr && qt == nullptr && colsum == nullptr) return fail(SIREN_EINVAL, "siren_fp8_quantize: nothing to write");
+    if (!aligned(q, 16) || !aligned(qt, 16) || !aligned(s, 4) || !aligned(st, 4) || !aligned(mult, 2))
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: q and qt must be 16-byte aligned, scales 4-byte aligned");
+    siren::Fp8Quant a{x, ld, rows, cols, mult, (uint8_t*)q, (uint8_t*)s, (uint8_t*)qt, (uint8_t*)st,
+                      colsum != nullptr ? colsum_ws : nullptr, dtype, format, tiles != 0};
+    siren::launch_fp8_quant((hipStream_t)stream, a);
+    if (colsum != nullptr)
+        siren::launch_fp8_colsum((hipStream_t)stream, colsum_ws, siren::fp8_blocks(rows), cols, colsum);
+    return hip_status("siren_fp8_quantize");
+}
+
+int32_t siren_fp8_matmul_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes) {
+    if (bytes == nullptr) return fail(SIREN_EINVAL, "bytes is NULL");
+    if (int rc = check_fp8_product(m, n, k)) return rc;
+    *bytes = m == 0 || n == 0 ? 0 : siren::fp8_product_ws_bytes(m, n, k);
+    return SIREN_OK;
+}
+
+int32_t siren_fp8_matmul(const void* a, const void* sa, int64_t m, int32_t a_tiles, int32_t a_format, const void* b,
+                         const void* sb, int64_t n, int32_t b_tiles, int64_t k, const float* bias, int32_t act,
+                         float omega, void* out, int32_t dtype, void* deriv, void* ws, void* stream) {
+    if (int rc = check_fp8_type(dtype)) return rc;
+    if (int rc = check_fp8_product(m, n, k)) return rc;
+    if (a_format != 0 && a_format != 1)
+        return fail(SIREN_EINVAL, "siren_fp8_matmul: a_format is 0 (e4m3) or 1 (e5m2)");
+    if (int rc = check_fp8_act(act, omega, deriv)) return rc;
+    if (m == 0 || n == 0) return SIREN_OK;
+    if (int rc = check_fp8_operands(a, sa, b, sb, bias, out, deriv)) return rc;
+    if (!aligned(ws, 16)) return fail(SIREN_EINVAL, "siren_fp8_matmul: ws must be 16-byte aligned");
+    if (siren::fp8_product_ws_bytes(m, n, k) > 0 && ws == nullptr)
+        return fail(SIREN_EINVAL, "siren_fp8_matmul: ws is NULL (siren_fp8_matmul_ws_bytes)");
+    siren::Fp8Product p{{(const uint8_t*)a, (const uint8_t*)sa, m, a_tiles ? 7 : 0},
+                        {(const uint8_t*)b, (const uint8_t*)sb, n, b_tiles ? 7 : 0},
+                        k, bias, act, omega, out, dtype, deriv, a_format, ws};
+    siren::launch_fp8_product((hipStream_t)stream, p);
+    return hip_status("siren_fp8_matmul");
+}
+
+int32_t siren_fp8_linear_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes) {
+    if (bytes == nullptr) return fail(SIREN_EINVAL, "bytes is NULL");
+    if (int rc = check_fp8_product(m, n, k)) return rc;
+    *bytes = m == 0 || n == 0 ? 0
+                              : (m * siren::fp8_padded(k) + m * siren::fp8_scale_cols(k) + 15) / 16 * 16 +
+                                    siren::fp8_product_ws_bytes(m, n, k);
+    return SIREN_OK;
+}
+
+int32_t siren_fp8_linear(const void* x, int32_t dtype, int64_t m, int64_t k, int64_t ld, const void* w, const void* sw,
+                         int64_t n, const float* bias, int32_t act, float omega, void* y, void* ws, void* stream) {
+    if (int rc = check_fp8_type(dtype)) return rc;
+    if (int rc = check_fp8_product(m, n, k)) return rc;
+    if (int rc = check_fp8_act(act, omega, nullptr)) return rc;
+    if (m == 0 || n == 0) return SIREN_OK;
+    if (int rc = check_fp8_source(x, dtype, m, k, ld)) return rc;
+    if (int rc = check_fp8_operands(ws, ws, w, sw, bias, y, nullptr)) return rc;
+    uint8_t* q = (uint8_t*)ws;
+    uint8_t* s = q + m * siren::fp8_padded(k);
+    uint8_t* rest = q + (m * siren::fp8_padded(k) + m * siren::fp8_scale_cols(k) + 15) / 16 * 16;
+    if (int rc = siren_fp8_quantize(x, dtype, m, k, ld, nullptr, 0, 0, q, s, nullptr, nullptr, nullptr, nullptr, stream))
+        return rc;
+    return siren_fp8_matmul(q, s, m, 0, 0, w, sw, n, 1, k, bias, act, omega, y, dtype, nullptr, rest, stream);
+}
+
+int32_t siren_adamw_scratch_bytes(int64_t count, int64_t* bytes) {
+    if (bytes == nullptr) return fail(SIREN_EINVAL, "bytes is NULL");
+    if (count < 0) return fail(SIREN_EINVAL, "siren_adamw_scratch_bytes: need count >= 0");
+    *bytes = siren::adamw_scratch_bytes(count);
+    return SIREN_OK;
+}
+
+int32_t siren_adamw_step(int64_t count, void* const* params, const void* const* grads, const int64_t* numels,
+                         const int32_t* dtypes, int32_t state_bits, void* exp_avg, void* exp_avg_sq, void* scale_avg,
+                         void* scale_avg_sq, int64_t* step, double lr, double beta1, double beta2, double eps,
+                         double weight_decay, double max_norm, uint64_t seed, void* scratch, void* stream) {
+    if (count < 0 || (state_bits != 8 && state_bits != 32))
+        return fail(SIREN_EINVAL, "siren_adamw_step: need count >= 0 and state_bits 8 or 32");
+    if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !std::isfinite(lr) ||
+        !std::isfinite(weight_decay) || !std::isfinite(eps))
+        return fail(SIREN_EINVAL, "siren_adamw_step: need 0 <= beta < 1, eps >= 0 and finite lr, weight_decay");
+    if (step == nullptr || scratch == nullptr || !aligned(step, 8) || !aligned(scratch, 16))
+        return fail(SIREN_EINVAL, "siren_adamw_step: step and scratch must be aligned device memory");
+    if (count > 0 && (params == nullptr || grads == nullptr || numels == nullptr || dtypes == nullptr))
+        return fail(SIREN_EINVAL, "siren_adamw_step: NULL pointer");
+    int64_t total = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (int rc = check_fp8_type(dtypes[i])) return rc;
+        if (numels[i] < 0) return fail(SIREN_EINVAL, "siren_adamw_step: negative numel");
+        const size_t size = dtypes[i] == siren::FP8_F32 ? 4 : 2;
+        if (numels[i] > 0 && (params[i] == nullptr || !aligned(params[i], size) || !aligned(grads[i], size)))
+            return fail(SIREN_EINVAL, "siren_adamw_step: a parameter is NULL or not aligned to its type");
+        total += siren::fp8_blocks(numels[i]);
+    }
+    if (total > 0xFFFFFFFFll) return fail(SIREN_EINVAL, "siren_adamw_step: more than 2^32 blocks of state");
+    if (total > 0 && (exp_avg == nullptr || exp_avg_sq == nullptr || !aligned(exp_avg, 16) || !aligned(exp_avg_sq, 16) ||
+                      (state_bits == 8 && (scale_avg == nullptr || scale_avg_sq == nullptr))))
+        return fail(SIREN_EINVAL, "siren_adamw_step: states must be 16-byte aligned, 8-bit ones with their scales");
+    siren::AdamwCall c;
+    c.count = count;
+    c.p = params;
+    c.g = grads;
+    c.numel = numels;
+    c.dtype = dtypes;
+    c.bits = state_bits;
+    c.m = exp_avg;
+    c.v = exp_avg_sq;
+    c.sm = (uint8_t*)scale_avg;
+    c.sv = (uint8_t*)scale_avg_sq;
+    c.step = step;
+    c.h = siren::AdamwHyper{lr, beta1, beta2, max_norm > 0.0 ? max_norm : 0.0, (float)(1.0 - beta1), (float)beta2,
+                            (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay), seed};
+    c.scratch = scratch;
+    siren::launch_adamw((hipStream_t)stream, c);
+    return hip_status("siren_adamw_step");
 }
 
 }  // extern "C"

@@ -1,0 +1,246 @@
+// tu_fp8_quant.hip — rounding tensors to 8 bits with a scale for each block of 128.
+//
+//   s = 2^e, the smallest with which the block's largest finite magnitude is at most 448 s (e5m2: 57344 s), e >= -126
+//   q = x / s to the nearest e4m3 (e5m2) value, ties to even; infinities and NaN become NaN (e5m2 keeps infinities)
+//
+// A power of two divides exactly, so the one rounding is q's, and a dequantised value is a bf16 number exactly.
+// A training step needs a tensor both as rows (blocks along the columns) and transposed (blocks along the rows, for
+// the product that sums over the rows): one workgroup holds a 128 x 128 tile in registers and writes both, with the
+// column sums of a bias's gradient on the way, so the tensor is read once. 64 values a thread: 16 rows x 4 columns, so
+// a row's maximum is a reduction over half a wave, a column's one over LDS, and the transpose leaves as 16-byte pieces.
+#include "fp8.h"
+#include "siren_common.h"
+
+namespace siren {
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr int QT = 128;           // tile edge
+constexpr int QSTRIDE = QT + 16;  // LDS row of the transposed bytes: 16-byte pieces on distinct banks
+
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = __builtin_fabsf(x);
+    return a < INFINITY ? a : 0.f;
+}
+
+// the exponent byte of a block whose largest finite magnitude is amax: 448 = 1.75 * 2^8, 57344 = 1.75 * 2^15
+template <bool E5M2>
+__device__ __forceinline__ int exponent_byte(float amax) {
+    const uint32_t b = __float_as_uint(amax);
+    const int e = (int)(b >> 23) - (E5M2 ? 15 : 8) + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return e < 1 ? 1 : e;
+}
+__device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
+
+template <bool E5M2>
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+    if constexpr (E5M2) {
+        const int lo = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_bf8_f32(c, d, lo, true);
+    } else {
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+    }
+}
+
+template <typename T, bool E5M2>
+__global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                                    const __bf16* __restrict__ mult, uint8_t* __restrict__ q,
+                                                    uint8_t* __restrict__ s, uint8_t* __restrict__ qt,
+                                                    uint8_t* __restrict__ st, float* __restrict__ colsum, int tiles,
+                                                    int vec, int col_blocks) {
+    __shared__ __align__(16) uint8_t tr[QT * QSTRIDE];
+    __shared__ float part[8][QT];
+    __shared__ float wmax[4];
+    const int t = threadIdx.x, c4 = t & 31, rg = t >> 5;
+    const int64_t rb = blockIdx.x / col_blocks;
+    const int cb = (int)(blockIdx.x % col_blocks);
+    const int64_t r0 = rb * QT + rg * 16;
+    const int64_t c0 = (int64_t)cb * QT + c4 * 4;
+    const int64_t row_blocks = (rows + QT - 1) / QT;
+    const int64_t s_ld = (col_blocks + 3) / 4 * 4, st_ld = (row_blocks + 3) / 4 * 4;
+
+    f32x4 v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        f32x4 e = {0.f, 0.f, 0.f, 0.f};
+        if (r0 + i < rows) {
+            const T* src = x + (r0 + i) * ld + c0;
+            if (vec && c0 + 4 <= cols) {
+                if constexpr (sizeof(T) == 4) {
+                    e = *(const f32x4*)src;
+                } else {
+                    typedef T T4 __attribute__((ext_vector_type(4)));
+                    const T4 h = *(const T4*)src;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) e[k] = (float)h[k];
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (c0 + k < cols) e[k] = (float)src[k];
+            }
+            if (mult != nullptr) {
+                const __bf16* ms = mult + (r0 + i) * cols + c0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (c0 + k < cols) e[k] *= (float)ms[k];
+            }
+        }
+        v[i] = e;
+    }
+
+    if (colsum != nullptr) {  // 16 rows a thread, then the 8 row groups in order
+        f32x4 sum = v[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) sum += v[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[rg][c4 * 4 + k] = sum[k];
+        __syncthreads();
+        if (t < QT && (int64_t)cb * QT + t < cols) {
+            float a = part[0][t];
+#pragma unroll
+            for (int g = 1; g < 8; ++g) a += part[g][t];
+            colsum[rb * cols + (int64_t)cb * QT + t] = a;
+        }
+        __syncthreads();
+    }
+
+    int tile_byte = 0;
+    if (tiles) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m = fmaxf(m, finite_abs(v[i][k]));
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+        if ((t & 63) == 0) wmax[t >> 6] = m;
+        __syncthreads();
+        tile_byte = exponent_byte<E5M2>(fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3])));
+        // pad bytes of the last word stand for 1
+        if (s != nullptr && t == 0) {
+            s[rb * s_ld + cb] = (uint8_t)tile_byte;
+            if (cb == col_blocks - 1)
+                for (int64_t p = col_blocks; p < s_ld; ++p) s[rb * s_ld + p] = 127;
+        }
+        if (st != nullptr && t == 0) {
+            st[(int64_t)cb * st_ld + rb] = (uint8_t)tile_byte;
+            if (rb == row_blocks - 1)
+                for (int64_t p = row_blocks; p < st_ld; ++p) st[(int64_t)cb * st_ld + p] = 127;
+        }
+    }
+
+    if (q != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            int byte = tile_byte;
+            if (!tiles) {
+                float m = fmaxf(fmaxf(finite_abs(v[i][0]), finite_abs(v[i][1])),
+                                fmaxf(finite_abs(v[i][2]), finite_abs(v[i][3])));
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+                byte = exponent_byte<E5M2>(m);
+            }
+            if (r0 + i < rows) {
+                const float inv = inverse_scale(byte);
+                *(uint32_t*)(q + (r0 + i) * ((int64_t)col_blocks * QT) + c0) =
+                    pack4<E5M2>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+                if (!tiles && c4 == 0) {
+                    s[(r0 + i) * s_ld + cb] = (uint8_t)byte;
+                    if (cb == col_blocks - 1)
+                        for (int64_t p = col_blocks; p < s_ld; ++p) s[(r0 + i) * s_ld + p] = 127;
+                }
+            }
+        }
+    }
+
+    if (qt != nullptr) {
+        float inv[4];
+        if (tiles) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) inv[k] = inverse_scale(tile_byte);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float m = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, finite_abs(v[i][k]));
+                part[rg][c4 * 4 + k] = m;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float m = part[0][c4 * 4 + k];
+#pragma unroll
+                for (int g = 1; g < 8; ++g) m = fmaxf(m, part[g][c4 * 4 + k]);
+                const int byte = exponent_byte<E5M2>(m);
+                inv[k] = inverse_scale(byte);
+                if (rg == 0 && c0 + k < cols) {
+                    st[(c0 + k) * st_ld + rb] = (uint8_t)byte;
+                    if (rb == row_blocks - 1)
+                        for (int64_t p = row_blocks; p < st_ld; ++p) st[(c0 + k) * st_ld + p] = 127;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[j] = pack4<E5M2>(v[4 * j][k] * inv[k], v[4 * j + 1][k] * inv[k], v[4 * j + 2][k] * inv[k],
+                                   v[4 * j + 3][k] * inv[k]);
+            *(u32x4*)(tr + (c4 * 4 + k) * QSTRIDE + rg * 16) = w;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // 8 lanes a column: 128 contiguous bytes of the transpose
+            const int c = j * 32 + (t >> 3), piece = t & 7;
+            if ((int64_t)cb * QT + c < cols)
+                *(u32x4*)(qt + ((int64_t)cb * QT + c) * (row_blocks * QT) + rb * QT + piece * 16) =
+                    *(const u32x4*)(tr + c * QSTRIDE + piece * 16);
+        }
+    }
+}
+
+// out[c] = sum_b colsum[b][c] in order, in 64 bits: 4 row groups a workgroup, joined in a fixed order
+__global__ __launch_bounds__(256) void colsum_kernel(const float* __restrict__ colsum, int64_t blocks, int64_t cols,
+                                                     float* __restrict__ out) {
+    __shared__ double red[4][64];
+    const int t = threadIdx.x, g = t >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + (t & 63);
+    double a = 0.0;
+    if (c < cols)
+        for (int64_t b = g; b < blocks; b += 4) a += (double)colsum[b * cols + c];
+    red[g][t & 63] = a;
+    __syncthreads();
+    if (g == 0 && c < cols) out[c] = (float)((red[0][t] + red[1][t]) + (red[2][t] + red[3][t]));
+}
+
+}  // namespace
+
+void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
+    const int64_t col_blocks = fp8_blocks(a.cols), grid = fp8_blocks(a.rows) * col_blocks;
+    const int64_t size = a.type == FP8_F32 ? 4 : 2;
+    const int vec = ((uintptr_t)a.x % (4 * size)) == 0 && a.ld % 4 == 0;
+#define SIREN_QUANT(T, E)                                                                                       \
+    hipLaunchKernelGGL((quant_kernel<T, E>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
+                       a.cols, (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, vec, (int)col_blocks)
+    if (a.e5m2) {
+        if (a.type == FP8_F32) SIREN_QUANT(float, true);
+        if (a.type == FP8_BF16) SIREN_QUANT(__bf16, true);
+        if (a.type == FP8_F16) SIREN_QUANT(_Float16, true);
+    } else {
+        if (a.type == FP8_F32) SIREN_QUANT(float, false);
+        if (a.type == FP8_BF16) SIREN_QUANT(__bf16, false);
+        if (a.type == FP8_F16) SIREN_QUANT(_Float16, false);
+    }
+#undef SIREN_QUANT
+}
+
+void launch_fp8_colsum(hipStream_t stream, const float* colsum, int64_t blocks, int64_t cols, float* out) {
+    hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, stream, colsum, blocks, cols, out);
+}
+
+}  // namespace siren

@@ -5,8 +5,12 @@ The parameters are re-seated as views of a flat fp32 buffer (state-dict order), 
 flat gradient buffer that zero_grad() clears in place, so autograd accumulates straight into the bucket and the
 step reads it without a gather. Semantics: torch.optim.Adam (amsgrad off, weight_decay 0, maximize off) after
 torch.nn.utils.clip_grad_norm_(params, max_norm) when max_norm is set.
+
+adamw_step / FusedAdamW: clip_grad_norm_ + torch.optim.AdamW.step over a list of tensors where they lie (siren_adamw_step,
+tu_adamw.hip), with the moments in 32 bits or in 8 with a scale for each block of 128.
 """
 import ctypes
+import math
 
 import torch
 
@@ -103,3 +107,152 @@ class FusedAdam:
     def grad_norm(self):
         """The pre-clip global gradient norm of the last clipped step (device tensor; no host sync)."""
         return self.scratch[1024]
+
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _state_size(params):
+    return sum((p.numel() + 127) // 128 * 128 for p in params)
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               max_norm=None, seed=0, scales=None):
+    """One AdamW step (torch.optim.AdamW: decoupled weight decay, amsgrad and maximize off) over all tensors at once,
+    after torch.nn.utils.clip_grad_norm_(max_norm) when max_norm is set. Everything is updated in place; nothing
+    synchronises with the host, and a captured step advances by itself on every replay (lr and the rest are captured).
+
+    params, grads: lists of tensors, fp32, bf16 or fp16, each gradient of its parameter's type and shape; a gradient may
+    be None (the tensor and its state stay as they are). Parameters are contiguous and do not overlap.
+    exp_avg, exp_avg_sq: flat states, each tensor's padded to a multiple of 128: fp32, or with scales (two uint8 tensors,
+    one byte per 128 elements) torch.float8_e4m3fn: exp_avg holds m, exp_avg_sq holds sqrt(v), value * 2^(byte - 127). The
+    8-bit states are rounded up or down at random, from (seed, step, element): the same call gives the same result.
+    step: int64, one element, on the device: the steps done so far; 1 is added.
+
+    Returns the gradients' norm before clipping (a device tensor), or None without max_norm."""
+    params, grads = list(params), list(grads)
+    if not params or len(params) != len(grads):
+        raise ValueError('adamw_step needs as many gradients as parameters, one at least; got %d and %d'
+                         % (len(params), len(grads)))
+    dev = params[0].device
+    if dev.type != 'cuda':
+        raise RuntimeError('adamw_step runs on ROCm devices (MI355X) only; got a %s tensor' % dev.type)
+    n = len(params)
+    ps, gs = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)()
+    numels, types = (ctypes.c_int64 * n)(), (ctypes.c_int32 * n)()
+    spans, keep, size = [], [], 0
+    for i, (p, g) in enumerate(zip(params, grads)):
+        code = _DTYPES.get(p.dtype)
+        if code is None or p.device != dev:
+            raise RuntimeError('adamw_step needs fp32, bf16 or fp16 parameters on one device; got %s on %s'
+                               % (p.dtype, p.device))
+        if not p.is_contiguous():
+            raise ValueError('adamw_step needs contiguous parameters; parameter %d has strides %s' % (i, p.stride()))
+        k = p.numel()
+        if g is not None:
+            if g.shape != p.shape or g.dtype != p.dtype or g.device != dev or g.layout != torch.strided:
+                raise ValueError('gradient %d must be %s %s on %s; got %s %s on %s'
+                                 % (i, tuple(p.shape), p.dtype, dev, tuple(g.shape), g.dtype, g.device))
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)
+            gs[i] = g.data_ptr()
+        at = p.data_ptr()
+        ps[i], numels[i], types[i] = at, k, code
+        if k:
+            spans.append((at, at + k * p.element_size()))
+        size += (k + 127) // 128 * 128
+    spans.sort()
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError('adamw_step: parameters overlap (is one listed twice?)')
+    bits = 32 if scales is None else 8
+    want = torch.float32 if scales is None else torch.float8_e4m3fn
+    for name, t in (('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq)):
+        if t.dtype != want or t.numel() != size or t.device != dev or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError('%s must be %d contiguous 16-byte aligned values of %s on %s; got %d of %s on %s'
+                             % (name, size, want, dev, t.numel(), t.dtype, t.device))
+    sm, sv = (None, None) if scales is None else scales
+    if scales is not None:
+        for t in scales:
+            if t.dtype != torch.uint8 or t.numel() != size // 128 or t.device != dev or not t.is_contiguous():
+                raise ValueError('scales must be two tensors of %d contiguous uint8 on %s' % (size // 128, dev))
+    if step.dtype != torch.int64 or step.numel() != 1 or step.device != dev:
+        raise ValueError('step must be one int64 on %s' % dev)
+    if max_norm is not None and not float(max_norm) > 0.:
+        raise ValueError('max_norm must be positive or None; got %r' % (max_norm,))
+    if not (0. <= betas[0] < 1. and 0. <= betas[1] < 1. and eps >= 0. and math.isfinite(lr) and math.isfinite(weight_decay)):
+        raise ValueError('need 0 <= betas < 1, eps >= 0 and finite lr and weight_decay')
+    lib, need = _lib.load(), ctypes.c_int64()
+    _lib.check(lib.siren_adamw_scratch_bytes(n, ctypes.byref(need)), 'siren_adamw_scratch_bytes')
+    scratch = torch.empty(need.value // 4, device=dev)
+    with torch.cuda.device(dev):
+        st = torch.cuda.current_stream(dev).cuda_stream
+        _lib.check(lib.siren_adamw_step(n, ps, gs, numels, types, bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+                                        sm.data_ptr() if sm is not None else None, sv.data_ptr() if sv is not None else None,
+                                        step.data_ptr(), lr, betas[0], betas[1], eps, weight_decay,
+                                        0. if max_norm is None else float(max_norm), seed & 0xFFFFFFFFFFFFFFFF,
+                                        scratch.data_ptr(), st), 'siren_adamw_step')
+    return None if max_norm is None else scratch[8]
+
+
+class FusedAdamW:
+    """AdamW over parameters where they lie (any mix of fp32, bf16, fp16; .grad may be replaced freely), two launches a
+    step. state_bits 8 keeps the moments in 8 bits (2 bytes a parameter instead of 8), rounded at random from seed."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32,
+                 seed=0):
+        self.params = [p for p in params]
+        if not self.params:
+            raise ValueError('FusedAdamW got an empty parameter list')
+        dev = self.params[0].device
+        if dev.type != 'cuda' or any(p.device != dev or p.dtype not in _DTYPES for p in self.params):
+            raise RuntimeError('FusedAdamW needs fp32, bf16 or fp16 parameters on one ROCm device')
+        if state_bits not in (8, 32):
+            raise ValueError('state_bits must be 8 or 32; got %r' % (state_bits,))
+        _lib.load()
+        self.lr, self.betas, self.eps, self.weight_decay = float(lr), tuple(betas), float(eps), float(weight_decay)
+        self.max_norm, self.state_bits, self.seed = max_norm, state_bits, int(seed)
+        n = _state_size(self.params)
+        dtype = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        self.exp_avg = torch.zeros(n, device=dev).to(dtype)
+        self.exp_avg_sq = torch.zeros(n, device=dev).to(dtype)
+        # byte 1 is the scale of a block of zeros
+        self.scales = None if state_bits == 32 else tuple(torch.ones(n // 128, dtype=torch.uint8, device=dev)
+                                                          for _ in range(2))
+        self.steps = torch.zeros(1, dtype=torch.int64, device=dev)
+        self._norm = None
+
+    def zero_grad(self, set_to_none=True):
+        for p in self.params:
+            if set_to_none:
+                p.grad = None
+            elif p.grad is not None:
+                p.grad.detach_().zero_()
+
+    @torch.no_grad()
+    def step(self):
+        self._norm = adamw_step(self.params, [p.grad for p in self.params], self.exp_avg, self.exp_avg_sq, self.steps,
+                                lr=self.lr, betas=self.betas, eps=self.eps, weight_decay=self.weight_decay,
+                                max_norm=self.max_norm or None, seed=self.seed, scales=self.scales)
+
+    def grad_norm(self):
+        """The pre-clip global gradient norm of the last clipped step (device tensor; no host sync)."""
+        return self._norm
+
+    def state_dict(self):
+        """The state's own tensors (8-bit ones as they are held): clone what must outlive the next step."""
+        out = {'state_bits': self.state_bits, 'seed': self.seed, 'steps': self.steps, 'exp_avg': self.exp_avg,
+               'exp_avg_sq': self.exp_avg_sq}
+        if self.scales is not None:
+            out['exp_avg_scale'], out['exp_avg_sq_scale'] = self.scales
+        return out
+
+    def load_state_dict(self, state):
+        if state['state_bits'] != self.state_bits or state['exp_avg'].numel() != self.exp_avg.numel():
+            raise ValueError('a state of %d bits and %d values does not fit this optimiser\'s %d bits and %d values'
+                             % (state['state_bits'], state['exp_avg'].numel(), self.state_bits, self.exp_avg.numel()))
+        self.seed = int(state['seed'])
+        mine = self.state_dict()
+        for k, t in mine.items():
+            if isinstance(t, torch.Tensor):
+                t.copy_(state[k])

@@ -1,0 +1,398 @@
+"""The 8-bit layer products (siren_amd.fp8) against a 64-bit restatement of their definition: the quantiser's bytes
+exactly, products within the rounding of a 32-bit sum, gradients from the quantised operands and against differences of
+the layer itself. Needs an MI355X."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
+
+
+# ---- the definition, in 64 bits on the CPU -----------------------------------------------------------------------------
+def grid(top, mant, emin):
+    """A format as (largest value, mantissa bits, exponent of the smallest normal number)."""
+    return top, mant, emin
+
+
+FORMATS = {E4M3: grid(448., 3, -6), E5M2: grid(57344., 2, -14)}
+
+
+def round_blocks(v, fmt):
+    """(values that 8 bits hold, exponent bytes) of the blocks along v's last axis (numpy float64)."""
+    top, mant, emin = FORMATS[fmt]
+    fin = np.where(np.isfinite(v), np.abs(v), 0.).max(-1, keepdims=True)
+    f, e = np.frexp(fin / top)
+    e = np.where(f > 0, np.maximum(np.where(f > 0.5, e, e - 1), -126), -126)
+    s = np.ldexp(1., e)
+    with np.errstate(invalid='ignore'):
+        u = v / s
+        step = np.ldexp(1., np.maximum(np.frexp(np.where(np.isfinite(u), u, 0.))[1] - 1, emin) - mant)
+        out = np.rint(u / step) * step * s
+    if fmt is E4M3:
+        out = np.where(np.isfinite(v), out, np.nan)
+    return out, (e + 127)[..., 0].astype(np.int64)
+
+
+def held(x, fmt=E4M3, tiles=False):
+    """(rows, cols) -> (values, bytes) quantised along the columns."""
+    x = np.asarray(x, np.float64)
+    r, c = x.shape
+    pc, pr = -c % 128, -r % 128
+    if not tiles:
+        v, b = round_blocks(np.pad(x, ((0, 0), (0, pc))).reshape(r, -1, 128), fmt)
+        return v.reshape(r, -1)[:, :c], b
+    t = np.pad(x, ((0, pr), (0, pc)))
+    nb, kb = t.shape[0] // 128, t.shape[1] // 128
+    v, b = round_blocks(t.reshape(nb, 128, kb, 128).transpose(0, 2, 1, 3).reshape(nb, kb, -1), fmt)
+    return v.reshape(nb, kb, 128, 128).transpose(0, 2, 1, 3).reshape(nb * 128, -1)[:r, :c], b
+
+
+def np64(t):
+    return t.detach().double().cpu().numpy()
+
+
+HALF = {torch.float32: 2. ** -24, torch.bfloat16: 2. ** -8, torch.float16: 2. ** -11}
+TINY = {torch.float32: 2. ** -149, torch.bfloat16: 2. ** -133, torch.float16: 2. ** -25}
+
+
+def product_tol(a, b, out, dtype, extra=0.):
+    """A sum of k exact products and a bias in 32 bits, in any order: at most (k + 2) roundings of half a step, each of at
+    most the sum of magnitudes; then one rounding to dtype."""
+    k = a.shape[1]
+    return (k + 2) * 2. ** -24 * (np.abs(a) @ np.abs(b).T + extra) + HALF[dtype] * np.abs(out) + TINY[dtype]
+
+
+def check(got, want, tol, what):
+    got = np64(got)
+    assert got.shape == want.shape, what
+    bad = np.abs(got - want) > tol
+    assert not bad.any(), '%s: %d of %d off, worst %.3g of its tolerance' % (
+        what, bad.sum(), bad.size, (np.abs(got - want) / tol).max())
+
+
+def values(shape, seed, scale=1.):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g) * torch.exp(torch.randn(shape[0], 1, generator=g)) * scale
+
+
+# ---- the quantiser -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('rows,cols', [(1, 1), (1, 128), (3, 100), (128, 129), (130, 640), (257, 1025)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('block', ['row', 'tile'])
+@pytest.mark.parametrize('fmt', [E4M3, E5M2])
+def test_quantize_is_the_definition(cuda, rows, cols, dtype, block, fmt):
+    from siren_amd import fp8
+    x = values((rows, cols), rows * 7 + cols).to(dtype)
+    b = fp8.quantize(x.to(cuda), block, fmt)
+    want, byte = held(np64(x), fmt, block == 'tile')
+    assert b.data.dtype == fmt and b.data.shape == (rows, (cols + 127) // 128 * 128)
+    assert b.scale.shape == (((rows + 127) // 128 if block == 'tile' else rows), (cols + 511) // 512 * 4)
+    kb = (cols + 127) // 128
+    assert np.array_equal(b.scale.cpu().numpy()[:, :kb], byte)
+    assert (b.scale[:, kb:] == 127).all() and (b.data[:, cols:].float() == 0).all()
+    assert np.array_equal(np64(fp8.dequantize(b)), want)
+    assert b.tiled == (block == 'tile' and rows > 1)
+
+
+def test_quantize_special_values(cuda):
+    """Zeros, subnormals, the format's borders and values that are not finite, in blocks of their own."""
+    from siren_amd import fp8
+    x = torch.zeros(8, 256)
+    x[1, :3] = torch.tensor([448., 449., -1.])
+    x[2, :4] = torch.tensor([float('inf'), 1., float('-inf'), float('nan')])
+    x[3, 0], x[3, 1] = 2. ** -149, -2. ** -126
+    x[4, 0], x[4, 1] = torch.finfo(torch.float32).max, 1.
+    x[5, :] = float('nan')
+    x[6, :128] = torch.arange(128) * 2. ** -9
+    x[7, :2] = torch.tensor([-0., 2. ** -120])
+    for fmt in (E4M3, E5M2):
+        b = fp8.quantize(x.to(cuda), 'row', fmt)
+        want, byte = held(x.double().numpy(), fmt)
+        assert np.array_equal(b.scale.cpu().numpy()[:, :2], byte)
+        # the largest fp32 number, 2^128 (1 - 2^-24), rounds to 2^128, which fp32 values hold as an infinity only
+        with np.errstate(over='ignore'):
+            want = want.astype(np.float32).astype(np.float64)
+        assert np.array_equal(np64(fp8.dequantize(b)), want, equal_nan=True)
+
+
+@pytest.mark.parametrize('rows,cols', [(1, 130), (200, 70), (128, 128), (129, 1)])
+@pytest.mark.parametrize('tiles', [False, True])
+def test_both_directions_in_one_pass(cuda, rows, cols, tiles):
+    """The transpose is the quantised transpose; the column sums are the unrounded ones'; mult multiplies first."""
+    from siren_amd import fp8
+    x = values((rows, cols), 5)
+    mult = values((rows, cols), 6).bfloat16()
+    q, qt, sums = fp8._quantize(x.to(cuda), tiles, transposed=True, mult=mult.to(cuda), colsum=True)
+    y = (x * mult.float()).numpy()
+    for b, v in ((q, y), (qt, y.T)):
+        want, byte = held(v, E4M3, tiles)
+        assert np.array_equal(np64(fp8.dequantize(fp8.Blocks(b.data, b.scale, v.shape[1]))), want)
+        assert np.array_equal(b.scale.cpu().numpy()[:, :byte.shape[1]], byte)
+    # 128 values of a row block are added in 32 bits: 15 roundings in a thread, 7 across; the blocks in 64
+    y = y.astype(np.float64)
+    check(sums, y.sum(0), 23 * 2. ** -24 * np.abs(y).sum(0) + 2. ** -24 * np.abs(y.sum(0)) + 2. ** -149, 'column sums')
+
+
+@pytest.mark.parametrize('view', ['strided', 'offset', 'transposed', 'expanded', 'wide'])
+def test_quantize_reads_views(cuda, view):
+    from siren_amd import fp8
+    base = values((300, 400), 9).to(cuda)
+    x = {'strided': base[:, ::2], 'offset': base[1:, 3:200], 'transposed': base.t(), 'expanded': base[:1].expand(9, 400),
+         'wide': base[::3]}[view]
+    assert np.array_equal(np64(fp8.dequantize(fp8.quantize(x))), held(np64(x))[0])
+
+
+# ---- the forward -------------------------------------------------------------------------------------------------------
+def layer(m, k, n, dtype, cuda, seed=0):
+    x = torch.sin(values((m, k), seed)).to(dtype)
+    g = torch.Generator().manual_seed(seed + 1)
+    w = (torch.rand(n, k, generator=g) * 2 - 1) * math.sqrt(6 / k) / 30
+    b = (torch.rand(n, generator=g) * 2 - 1) / math.sqrt(k)
+    return x.to(cuda), w.to(cuda), b.to(cuda)
+
+
+SIZES = [(1, 1, 1), (1, 256, 512), (2, 128, 128), (3, 100, 257), (15, 257, 130), (17, 64, 1), (32, 256, 1024), (33, 1024, 320),
+         (129, 4096, 65), (130, 129, 127), (300, 640, 385), (1000, 384, 513)]
+
+
+@pytest.mark.parametrize('m,k,n', SIZES)
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('act', [None, 'sine'])
+def test_linear_forward(cuda, m, k, n, dtype, act):
+    from siren_amd import fp8
+    x, w, b = layer(m, k, n, dtype, cuda, m + k + n)
+    y = fp8.linear(x, fp8.quantize(w, 'tile'), b, activation=act)
+    assert y.dtype == dtype and y.shape == (m, n)
+    xq, wq = held(np64(x))[0], held(np64(w), tiles=True)[0]
+    z = xq @ wq.T + np64(b)
+    if act is None:
+        check(y, z, product_tol(xq, wq, z, dtype, np.abs(np64(b))), 'y')
+    else:  # the phase is rounded once more, the sine to 2^-22
+        tol = 30 * product_tol(xq, wq, 0 * z, torch.float32, np.abs(np64(b))) + np.abs(30 * z) * 2. ** -23 + 2. ** -22
+        check(y, np.sin(30 * z), tol + HALF[dtype] * np.abs(np.sin(30 * z)) + TINY[dtype], 'sin')
+    assert torch.equal(y, fp8.linear(x, w, b, activation=act)), 'a weight quantised on the way is the same'
+    assert torch.equal(y, fp8.linear(x, fp8.quantize(w, 'tile'), b, activation=act)), 'the same call, the same result'
+
+
+def test_linear_shapes_bias_and_omega(cuda):
+    from siren_amd import fp8
+    x, w, b = layer(60, 96, 40, torch.float32, cuda)
+    w8 = fp8.quantize(w, 'tile')
+    y = fp8.linear(x, w8, b, 'sine', omega=7.)
+    assert torch.equal(fp8.linear(x.view(3, 4, 5, 96), w8, b, 'sine', omega=7.).view(60, 40), y)
+    assert torch.equal(fp8.linear(x[7], w8, b, 'sine', omega=7.), y[7])
+    assert fp8.linear(x[:0], w8, b).shape == (0, 40)
+    z = fp8.linear(x, w8)
+    assert torch.allclose(torch.sin(7 * (z + b)), y, atol=1e-5)
+    assert torch.equal(fp8.linear(x, w8, b.bfloat16()), fp8.linear(x, w8, b.bfloat16().float()))
+    strided = torch.empty(60, 200, device=cuda)[:, 3:99].copy_(x)
+    assert torch.equal(fp8.linear(strided, w8, b, 'sine', omega=7.), y)
+
+
+def test_linear_not_finite(cuda):
+    """A NaN or an infinity spoils its own row of y and no other."""
+    from siren_amd import fp8
+    x, w, b = layer(40, 300, 200, torch.float32, cuda)
+    y = fp8.linear(x, w, b)
+    x[3, 7], x[20, 299] = float('nan'), float('inf')
+    z = fp8.linear(x, w, b)
+    keep = torch.ones(40, dtype=torch.bool, device=cuda)
+    keep[3] = keep[20] = False
+    assert torch.isnan(z[~keep]).all() and torch.equal(z[keep], y[keep])
+
+
+# ---- gradients ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('m,k,n', [(1, 1, 1), (1, 256, 300), (32, 256, 1024), (33, 130, 64), (129, 257, 130), (1500, 192, 320)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('fmt', [E4M3, E5M2])
+def test_linear_gradients(cuda, m, k, n, dtype, fmt):
+    """dx, dW and db are the products of the operands as 8 bits hold them."""
+    from siren_amd import fp8
+    x, w, b = layer(m, k, n, dtype, cuda, 3)
+    dy = values((m, n), 4, 1 / 64).to(dtype).to(cuda)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = fp8.linear(x, w, b, grad_dtype=fmt)
+    with torch.no_grad():
+        assert torch.equal(y, fp8.linear(x, w, b))
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    assert dx.dtype == dtype and dw.dtype == torch.float32 and db.dtype == torch.float32
+    d = np64(dy)
+    wq, dq = held(np64(w), tiles=True)[0], held(d, fmt)[0]
+    check(dx, dq @ wq, product_tol(dq, wq.T, dq @ wq, dtype), 'dx')
+    dqt, xqt = held(d.T, fmt)[0], held(np64(x).T)[0]
+    check(dw, dqt @ xqt.T, product_tol(dqt, xqt, dqt @ xqt.T, torch.float32), 'dw')
+    check(db, d.sum(0), 24 * 2. ** -24 * np.abs(d).sum(0) + 2. ** -149, 'db')
+    # one gradient at a time is the same gradient
+    for i, g in enumerate((dx, dw, db)):
+        ts = [t.detach().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        assert torch.equal(torch.autograd.grad(fp8.linear(*ts, grad_dtype=fmt), ts[i], dy)[0], g)
+
+
+def test_sine_gradients(cuda):
+    """The sine's gradient is dy omega cos(omega z), the cosine held in bf16, then the linear layer's."""
+    from siren_amd import fp8
+    m, k, n = 200, 192, 260
+    x, w, b = layer(m, k, n, torch.float32, cuda, 8)
+    dy = values((m, n), 4, 1 / 64).to(cuda)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(fp8.linear(x, w, b, 'sine'), leaves, dy)
+    xq, wq = held(np64(x))[0], held(np64(w), tiles=True)[0]
+    z = xq @ wq.T + np64(b)
+    _, deriv = fp8._product(fp8.quantize(x), fp8.quantize(w, 'tile'), b.detach(), 1, 30., torch.float32, deriv=True)
+    tol = 30 * (30 * product_tol(xq, wq, 0 * z, torch.float32, np.abs(np64(b))) + np.abs(30 * z) * 2. ** -23 + 2. ** -22)
+    check(deriv, 30 * np.cos(30 * z), tol + 2. ** -8 * np.abs(30 * np.cos(30 * z)), 'derivative')
+    g = (dy * deriv.float()).cpu().double().numpy()
+    gq, gqt, xqt = held(g)[0], held(g.T)[0], held(np64(x).T)[0]
+    check(dx, gq @ wq, product_tol(gq, wq.T, gq @ wq, torch.float32), 'dx')
+    check(dw, gqt @ xqt.T, product_tol(gqt, xqt, gqt @ xqt.T, torch.float32), 'dw')
+    check(db, g.sum(0), 24 * 2. ** -24 * np.abs(g).sum(0) + 2. ** -149, 'db')
+
+
+@pytest.mark.parametrize('act', [None, 'sine'])
+def test_gradients_against_differences(cuda, act):
+    """Along random directions the gradients are those of the layer without 8 bits (central differences in 64), up to what
+    rounding each operand can do: an e4m3 value is off by 2^-4 of itself or 2^-10 of its block's scale, at most
+    2 amax / 448; a bf16 cosine by 2^-8; the phase's error moves the sine's own derivative by omega^2 |dz|."""
+    from siren_amd import fp8
+    m, k, n = 24, 140, 150
+    x, w, b = layer(m, k, n, torch.float32, cuda, 21)
+    dy = values((m, n), 22, 1 / 8).to(cuda)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    got = [np64(g) for g in torch.autograd.grad(fp8.linear(x, w, b, act), leaves, dy)]
+    X, W, B, D = (np64(t) for t in (x, w, b, dy))
+
+    def off(a):
+        return 2. ** -4 * np.abs(a) + 2. ** -10 * np.abs(a).max() / 224
+
+    z = X @ W.T + B
+    dz = off(X) @ np.abs(W).T + np.abs(X) @ off(W).T + off(X) @ off(W).T + 1e-5
+    if act == 'sine':
+        G = D * 30 * np.cos(30 * z)
+        eg = np.abs(D) * (30 * np.minimum(30 * dz, 2.) + 30 * 2. ** -8)
+    else:
+        G, eg = D, 0 * D
+    eq = eg + 2. ** -4 * (np.abs(G) + eg) + 2. ** -10 * (np.abs(G) + eg).max() / 224
+    tols = [eq @ np.abs(W) + np.abs(G) @ off(W) + eq @ off(W), eq.T @ np.abs(X) + np.abs(G).T @ off(X) + eq.T @ off(X), eg.sum(0)]
+
+    def loss(X, W, B):
+        y = X @ W.T + B
+        return (D * (np.sin(30 * y) if act == 'sine' else y)).sum()
+
+    rng = np.random.default_rng(0)
+    for i, (g, t) in enumerate(zip(got, tols)):
+        for _ in range(4):
+            v = rng.normal(size=g.shape)
+            h = 1e-5
+            lo, hi = [X, W, B], [X, W, B]
+            lo[i], hi[i] = lo[i] - h * v, hi[i] + h * v
+            diff = (loss(*hi) - loss(*lo)) / (2 * h)
+            bound = (t * np.abs(v)).sum() + 1e-4 * np.abs(diff) + 1e-6 * np.abs(G).sum()
+            assert abs((g * v).sum() - diff) <= bound, (i, (g * v).sum(), diff, bound)
+
+
+def test_empty_batch_and_broadcast_gradient(cuda):
+    from siren_amd import fp8
+    x, w, b = layer(9, 40, 30, torch.float32, cuda)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(fp8.linear(x[:0], w, b).sum(), leaves)
+    assert not dx.any() and not dw.any() and not db.any()
+    one = torch.autograd.grad(fp8.linear(x, w, b).sum(), leaves)  # dy is one number, expanded
+    two = torch.autograd.grad(fp8.linear(x, w, b), leaves, torch.ones(9, 30, device=cuda))
+    assert all(torch.equal(p, q) for p, q in zip(one, two))
+    shared = fp8.linear(x, w, b) + fp8.linear(x * 2, w, b)  # a weight used twice: its gradients add
+    dw2, = torch.autograd.grad(shared, w, torch.ones(9, 30, device=cuda))
+    assert torch.allclose(dw2, 3 * two[1], rtol=0.2, atol=1e-3)
+
+
+def test_second_derivatives_and_packed_gradients_are_refused(cuda):
+    from siren_amd import fp8
+    x, w, b = layer(9, 40, 30, torch.float32, cuda)
+    w8 = fp8.quantize(w, 'tile')
+    x.requires_grad_(True)
+    with pytest.raises(RuntimeError, match='forward only'):
+        fp8.linear(x, w8, b)
+    with torch.no_grad():
+        fp8.linear(x, w8, b)
+    g, = torch.autograd.grad(fp8.linear(x, w, b).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+# ---- streams, graphs, long offsets -------------------------------------------------------------------------------------
+def test_streams_and_graphs(cuda):
+    """Calls on a side stream and captured calls replayed on new inputs; two graphs share nothing."""
+    from siren_amd import fp8
+    x, w, b = layer(70, 1100, 200, torch.float32, cuda)
+    w8 = fp8.quantize(w, 'tile')
+    want = [fp8.linear(x * s, w8, b, 'sine') for s in (1., 0.5, 0.25)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(fp8.linear(x, w8, b, 'sine'), want[0])
+    torch.cuda.synchronize()
+    graphs, ins, outs = [], [], []
+    for s in (1., 0.5):
+        xin = (x * s).clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = fp8.linear(xin, w8, b, 'sine')
+        graphs.append(g), ins.append(xin), outs.append(y)
+    for _ in range(3):
+        graphs[0].replay(), graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+        torch.randn(1000, device=cuda).sum().item()
+    ins[0].copy_(x * 0.25)
+    graphs[0].replay()
+    assert torch.equal(outs[0], want[2])
+
+
+def test_captured_training_step(cuda):
+    from siren_amd import fp8
+    x, w, b = layer(260, 300, 140, torch.float32, cuda)
+    dy = values((260, 140), 2).to(cuda)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(fp8.linear(x, w, b, 'sine'), leaves, dy)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(fp8.linear(x, w, b, 'sine'), leaves, dy)
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+def test_offsets_past_32_bits(cuda):
+    """Rows whose bytes, and outputs whose elements, begin past 2^32."""
+    from siren_amd import fp8
+    m, k, n = (1 << 21) + 3, 260, 2100
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=cuda)
+    g = torch.Generator(device='cuda').manual_seed(0)
+    some = torch.cat([torch.arange(5), torch.tensor([m // 2]), torch.arange(m - 200, m)]).to(cuda)
+    x[some] = torch.randn(some.numel(), k, generator=g, device=cuda).bfloat16()
+    w8 = fp8.quantize(torch.randn(n, k, generator=g, device=cuda), 'tile')
+    assert m * n > 1 << 32
+    y = fp8.linear(x, w8)
+    assert torch.equal(y[some], fp8.linear(x[some], w8))
+    assert not y[1000:2000].any()
+
+
+# ---- in the modules ----------------------------------------------------------------------------------------------------
+def test_rows_of_a_batch_do_not_depend_on_it(cuda):
+    """One row, a few and many take different kernels; a row's result may differ by the order of its sums only."""
+    from siren_amd import fp8
+    x, w, b = layer(700, 1000, 300, torch.float32, cuda)
+    w8 = fp8.quantize(w, 'tile')
+    y = fp8.linear(x, w8, b)
+    xq, wq = held(np64(x))[0], held(np64(w), tiles=True)[0]
+    tol = 2 * product_tol(xq, wq, np64(y), torch.float32, np.abs(np64(b)))
+    for m in (1, 2, 5, 16, 17, 31, 32, 33, 64, 65, 128, 129, 257):
+        check(fp8.linear(x[:m], w8, b), np64(y)[:m], tol[:m], m)

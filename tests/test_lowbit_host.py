@@ -1,0 +1,109 @@
+"""Refusals of the 8-bit training entry points that need no GPU: the C ABI validates before any device work, and the Python
+entry points refuse CPU tensors and wrong arguments."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope='module')
+def lib():
+    import __graft_entry__
+    __graft_entry__.build()
+    from siren_amd import _lib
+    return _lib.load()
+
+
+P = ctypes.c_void_p
+OK, EINVAL = 0, 1
+
+
+def test_quantize_validates(lib):
+    def call(x=P(64), dtype=0, rows=4, cols=8, ld=8, mult=None, fmt=0, tiles=0, q=P(64), s=P(64), qt=None, st=None,
+             ws=None, sums=None):
+        return lib.siren_fp8_quantize(x, dtype, rows, cols, ld, mult, fmt, tiles, q, s, qt, st, ws, sums, None)
+    assert call(rows=0) == OK and call(cols=0, ld=0) == OK
+    for bad in (dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(cols=-1), dict(ld=7), dict(fmt=2), dict(s=None), dict(q=None),
+                dict(qt=P(64)), dict(st=P(64)), dict(sums=P(64)), dict(x=None), dict(q=None, s=None), dict(q=P(72)),
+                dict(x=P(66)), dict(dtype=1, x=P(65)), dict(qt=P(8), st=P(64)),
+                dict(rows=1 << 40, cols=1 << 30, ld=1 << 30)):
+        assert call(**bad) == EINVAL, bad
+        assert lib.siren_last_error()
+
+
+def test_products_validate(lib):
+    def call(a=P(64), sa=P(64), m=4, b=P(64), sb=P(64), n=4, k=8, bias=None, act=0, omega=30., out=P(64), dtype=0, deriv=None,
+             ws=None, fmt=0):
+        return lib.siren_fp8_matmul(a, sa, m, 0, fmt, b, sb, n, 1, k, bias, act, omega, out, dtype, deriv, ws, None)
+    assert call(m=0) == OK and call(n=0) == OK
+    for bad in (dict(m=-1), dict(n=-1), dict(k=0), dict(fmt=2), dict(act=2), dict(dtype=9), dict(a=None), dict(sa=None),
+                dict(b=None), dict(sb=None), dict(out=None), dict(a=P(8)), dict(b=P(8)), dict(sa=P(2)), dict(sb=P(2)),
+                dict(out=P(8)), dict(bias=P(2)), dict(deriv=P(64)), dict(act=1, omega=float('nan')),
+                dict(act=1, omega=float('inf')), dict(act=1, deriv=P(4)), dict(k=1 << 20), dict(m=1 << 40, n=1 << 40)):
+        assert call(**bad) == EINVAL, bad  # k = 2^20 with 4 x 4 outputs is split: it needs ws
+    c = ctypes.c_int64(-7)
+    for fn in (lib.siren_fp8_matmul_ws_bytes, lib.siren_fp8_linear_ws_bytes):
+        assert fn(4, 4, 0, ctypes.byref(c)) == EINVAL and fn(-1, 4, 4, ctypes.byref(c)) == EINVAL and c.value == -7
+        assert fn(4, 4, 4, None) == EINVAL
+        assert fn(0, 4, 4, ctypes.byref(c)) == OK and c.value == 0
+        c.value = -7
+    assert lib.siren_fp8_matmul_ws_bytes(1 << 18, 1024, 1024, ctypes.byref(c)) == OK and c.value == 0
+    assert lib.siren_fp8_matmul_ws_bytes(1024, 1024, 1 << 18, ctypes.byref(c)) == OK and c.value % (4 << 20) == 0 and c.value
+
+    def lin(x=P(64), m=4, k=8, ld=8, w=P(64), sw=P(64), n=4, y=P(64), ws=P(64)):
+        return lib.siren_fp8_linear(x, 0, m, k, ld, w, sw, n, None, 0, 30., y, ws, None)
+    assert lin(m=0) == OK and lin(n=0) == OK
+    for bad in (dict(m=-1), dict(k=0), dict(x=None), dict(w=None), dict(sw=None), dict(y=None), dict(ws=None), dict(ws=P(8)),
+                dict(w=P(4)), dict(sw=P(1)), dict(ld=3), dict(x=P(66)), dict(y=P(4))):
+        assert lin(**bad) == EINVAL, bad
+
+
+def test_adamw_validates(lib):
+    def call(count=1, p=64, g=64, n=5, dtype=0, bits=32, m=P(64), v=P(64), sm=None, sv=None, step=P(64), lr=1e-3, b1=.9, b2=.99,
+             eps=1e-8, wd=0., scratch=P(64), arrays=True):
+        ps, gs = (P * 1)(p), (P * 1)(g)
+        ns, ts = (ctypes.c_int64 * 1)(n), (ctypes.c_int32 * 1)(dtype)
+        a = (ps, gs, ns, ts) if arrays else (None,) * 4
+        return lib.siren_adamw_step(count, *a, bits, m, v, sm, sv, step, lr, b1, b2, eps, wd, 0., 0, scratch, None)
+    for bad in (dict(count=-1), dict(bits=16), dict(b1=1.), dict(b2=-.1), dict(eps=-1.), dict(eps=float('nan')),
+                dict(lr=float('inf')), dict(wd=float('nan')), dict(step=None), dict(step=P(4)), dict(scratch=None),
+                dict(arrays=False), dict(dtype=3), dict(n=-1), dict(p=None), dict(p=66), dict(g=66), dict(m=None), dict(v=None),
+                dict(m=P(8)), dict(bits=8), dict(bits=8, sm=P(64)), dict(n=1 << 45)):
+        assert call(**bad) == EINVAL, bad
+    c = ctypes.c_int64(-7)
+    assert lib.siren_adamw_scratch_bytes(-1, ctypes.byref(c)) == EINVAL and c.value == -7
+    assert lib.siren_adamw_scratch_bytes(1000, None) == EINVAL
+    assert lib.siren_adamw_scratch_bytes(1000, ctypes.byref(c)) == OK and c.value > 64
+
+
+def test_python_entry_points_refuse_the_cpu():
+    from siren_amd import fp8, optim
+    x, w = torch.zeros(2, 4), torch.zeros(3, 4)
+    with pytest.raises(RuntimeError, match='ROCm'):
+        fp8.linear(x, w)
+    with pytest.raises(RuntimeError, match='ROCm'):
+        fp8.quantize(x)
+    with pytest.raises(TypeError):
+        fp8.linear([1.], w)
+    with pytest.raises(RuntimeError, match='ROCm'):
+        optim.adamw_step([x], [x], x, x, x)
+    with pytest.raises(RuntimeError, match='ROCm'):
+        optim.FusedAdamW([x])
+    with pytest.raises(ValueError):
+        optim.FusedAdamW([])
+    with pytest.raises(ValueError):
+        optim.adamw_step([], [], x, x, x)
+
+
+def test_dequantize_is_the_layout():
+    """Blocks by hand: two rows of 200 columns, scales per row and per tile."""
+    from siren_amd import fp8
+    data = torch.zeros(2, 256)
+    data[0, :200], data[1, :200] = 1., -2.
+    data = data.to(torch.float8_e4m3fn)
+    row = torch.tensor([[127, 128, 127, 127], [126, 129, 127, 127]], dtype=torch.uint8)
+    got = fp8.dequantize(fp8.Blocks(data, row, 200))
+    want = torch.cat([torch.tensor([[1.], [-1.]]).expand(2, 128), torch.tensor([[2.], [-8.]]).expand(2, 72)], 1)
+    assert torch.equal(got, want)
+    tile = fp8.dequantize(fp8.Blocks(data, row[:1], 200))
+    assert torch.equal(tile, torch.cat([torch.tensor([[1.], [-2.]]).expand(2, 128), torch.tensor([[2.], [-4.]]).expand(2, 72)], 1))

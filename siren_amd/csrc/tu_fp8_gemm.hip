@@ -85,15 +85,28 @@ __device__ __forceinline__ void finish(const GemmArgs& g, int64_t row, int64_t c
             if (k < valid) v[k] += g.bias[col + k];
     }
     if (g.act == FP8_ACT_SINE) {
-        f32x4 d;
+        f32x4 t = v * g.omega;
+        const float top = fmaxf(fmaxf(__builtin_fabsf(t[0]), __builtin_fabsf(t[1])),
+                                fmaxf(__builtin_fabsf(t[2]), __builtin_fabsf(t[3])));
+        if (__builtin_expect(top > 1.0e5f, 0)) {  // past the reduction's exact range
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float sn, cs;
-            sincos_phase(g.omega * v[k], sn, cs);
-            v[k] = sn;
-            d[k] = g.omega * cs;
+            for (int k = 0; k < 4; ++k) v[k] = sinf(t[k]);
+            if (g.deriv != nullptr) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) t[k] = g.omega * cosf(t[k]);
+                put4(g.deriv + row * g.n + col, t, valid, vec);
+            }
+        } else {
+            f32x4 d;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float sn, cs;
+                sincos_fast(t[k], sn, cs);  // 4e-7; the cosine falls away where nothing takes it
+                v[k] = sn;
+                d[k] = g.omega * cs;
+            }
+            if (g.deriv != nullptr) put4(g.deriv + row * g.n + col, d, valid, vec);
         }
-        if (g.deriv != nullptr) put4(g.deriv + row * g.n + col, d, valid, vec);
     }
     put4((T*)g.out + row * g.n + col, v, valid, vec);
 }
@@ -216,24 +229,57 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
     }
 }
 
-// out = act(sum of the splits' partial products, in order, + bias), four columns a thread
-template <typename T>
+// out = act(sum of the splits' partial products + bias), four columns a thread. GROUPS threads share an element's splits,
+// each its own contiguous run of them, and are added in order: few outputs with many splits (a reduction over 65536)
+// would otherwise leave most of the card idle behind one long chain of loads (33 us for 32 x 256 of 128 splits).
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void join_kernel(GemmArgs g, const float* __restrict__ part, int splits) {
+    constexpr int QUADS = 256 / GROUPS;
+    __shared__ f32x4 red[GROUPS][QUADS];
     const int64_t n4 = (g.n + 3) / 4, total = g.m * n4, plane = g.m * g.n;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int grp = threadIdx.x / QUADS, at = threadIdx.x % QUADS;
+    const int per = (splits + GROUPS - 1) / GROUPS;
+    const int lo = grp * per, hi = lo + per < splits ? lo + per : splits;
+    for (int64_t base = (int64_t)blockIdx.x * QUADS; base < total; base += (int64_t)gridDim.x * QUADS) {
+        const int64_t i = base + at;
         const int64_t row = i / n4, col = (i - row * n4) * 4;
-        const float* src = part + row * g.n + col;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if ((g.n & 3) == 0) {
-            for (int s = 0; s < splits; ++s) v += *(const f32x4*)(src + s * plane);
-        } else {
-            for (int s = 0; s < splits; ++s)
+        if (i < total) {
+            const float* src = part + row * g.n + col;
+            if ((g.n & 3) == 0) {
+#pragma unroll 8
+                for (int s = lo; s < hi; ++s) v += *(const f32x4*)(src + s * plane);
+            } else {
+                for (int s = lo; s < hi; ++s)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (col + k < g.n) v[k] += src[s * plane + k];
+                    for (int k = 0; k < 4; ++k)
+                        if (col + k < g.n) v[k] += src[s * plane + k];
+            }
         }
-        finish<T>(g, row, col, v);
+        if (GROUPS > 1) {
+            red[grp][at] = v;
+            __syncthreads();
+            if (grp == 0) {
+#pragma unroll
+                for (int k = 1; k < GROUPS; ++k) v += red[k][at];
+            }
+            __syncthreads();
+        }
+        if (grp == 0 && i < total) finish<T>(g, row, col, v);
     }
+}
+
+template <typename T>
+void launch_join(hipStream_t stream, const GemmArgs& g, const void* part, int splits) {
+    const int64_t quads = g.m * ((g.n + 3) / 4);
+    // 8 waves a CU of one thread an element is 131072 elements; below that, threads share them
+    const bool share = quads < 131072 && splits >= 16;
+    const int64_t want = share ? (quads + 15) / 16 : (quads + 255) / 256;
+    const dim3 grid((unsigned)(want < 8192 ? want : 8192));
+    if (share)
+        hipLaunchKernelGGL((join_kernel<T, 16>), grid, dim3(256), 0, stream, g, (const float*)part, splits);
+    else
+        hipLaunchKernelGGL((join_kernel<T, 1>), grid, dim3(256), 0, stream, g, (const float*)part, splits);
 }
 
 // splits of the k axis: enough workgroups to fill 256 CUs twice, at least 4 steps each
@@ -283,11 +329,9 @@ void launch_fp8_product(hipStream_t stream, const Fp8Product& p) {
         else
             SIREN_GEMM(float, false, true);
         g.out = p.out;
-        const int64_t want = (g.m * ((g.n + 3) / 4) + 255) / 256;
-        const dim3 jgrid((unsigned)(want < 4096 ? want : 4096));
-        if (p.type == FP8_F32) hipLaunchKernelGGL(join_kernel<float>, jgrid, dim3(256), 0, stream, g, (const float*)p.ws, splits);
-        if (p.type == FP8_BF16) hipLaunchKernelGGL(join_kernel<__bf16>, jgrid, dim3(256), 0, stream, g, (const float*)p.ws, splits);
-        if (p.type == FP8_F16) hipLaunchKernelGGL(join_kernel<_Float16>, jgrid, dim3(256), 0, stream, g, (const float*)p.ws, splits);
+        if (p.type == FP8_F32) launch_join<float>(stream, g, p.ws, splits);
+        if (p.type == FP8_BF16) launch_join<__bf16>(stream, g, p.ws, splits);
+        if (p.type == FP8_F16) launch_join<_Float16>(stream, g, p.ws, splits);
         return;
     }
     if (p.e5m2_a) {

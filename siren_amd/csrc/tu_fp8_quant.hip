@@ -61,34 +61,49 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
     const int64_t row_blocks = (rows + QT - 1) / QT;
     const int64_t s_ld = (col_blocks + 3) / 4 * 4, st_ld = (row_blocks + 3) / 4 * 4;
 
+    // Every load is issued before any is waited for: rows past the end read the last row and are zeroed afterwards (a
+    // branch around each row's load made 16 round trips of them: 8 us for one row).
     f32x4 v[16];
+    const bool wide = vec && c0 + 4 <= cols;
+    if (wide) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 h[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        f32x4 e = {0.f, 0.f, 0.f, 0.f};
-        if (r0 + i < rows) {
-            const T* src = x + (r0 + i) * ld + c0;
-            if (vec && c0 + 4 <= cols) {
-                if constexpr (sizeof(T) == 4) {
-                    e = *(const f32x4*)src;
-                } else {
-                    typedef T T4 __attribute__((ext_vector_type(4)));
-                    const T4 h = *(const T4*)src;
+        for (int i = 0; i < 16; ++i) h[i] = *(const T4*)(x + (r0 + i < rows ? r0 + i : rows - 1) * ld + c0);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) e[k] = (float)h[k];
-                }
-            } else {
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i][k] = r0 + i < rows ? (float)h[i][k] : 0.f;
+    } else {
+        T h[16][4];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                h[i][k] = x[(r0 + i < rows ? r0 + i : rows - 1) * ld + (c0 + k < cols ? c0 + k : cols - 1)];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i][k] = r0 + i < rows && c0 + k < cols ? (float)h[i][k] : 0.f;
+    }
+    if (mult != nullptr) {
+        const bool mwide = (cols & 3) == 0 && c0 + 4 <= cols;
+        typedef __bf16 B4 __attribute__((ext_vector_type(4)));
+        if (mwide) {
+            B4 h[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) h[i] = *(const B4*)(mult + (r0 + i < rows ? r0 + i : rows - 1) * cols + c0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[i][k] *= r0 + i < rows ? (float)h[i][k] : 0.f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (c0 + k < cols) e[k] = (float)src[k];
-            }
-            if (mult != nullptr) {
-                const __bf16* ms = mult + (r0 + i) * cols + c0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (c0 + k < cols) e[k] *= (float)ms[k];
-            }
+                    if (r0 + i < rows && c0 + k < cols) v[i][k] *= (float)mult[(r0 + i) * cols + c0 + k];
         }
-        v[i] = e;
     }
 
     if (colsum != nullptr) {  // 16 rows a thread, then the 8 row groups in order
@@ -204,18 +219,24 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
     }
 }
 
-// out[c] = sum_b colsum[b][c] in order, in 64 bits: 4 row groups a workgroup, joined in a fixed order
-__global__ __launch_bounds__(256) void colsum_kernel(const float* __restrict__ colsum, int64_t blocks, int64_t cols,
-                                                     float* __restrict__ out) {
-    __shared__ double red[4][64];
-    const int t = threadIdx.x, g = t >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + (t & 63);
+// out[c] = sum_b colsum[b][c] in 64 bits: 32 columns x 32 groups of row blocks a workgroup, the groups joined in a fixed
+// order (4 groups of 64 columns left 16 workgroups for 1024 columns: 213 us for 2048 row blocks)
+__global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ colsum, int64_t blocks, int64_t cols,
+                                                      float* __restrict__ out) {
+    __shared__ double red[32][33];
+    const int t = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + t;
     double a = 0.0;
-    if (c < cols)
-        for (int64_t b = g; b < blocks; b += 4) a += (double)colsum[b * cols + c];
-    red[g][t & 63] = a;
+    if (c < cols) {
+#pragma unroll 8
+        for (int64_t b = g; b < blocks; b += 32) a += (double)colsum[b * cols + c];
+    }
+    red[g][t] = a;
     __syncthreads();
-    if (g == 0 && c < cols) out[c] = (float)((red[0][t] + red[1][t]) + (red[2][t] + red[3][t]));
+    if (g == 0 && c < cols) {
+        for (int k = 1; k < 32; ++k) a += red[k][t];
+        out[c] = (float)a;
+    }
 }
 
 }  // namespace
@@ -223,7 +244,7 @@ __global__ __launch_bounds__(256) void colsum_kernel(const float* __restrict__ c
 void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
     const int64_t col_blocks = fp8_blocks(a.cols), grid = fp8_blocks(a.rows) * col_blocks;
     const int64_t size = a.type == FP8_F32 ? 4 : 2;
-    const int vec = ((uintptr_t)a.x % (4 * size)) == 0 && a.ld % 4 == 0;
+    const int vec = ((uintptr_t)a.x % (4 * size)) == 0 && (a.ld % 4 == 0 || a.rows == 1);
 #define SIREN_QUANT(T, E)                                                                                       \
     hipLaunchKernelGGL((quant_kernel<T, E>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
                        a.cols, (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, vec, (int)col_blocks)
@@ -240,7 +261,7 @@ void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
 }
 
 void launch_fp8_colsum(hipStream_t stream, const float* colsum, int64_t blocks, int64_t cols, float* out) {
-    hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, stream, colsum, blocks, cols, out);
+    hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, stream, colsum, blocks, cols, out);
 }
 
 }  // namespace siren

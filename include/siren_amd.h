@@ -430,7 +430,7 @@ int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t c
                            int32_t format, int32_t tiles, void* q, void* s, void* qt, void* st, float* colsum_ws,
                            float* colsum, void* stream);
 
-/* out (m, n) = act(a b^T + bias) of a (m, k) and b (n, k) quantised along k, sums in 32 bits. a may be e4m3 or e5m2,
+/* out (m, n) = act(a b^T + bias) of a (m, k) and b (n, k) quantised along k (k < 2^24, n < 2^22), sums in 32 bits. a may be e4m3 or e5m2,
  * b is e4m3. act 0: none, 1: sin(omega z), with deriv (m, n) bf16, nullable, = omega cos(omega z). bias (n) fp32,
  * nullable. ws: siren_fp8_matmul_ws_bytes(m, n, k) bytes. */
 int32_t siren_fp8_matmul_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes);

@@ -5,13 +5,15 @@
 // The card's fp8 matrix instructions keep about 17 bits of the products that one instruction sums (errors of 1e-5 of
 // the result on random operands, whatever the length), the bf16 ones lose nothing of these operands' products; an e4m3
 // value times a power of two is a bf16 number exactly, and v_cvt_scalef32_pk_bf16_fp8 makes two of them at once. So the
-// operands travel as bytes through HBM and LDS, are scaled and widened in registers, and the bf16 matrix pipe sums them.
+// operands travel as bytes through HBM and LDS, are scaled and widened in registers, and the bf16 matrix pipe sums them,
+// for 16-bit results too (an output that nearly cancels would show the fp8 instructions' missing bits there as well).
 //
-// A workgroup of 4 waves owns 128 x 128 of out, each wave 64 x 64 (16 accumulators of 16 x 16). A step takes one block
-// of 128 k of both operands: 16 + 16 KiB by direct global-to-LDS loads, two buffers, so one step's loads run behind the
-// other's products. An LDS row is the 128 bytes of one operand row; its 16-byte pieces are permuted by (row >> 1) & 7 on
-// the way in, so that the 16 lanes that read one piece of 16 rows hit distinct banks. The sums do not care in which
-// order k is taken as long as both operands agree: piece p of a row serves as k-slices 2p, 2p + 1 of 8 x 8.
+// A workgroup of 4 waves owns 256 x 128 of out (128 x 128 where rows are few), each wave 128 x 64 (64 x 64) in tiles of
+// 32 x 32. Half a block, 64 k of both operands, is one stage of LDS: 24 KiB by direct global-to-LDS loads, three stages, so
+// the loads run two half blocks ahead; two workgroups share a CU, and one's stores run behind the other's products. An
+// LDS row is 64 bytes of one operand row; its 16-byte pieces are permuted by (row >> 2) & 3 on the way in, so that the 16
+// lanes that read one piece of 16 rows hit distinct banks. The sums do not care in which order k is taken as long as both
+// operands agree, so a lane's 16 contiguous bytes serve two instructions of 8.
 #include "fp8.h"
 #include "siren_common.h"
 
@@ -20,13 +22,13 @@ namespace siren {
 namespace {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int TM = 128, TN = 128, BK = 128;  // workgroup tile, k of one step
-constexpr int OPERAND = 128 * BK;            // bytes of one operand's step
+constexpr int TN = 128;  // columns of a workgroup's tile
+constexpr int BK = 128;  // k of one block of scales
+constexpr int HK = 64;   // k of one stage of LDS: half a block
 
 struct GemmArgs {
     const uint8_t *a, *b, *sa, *sb;
@@ -73,11 +75,26 @@ __device__ __forceinline__ void put4(T* dst, f32x4 v, int valid, bool vec) {
     }
 }
 
-// bias, sine and the store of out[row][col .. col + 3]
+constexpr float EXACT_PHASE = 1.0e5f;  // past this sincos_fast's reduction is not exact
+
+// v <- sin t, returns cos t. far: t may be past EXACT_PHASE: its turns are taken in 64 bits (an fp32 phase over 1e9 is
+// itself off by turns)
+__device__ __forceinline__ float sine(float t, bool far, float& v) {
+    float cs;
+    if (far) {
+        const float u = (float)__builtin_amdgcn_fract((double)t * 0.15915494309189533577);
+        v = __builtin_amdgcn_sinf(u);
+        cs = __builtin_amdgcn_cosf(u);
+    } else {
+        sincos_fast(t, v, cs);  // to 4e-7
+    }
+    return cs;
+}
+
+// bias, sine and the store of out[row][col .. col + 3], of which valid exist
 template <typename T>
 __device__ __forceinline__ void finish(const GemmArgs& g, int64_t row, int64_t col, f32x4 v) {
-    const int64_t left = g.n - col;
-    const int valid = left < 4 ? (int)left : 4;
+    const int valid = g.n - col < 4 ? (int)(g.n - col) : 4;
     const bool vec = (g.n & 3) == 0;
     if (g.bias != nullptr) {
 #pragma unroll
@@ -85,146 +102,203 @@ __device__ __forceinline__ void finish(const GemmArgs& g, int64_t row, int64_t c
             if (k < valid) v[k] += g.bias[col + k];
     }
     if (g.act == FP8_ACT_SINE) {
-        f32x4 t = v * g.omega;
-        const float top = fmaxf(fmaxf(__builtin_fabsf(t[0]), __builtin_fabsf(t[1])),
-                                fmaxf(__builtin_fabsf(t[2]), __builtin_fabsf(t[3])));
-        if (__builtin_expect(top > 1.0e5f, 0)) {  // past the reduction's exact range
+        f32x4 d;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = sinf(t[k]);
-            if (g.deriv != nullptr) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) t[k] = g.omega * cosf(t[k]);
-                put4(g.deriv + row * g.n + col, t, valid, vec);
-            }
-        } else {
-            f32x4 d;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float sn, cs;
-                sincos_fast(t[k], sn, cs);  // 4e-7; the cosine falls away where nothing takes it
-                v[k] = sn;
-                d[k] = g.omega * cs;
-            }
-            if (g.deriv != nullptr) put4(g.deriv + row * g.n + col, d, valid, vec);
+        for (int k = 0; k < 4; ++k) {
+            const float t = g.omega * v[k];
+            float sn;
+            d[k] = g.omega * sine(t, __builtin_fabsf(t) > EXACT_PHASE, sn);
+            v[k] = sn;
         }
+        if (g.deriv != nullptr) put4(g.deriv + row * g.n + col, d, valid, vec);
     }
     put4((T*)g.out + row * g.n + col, v, valid, vec);
 }
 
-template <typename T, bool E5M2A, bool SPLIT>
+// The products of one half block (64 k) of a wave's RT x 2 tiles of 32 x 32: bytes to bf16, scaled on the way
+template <bool E5M2A, int RT>
+__device__ __forceinline__ void half_block(const uint8_t* la, const uint8_t* lb, int lane, const uint32_t (&ba)[RT],
+                                           const uint32_t (&bb)[2], f32x16 (&acc)[RT][2]) {
+    const int r = lane & 31, h = lane >> 5, sw = (r >> 2) & 3;
+    // this lane's two 16-byte pieces of a row: piece 2 i + h of the row lies at (2 i + h) ^ sw
+    const int at0 = r * HK + ((h ^ sw) * 16), at1 = r * HK + (((2 + h) ^ sw) * 16);
+    bf16x8 vb[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const float f = __uint_as_float(bb[j] << 23);
+        const u32x4 p = *(const u32x4*)(lb + j * 32 * HK + at0), q = *(const u32x4*)(lb + j * 32 * HK + at1);
+        vb[j][0] = widen8<false>(p[0], p[1], f);
+        vb[j][1] = widen8<false>(p[2], p[3], f);
+        vb[j][2] = widen8<false>(q[0], q[1], f);
+        vb[j][3] = widen8<false>(q[2], q[3], f);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const float f = __uint_as_float(ba[i] << 23);
+        const u32x4 p = *(const u32x4*)(la + i * 32 * HK + at0), q = *(const u32x4*)(la + i * 32 * HK + at1);
+        const bf16x8 va[4] = {widen8<E5M2A>(p[0], p[1], f), widen8<E5M2A>(p[2], p[3], f), widen8<E5M2A>(q[0], q[1], f),
+                              widen8<E5M2A>(q[2], q[3], f)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[k], vb[j][k], acc[i][j], 0, 0, 0);
+    }
+}
+
+template <typename T, bool E5M2A, bool SPLIT, int RT>
 __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
-    __shared__ __align__(16) uint8_t lds[2][2][OPERAND];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int r = lane & 15, q = lane >> 4;
+    constexpr int TM = RT * 64;                 // rows of the workgroup's tile: 2 waves of RT x 32
+    constexpr int STAGE = (TM + TN) * HK;       // bytes of one half block
+    constexpr int LOADS = (TM + TN) / 16 / 4;   // 1 KiB pieces of it a wave loads
+    __shared__ __align__(16) uint8_t lds[3 * STAGE];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave & 1, wn = wave >> 1;
 
-    // workgroups go round-robin to the 8 dies: give each die a contiguous run of tiles, columns fastest, so that the
-    // tiles that share rows of A meet in one L2
+    // Workgroups go round-robin to the 8 dies: give each die a contiguous run of the (split, tile) list, columns fastest, so
+    // that the tiles that share rows of A, or a split's k of both operands, meet in one L2 (the splits of a 1024 x 1024
+    // product over 262144, dealt out tile by tile, read B from HBM on every die: 540 us instead of XXX)
     const int tiles = g.tiles_m * g.tiles_n;
     int tile = blockIdx.x;
     {
-        const int per = tiles / 8, rest = tiles % 8, x = tile & 7, y = tile >> 3;
+        const int all = gridDim.x, per = all / 8, rest = all % 8, x = tile & 7, y = tile >> 3;
         tile = x * per + (x < rest ? x : rest) + y;
     }
-    const int64_t m0 = (int64_t)(tile / g.tiles_n) * TM, n0 = (int64_t)(tile % g.tiles_n) * TN;
-    const int first = blockIdx.y * g.steps_per_split;
+    const int split = SPLIT ? __builtin_amdgcn_readfirstlane(tile / tiles) : 0;
+    tile -= split * tiles;
+    const int tm = __builtin_amdgcn_readfirstlane(tile / g.tiles_n), tn = tile - tm * g.tiles_n;
+    const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
+    const int first = split * g.steps_per_split;
     const int last = first + g.steps_per_split < g.steps ? first + g.steps_per_split : g.steps;
+    const int halves = 2 * (last - first);
 
-    // this thread's pieces of a step: rows (wave * 4 + j) * 8 + lane / 8, piece lane % 8 of the permuted row. Rows past
-    // the operand's end read its last row; their products are not stored.
-    const uint8_t *pa[4], *pb[4];
+    // This wave's 1 KiB pieces of a stage: 16 rows of A or of B each, lane / 4 the row, lane % 4 the place in LDS. Rows
+    // past the operand's end read its last row; their products are not stored.
+    const uint8_t* base[LOADS];
+    uint32_t off[LOADS];
+    const int prow = lane >> 2, piece = (lane & 3) ^ ((prow >> 2) & 3);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int row = (wave * 4 + j) * 8 + (lane >> 3);
-        const int piece = (lane & 7) ^ ((row >> 1) & 7);
-        const int64_t ra = m0 + row < g.m ? m0 + row : g.m - 1, rb = n0 + row < g.n ? n0 + row : g.n - 1;
-        pa[j] = g.a + ra * g.lda + (int64_t)first * BK + piece * 16;
-        pb[j] = g.b + rb * g.ldb + (int64_t)first * BK + piece * 16;
+    for (int j = 0; j < LOADS; ++j) {
+        const int p = wave * LOADS + j;  // a piece is all A or all B: TM / 16 pieces of A
+        const bool is_a = p < TM / 16;
+        const int64_t row0 = is_a ? m0 : n0, rows = is_a ? g.m : g.n, ld = is_a ? g.lda : g.ldb;
+        const int64_t row = (is_a ? p * 16 : p * 16 - TM) + prow;
+        base[j] = (is_a ? g.a : g.b) + row0 * ld + (int64_t)first * BK;
+        off[j] = (uint32_t)((row0 + row < rows ? row : rows - 1 - row0) * ld) + piece * 16;
     }
-    auto load = [&](int buf) {
+    const unsigned lds0 = lds_addr(lds);
+    auto load = [&](int stage, int half) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)pa[j],
-                                             (__attribute__((address_space(3))) void*)(lds[buf][0] + (wave * 4 + j) * 1024),
-                                             16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)pb[j],
-                                             (__attribute__((address_space(3))) void*)(lds[buf][1] + (wave * 4 + j) * 1024),
-                                             16, 0, 0);
-            pa[j] += BK;
-            pb[j] += BK;
-        }
+        for (int j = 0; j < LOADS; ++j)
+            glds_x4(base[j] + (int64_t)half * HK, off[j], lds0 + stage * STAGE + (wave * LOADS + j) * 1024);
     };
 
-    // the scales of this lane's rows, four steps to a word
-    const uint8_t *qa[4], *qb[4];
+    // the scales of this lane's rows, eight blocks of k in two words
+    const uint8_t *qa[RT], *qb[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t ra = m0 + wm * 64 + i * 16 + r, rb = n0 + wn * 64 + i * 16 + r;
+    for (int i = 0; i < RT; ++i) {
+        const int64_t ra = m0 + (wm * RT + i) * 32 + (lane & 31);
         qa[i] = g.sa + ((ra < g.m ? ra : g.m - 1) >> g.sha) * g.lsa;
-        qb[i] = g.sb + ((rb < g.n ? rb : g.n - 1) >> g.shb) * g.lsb;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t rb = n0 + (wn * 2 + j) * 32 + (lane & 31);
+        qb[j] = g.sb + ((rb < g.n ? rb : g.n - 1) >> g.shb) * g.lsb;
     }
 
-    f32x4 acc[4][4] = {};
-    uint32_t wa[4], wb[4];
-    load(0);
-    for (int step = first; step < last; ++step) {
-        const int buf = (step - first) & 1;
-        if (step == first || (step & 3) == 0) {
+    f32x16 acc[RT][2] = {};
+    uint64_t wa[RT], wb[2];
+    load(0, 0);
+    load(1, 1);
+    int stage = 0;
+    for (int half = 0; half < halves; ++half) {
+        const int block = first + (half >> 1);
+        if (half == 0 || ((half & 1) == 0 && (block & 7) == 0)) {
+            const int at = block & ~7, more = at + 4 < g.lsa ? at + 4 : at;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                wa[i] = *(const uint32_t*)(qa[i] + (step & ~3));
-                wb[i] = *(const uint32_t*)(qb[i] + (step & ~3));
-            }
+            for (int i = 0; i < RT; ++i)
+                wa[i] = *(const uint32_t*)(qa[i] + at) | (uint64_t) * (const uint32_t*)(qa[i] + more) << 32;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                wb[j] = *(const uint32_t*)(qb[j] + at) | (uint64_t) * (const uint32_t*)(qb[j] + more) << 32;
+            // vmcnt(0), here and not at their first use: hipcc does not count the direct-to-LDS loads, so its own wait in
+            // the loop's body would be for all of those, every half block
+            __builtin_amdgcn_s_waitcnt(0x0F70);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's direct-to-LDS loads of this step
-        __syncthreads();  // every wave's are in, and the other buffer has been read
-        if (step + 1 < last) load(buf ^ 1);
-        const int shift = 8 * (step & 3);
-        float fa[4], fb[4];
+        // Everything but the newest stage's loads is in: they return in order, and this stage's were issued before those.
+        // At the last stage there are no newer ones. This wave's own reads of the stage before are done too.
+        if (half + 1 < halves)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        // every wave's are in, and every wave has read the stage before this one, which the next loads overwrite
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (half + 2 < halves) load(stage == 0 ? 2 : stage - 1, half + 2);
+        const int shift = 8 * (block & 7);
+        uint32_t ba[RT], bb[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            fa[i] = __uint_as_float(((wa[i] >> shift) & 0xFFu) << 23);
-            fb[i] = __uint_as_float(((wb[i] >> shift) & 0xFFu) << 23);
-        }
+        for (int i = 0; i < RT; ++i) ba[i] = (uint32_t)(wa[i] >> shift) & 0xFFu;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = r * BK + (((h * 4 + q) ^ ((r >> 1) & 7)) * 16);
-            bf16x8 va[4][2], vb[4][2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const u32x4 ba = *(const u32x4*)(lds[buf][0] + (wm * 64 + i * 16) * BK + at);
-                const u32x4 bb = *(const u32x4*)(lds[buf][1] + (wn * 64 + i * 16) * BK + at);
-                va[i][0] = widen8<E5M2A>(ba[0], ba[1], fa[i]);
-                va[i][1] = widen8<E5M2A>(ba[2], ba[3], fa[i]);
-                vb[i][0] = widen8<false>(bb[0], bb[1], fb[i]);
-                vb[i][1] = widen8<false>(bb[2], bb[3], fb[i]);
-            }
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb[j][p], va[i][p], acc[i][j], 0, 0, 0);
-        }
+        for (int j = 0; j < 2; ++j) bb[j] = (uint32_t)(wb[j] >> shift) & 0xFFu;
+        const uint8_t* la = lds + stage * STAGE + wm * RT * 32 * HK;
+        const uint8_t* lb = lds + stage * STAGE + (TM + wn * 64) * HK;
+        half_block<E5M2A, RT>(la, lb, lane, ba, bb, acc);
+        stage = stage == 2 ? 0 : stage + 1;
     }
 
-    // B rows are the instruction's rows: lane (r, q) holds out[m][n .. n + 3] with m = r, n = 4 q of each 16 x 16
+    // Register 4 k + e of a 32 x 32 tile is out[8 k + 4 (lane / 32) + e][lane % 32]: 32 lanes write 32 consecutive columns.
+    // (The other operand order, four columns a lane, stored 32 bytes a row at a time and cost HBM twice the requests.)
+    const int64_t rows_left = g.m - m0;
+    const int row0 = wm * RT * 32 + 4 * (lane >> 5), col0 = wn * 64 + (lane & 31);
+    const uint32_t n = (uint32_t)g.n;
+    if constexpr (SPLIT) {
+        float* tile_out = (float*)g.out + (split * g.m + m0) * g.n + n0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = m0 + wm * 64 + i * 16 + r;
-        if (row >= g.m) continue;
+        for (int j = 0; j < 2; ++j)
+            if (n0 + col0 + 32 * j < g.n) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t col = n0 + wn * 64 + j * 16 + q * 4;
-            if (col >= g.n) continue;
-            if constexpr (SPLIT) {
-                const int64_t left = g.n - col;
-                put4((float*)g.out + ((int64_t)blockIdx.y * g.m + row) * g.n + col, acc[i][j],
-                     left < 4 ? (int)left : 4, (g.n & 3) == 0);
-            } else {
-                finish<T>(g, row, col, acc[i][j]);
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int row = row0 + 32 * i + 8 * (e >> 2) + (e & 3);
+                        if (row < rows_left) tile_out[row * n + col0 + 32 * j] = acc[i][j][e];
+                    }
             }
+        return;
+    }
+    T* tile_out = (T*)g.out + m0 * g.n + n0;
+    __bf16* tile_deriv = g.deriv == nullptr ? nullptr : g.deriv + m0 * g.n + n0;
+    const bool whole = rows_left >= TM;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const bool inside = n0 + col0 + 32 * j < g.n;
+        const float bias = g.bias != nullptr && inside ? g.bias[n0 + col0 + 32 * j] : 0.f;
+        bool far = false;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                acc[i][j][e] += bias;
+                far |= __builtin_fabsf(g.omega * acc[i][j][e]) > EXACT_PHASE;
+            }
+        const bool any_far = g.act == FP8_ACT_SINE && __any(far);
+        if (inside) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int row = row0 + 32 * i + 8 * (e >> 2) + (e & 3);
+                    if (whole || row < rows_left) {
+                        const uint32_t at = row * n + col0 + 32 * j;
+                        float v = acc[i][j][e];
+                        if (g.act == FP8_ACT_SINE) {
+                            const float cs = sine(g.omega * v, any_far, v);
+                            if (tile_deriv != nullptr) tile_deriv[at] = (__bf16)(g.omega * cs);
+                        }
+                        tile_out[at] = (T)v;
+                    }
+                }
         }
     }
 }
@@ -282,14 +356,28 @@ void launch_join(hipStream_t stream, const GemmArgs& g, const void* part, int sp
         hipLaunchKernelGGL((join_kernel<T, 1>), grid, dim3(256), 0, stream, g, (const float*)part, splits);
 }
 
-// splits of the k axis: enough workgroups to fill 256 CUs twice, at least 4 steps each
+// 256 rows a tile where that leaves the card two workgroups a CU, 128 otherwise
+bool tall(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + TN - 1) / TN) >= 512; }
+
+// splits of the k axis: enough workgroups to fill 256 CUs twice, at least 4 blocks each
 int splits_of(int64_t m, int64_t n, int64_t k) {
-    const int64_t tiles = ((m + TM - 1) / TM) * ((n + TN - 1) / TN), steps = fp8_blocks(k);
+    const int64_t tm = m > 128 ? 256 : 128, tiles = ((m + tm - 1) / tm) * ((n + TN - 1) / TN), steps = fp8_blocks(k);
     if (tiles >= 256 || steps < 8) return 1;
     int64_t s = (512 + tiles - 1) / tiles;
     if (s > steps / 4) s = steps / 4;
     const int64_t per = (steps + s - 1) / s;
     return (int)((steps + per - 1) / per);
+}
+
+template <typename T, bool E5M2A, bool SPLIT>
+void launch_gemm(hipStream_t stream, GemmArgs& g, int splits, bool rows256) {
+    g.tiles_m = (int)((g.m + (rows256 ? 255 : 127)) / (rows256 ? 256 : 128));
+    g.tiles_n = (int)((g.n + TN - 1) / TN);
+    const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * splits));
+    if (rows256)
+        hipLaunchKernelGGL((gemm_kernel<T, E5M2A, SPLIT, 4>), grid, dim3(256), 0, stream, g);
+    else
+        hipLaunchKernelGGL((gemm_kernel<T, E5M2A, SPLIT, 2>), grid, dim3(256), 0, stream, g);
 }
 
 }  // namespace
@@ -312,8 +400,6 @@ void launch_fp8_product(hipStream_t stream, const Fp8Product& p) {
     g.sha = p.a.shift;
     g.shb = p.b.shift;
     g.steps = (int)fp8_blocks(p.k);
-    g.tiles_m = (int)((g.m + TM - 1) / TM);
-    g.tiles_n = (int)((g.n + TN - 1) / TN);
     g.bias = p.bias;
     g.act = p.act;
     g.omega = p.omega;
@@ -321,29 +407,27 @@ void launch_fp8_product(hipStream_t stream, const Fp8Product& p) {
     const int splits = splits_of(g.m, g.n, p.k);
     g.steps_per_split = (g.steps + splits - 1) / splits;
     g.out = splits > 1 ? p.ws : p.out;
-    const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), (unsigned)splits);
-#define SIREN_GEMM(T, E, S) hipLaunchKernelGGL((gemm_kernel<T, E, S>), grid, dim3(256), 0, stream, g)
     if (splits > 1) {
         if (p.e5m2_a)
-            SIREN_GEMM(float, true, true);
+            launch_gemm<float, true, true>(stream, g, splits, g.m > 128);
         else
-            SIREN_GEMM(float, false, true);
+            launch_gemm<float, false, true>(stream, g, splits, g.m > 128);
         g.out = p.out;
         if (p.type == FP8_F32) launch_join<float>(stream, g, p.ws, splits);
         if (p.type == FP8_BF16) launch_join<__bf16>(stream, g, p.ws, splits);
         if (p.type == FP8_F16) launch_join<_Float16>(stream, g, p.ws, splits);
         return;
     }
+    const bool rows256 = tall(g.m, g.n);
     if (p.e5m2_a) {
-        if (p.type == FP8_F32) SIREN_GEMM(float, true, false);
-        if (p.type == FP8_BF16) SIREN_GEMM(__bf16, true, false);
-        if (p.type == FP8_F16) SIREN_GEMM(_Float16, true, false);
+        if (p.type == FP8_F32) launch_gemm<float, true, false>(stream, g, 1, rows256);
+        if (p.type == FP8_BF16) launch_gemm<__bf16, true, false>(stream, g, 1, rows256);
+        if (p.type == FP8_F16) launch_gemm<_Float16, true, false>(stream, g, 1, rows256);
     } else {
-        if (p.type == FP8_F32) SIREN_GEMM(float, false, false);
-        if (p.type == FP8_BF16) SIREN_GEMM(__bf16, false, false);
-        if (p.type == FP8_F16) SIREN_GEMM(_Float16, false, false);
+        if (p.type == FP8_F32) launch_gemm<float, false, false>(stream, g, 1, rows256);
+        if (p.type == FP8_BF16) launch_gemm<__bf16, false, false>(stream, g, 1, rows256);
+        if (p.type == FP8_F16) launch_gemm<_Float16, false, false>(stream, g, 1, rows256);
     }
-#undef SIREN_GEMM
 }
 
 }  // namespace siren

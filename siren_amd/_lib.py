@@ -99,7 +99,7 @@ _SIGS = {
     'siren_second_order_batched': [_CFG, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P],
     'siren_hvp_backward_batched_ws_floats': [_CFG, _I64, _I64, ctypes.POINTER(_I64)],
     'siren_hvp_backward_batched': [_CFG, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P],
-    'siren_fp8_quantize': [_P, _I32, _I64, _I64, _I64, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _P],
+    'siren_fp8_quantize': [_P, _I32, _I64, _I64, _I64, _P, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P],
     'siren_fp8_matmul_ws_bytes': [_I64, _I64, _I64, ctypes.POINTER(_I64)],
     'siren_fp8_matmul': [_P, _P, _I64, _I32, _I32, _P, _P, _I64, _I32, _I64, _P, _I32, ctypes.c_float, _P, _I32, _P, _P,
                          _P],

@@ -24,18 +24,19 @@ struct Fp8Quant {
     const void* mult;
     uint8_t *q, *s, *qt, *st;
     float* colsum;
-    int type, e5m2, tiles;
+    int type, e5m2, tiles, panels;  // panels: of q and of qt, as in Fp8Operand
 };
 void launch_fp8_quant(hipStream_t st, const Fp8Quant& a);
 // out[c] = sum over the row blocks of colsum (blocks, cols), in order
 void launch_fp8_colsum(hipStream_t st, const float* colsum, int64_t blocks, int64_t cols, float* out);
 
-// One operand of a product: rows of `padded` bytes, block scales per row (shift 0) or per 128 rows (shift 7)
+// One operand of a product, block scales per row (shift 0) or per 128 rows (shift 7). data: rows of `padded` bytes, or in
+// panels (padded / 64, rows, 64): 64 k of all rows, then the next 64.
 struct Fp8Operand {
     const uint8_t* data;
     const uint8_t* scale;
     int64_t rows;
-    int shift;
+    int shift, panels;
 };
 // out (a.rows, b.rows) = act(a b^T + bias), sums over k; deriv (nullable, bf16): omega cos(omega z) of the sine
 struct Fp8Product {

@@ -1699,8 +1699,8 @@ int check_fp8_source(const void* x, int32_t dtype, int64_t rows, int64_t cols, i
 }  // namespace
 
 int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, const void* mult,
-                           int32_t format, int32_t tiles, void* q, void* s, void* qt, void* st, float* colsum_ws,
-                           float* colsum, void* stream) {
+                           int32_t format, int32_t tiles, int32_t panels, void* q, void* s, void* qt, void* st,
+                           float* colsum_ws, float* colsum, void* stream) {
     if (int rc = check_fp8_type(dtype)) return rc;
     if (rows < 0 || cols < 0 || (format != 0 && format != 1))
         return fail(SIREN_EINVAL, "siren_fp8_quantize: need rows, cols >= 0 and format 0 (e4m3) or 1 (e5m2)");
@@ -1715,7 +1715,7 @@ int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t c
     if (!aligned(q, 16) || !aligned(qt, 16) || !aligned(s, 4) || !aligned(st, 4) || !aligned(mult, 2))
         return fail(SIREN_EINVAL, "siren_fp8_quantize: q and qt must be 16-byte aligned, scales 4-byte aligned");
     siren::Fp8Quant a{x, ld, rows, cols, mult, (uint8_t*)q, (uint8_t*)s, (uint8_t*)qt, (uint8_t*)st,
-                      colsum != nullptr ? colsum_ws : nullptr, dtype, format, tiles != 0};
+                      colsum != nullptr ? colsum_ws : nullptr, dtype, format, tiles != 0, panels != 0};
     siren::launch_fp8_quant((hipStream_t)stream, a);
     if (colsum != nullptr)
         siren::launch_fp8_colsum((hipStream_t)stream, colsum_ws, siren::fp8_blocks(rows), cols, colsum);
@@ -1729,21 +1729,21 @@ int32_t siren_fp8_matmul_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* byte
     return SIREN_OK;
 }
 
-int32_t siren_fp8_matmul(const void* a, const void* sa, int64_t m, int32_t a_tiles, int32_t a_format, const void* b,
-                         const void* sb, int64_t n, int32_t b_tiles, int64_t k, const float* bias, int32_t act,
+int32_t siren_fp8_matmul(const void* a, const void* sa, int64_t m, int32_t a_layout, int32_t a_format, const void* b,
+                         const void* sb, int64_t n, int32_t b_layout, int64_t k, const float* bias, int32_t act,
                          float omega, void* out, int32_t dtype, void* deriv, void* ws, void* stream) {
     if (int rc = check_fp8_type(dtype)) return rc;
     if (int rc = check_fp8_product(m, n, k)) return rc;
-    if (a_format != 0 && a_format != 1)
-        return fail(SIREN_EINVAL, "siren_fp8_matmul: a_format is 0 (e4m3) or 1 (e5m2)");
+    if ((a_format != 0 && a_format != 1) || (a_layout & ~3) != 0 || (b_layout & ~3) != 0)
+        return fail(SIREN_EINVAL, "siren_fp8_matmul: a_format is 0 (e4m3) or 1 (e5m2), layouts are SIREN_FP8_TILES | SIREN_FP8_PANELS");
     if (int rc = check_fp8_act(act, omega, deriv)) return rc;
     if (m == 0 || n == 0) return SIREN_OK;
     if (int rc = check_fp8_operands(a, sa, b, sb, bias, out, deriv)) return rc;
     if (!aligned(ws, 16)) return fail(SIREN_EINVAL, "siren_fp8_matmul: ws must be 16-byte aligned");
     if (siren::fp8_product_ws_bytes(m, n, k) > 0 && ws == nullptr)
         return fail(SIREN_EINVAL, "siren_fp8_matmul: ws is NULL (siren_fp8_matmul_ws_bytes)");
-    siren::Fp8Product p{{(const uint8_t*)a, (const uint8_t*)sa, m, a_tiles ? 7 : 0},
-                        {(const uint8_t*)b, (const uint8_t*)sb, n, b_tiles ? 7 : 0},
+    siren::Fp8Product p{{(const uint8_t*)a, (const uint8_t*)sa, m, (a_layout & SIREN_FP8_TILES) ? 7 : 0, a_layout & SIREN_FP8_PANELS},
+                        {(const uint8_t*)b, (const uint8_t*)sb, n, (b_layout & SIREN_FP8_TILES) ? 7 : 0, b_layout & SIREN_FP8_PANELS},
                         k, bias, act, omega, out, dtype, deriv, a_format, ws};
     siren::launch_fp8_product((hipStream_t)stream, p);
     return hip_status("siren_fp8_matmul");
@@ -1769,9 +1769,9 @@ int32_t siren_fp8_linear(const void* x, int32_t dtype, int64_t m, int64_t k, int
     uint8_t* q = (uint8_t*)ws;
     uint8_t* s = q + m * siren::fp8_padded(k);
     uint8_t* rest = q + (m * siren::fp8_padded(k) + m * siren::fp8_scale_cols(k) + 15) / 16 * 16;
-    if (int rc = siren_fp8_quantize(x, dtype, m, k, ld, nullptr, 0, 0, q, s, nullptr, nullptr, nullptr, nullptr, stream))
+    if (int rc = siren_fp8_quantize(x, dtype, m, k, ld, nullptr, 0, 0, 1, q, s, nullptr, nullptr, nullptr, nullptr, stream))
         return rc;
-    return siren_fp8_matmul(q, s, m, 0, 0, w, sw, n, 1, k, bias, act, omega, y, dtype, nullptr, rest, stream);
+    return siren_fp8_matmul(q, s, m, SIREN_FP8_PANELS, 0, w, sw, n, SIREN_FP8_TILES, k, bias, act, omega, y, dtype, nullptr, rest, stream);
 }
 
 int32_t siren_adamw_scratch_bytes(int64_t count, int64_t* bytes) {

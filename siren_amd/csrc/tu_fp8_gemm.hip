@@ -32,7 +32,8 @@ constexpr int HK = 64;   // k of one stage of LDS: half a block
 
 struct GemmArgs {
     const uint8_t *a, *b, *sa, *sb;
-    int64_t lda, ldb, lsa, lsb;  // bytes of a row, of a row's scales
+    int64_t rsa, rsb, hsa, hsb;  // bytes from row to row, from half block to half block
+    int64_t lsa, lsb;            // bytes of a row's scales
     int64_t m, n;
     int sha, shb;                // scales per row (0) or per 128 rows (7)
     int steps, steps_per_split;  // blocks of k, and of one split
@@ -93,56 +94,83 @@ __device__ __forceinline__ float sine(float t, bool far, float& v) {
 
 // bias, sine and the store of out[row][col .. col + 3], of which valid exist
 template <typename T>
-__device__ __forceinline__ void finish(const GemmArgs& g, int64_t row, int64_t col, f32x4 v) {
-    const int valid = g.n - col < 4 ? (int)(g.n - col) : 4;
-    const bool vec = (g.n & 3) == 0;
-    if (g.bias != nullptr) {
+struct Finish {
+    int64_t col;
+    int valid;
+    bool vec;
+    f32x4 bias;
+    __device__ __forceinline__ Finish(const GemmArgs& g, int64_t c) : col(c) {
+        valid = g.n - col < 4 ? (int)(g.n - col) : 4;
+        vec = (g.n & 3) == 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < valid) v[k] += g.bias[col + k];
+        for (int k = 0; k < 4; ++k) bias[k] = g.bias != nullptr && k < valid ? g.bias[col + k] : 0.f;
     }
-    if (g.act == FP8_ACT_SINE) {
-        f32x4 d;
+    __device__ __forceinline__ void store(const GemmArgs& g, int64_t row, f32x4 v) const {
+        v += bias;
+        if (g.act == FP8_ACT_SINE) {
+            f32x4 d;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float t = g.omega * v[k];
-            float sn;
-            d[k] = g.omega * sine(t, __builtin_fabsf(t) > EXACT_PHASE, sn);
-            v[k] = sn;
+            for (int k = 0; k < 4; ++k) {
+                const float t = g.omega * v[k];
+                float sn;
+                d[k] = g.omega * sine(t, __builtin_fabsf(t) > EXACT_PHASE, sn);
+                v[k] = sn;
+            }
+            if (g.deriv != nullptr) put4(g.deriv + row * g.n + col, d, valid, vec);
         }
-        if (g.deriv != nullptr) put4(g.deriv + row * g.n + col, d, valid, vec);
+        put4((T*)g.out + row * g.n + col, v, valid, vec);
     }
-    put4((T*)g.out + row * g.n + col, v, valid, vec);
-}
+};
 
-// The products of one half block (64 k) of a wave's RT x 2 tiles of 32 x 32: bytes to bf16, scaled on the way
+// The products of one half block (64 k) of a wave's RT x 2 tiles of 32 x 32, bytes to bf16 and scaled on the way, in four
+// slices of 16 k: a wave issues in order, so the next slice's widening (3 instructions a product at RT = 4) has to stand
+// between this one's products for the matrix pipe not to wait for it.
 template <bool E5M2A, int RT>
 __device__ __forceinline__ void half_block(const uint8_t* la, const uint8_t* lb, int lane, const uint32_t (&ba)[RT],
                                            const uint32_t (&bb)[2], f32x16 (&acc)[RT][2]) {
     const int r = lane & 31, h = lane >> 5, sw = (r >> 2) & 3;
     // this lane's two 16-byte pieces of a row: piece 2 i + h of the row lies at (2 i + h) ^ sw
-    const int at0 = r * HK + ((h ^ sw) * 16), at1 = r * HK + (((2 + h) ^ sw) * 16);
-    bf16x8 vb[2][4];
+    const int at[2] = {r * HK + ((h ^ sw) * 16), r * HK + (((2 + h) ^ sw) * 16)};
+    u32x4 ra[2][RT], rb[2][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const float f = __uint_as_float(bb[j] << 23);
-        const u32x4 p = *(const u32x4*)(lb + j * 32 * HK + at0), q = *(const u32x4*)(lb + j * 32 * HK + at1);
-        vb[j][0] = widen8<false>(p[0], p[1], f);
-        vb[j][1] = widen8<false>(p[2], p[3], f);
-        vb[j][2] = widen8<false>(q[0], q[1], f);
-        vb[j][3] = widen8<false>(q[2], q[3], f);
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) rb[p][j] = *(const u32x4*)(lb + j * 32 * HK + at[p]);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) ra[p][i] = *(const u32x4*)(la + i * 32 * HK + at[p]);
     }
+    float fa[RT], fb[2];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const float f = __uint_as_float(ba[i] << 23);
-        const u32x4 p = *(const u32x4*)(la + i * 32 * HK + at0), q = *(const u32x4*)(la + i * 32 * HK + at1);
-        const bf16x8 va[4] = {widen8<E5M2A>(p[0], p[1], f), widen8<E5M2A>(p[2], p[3], f), widen8<E5M2A>(q[0], q[1], f),
-                              widen8<E5M2A>(q[2], q[3], f)};
+    for (int i = 0; i < RT; ++i) fa[i] = __uint_as_float(ba[i] << 23);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+    for (int j = 0; j < 2; ++j) fb[j] = __uint_as_float(bb[j] << 23);
+    bf16x8 va[2][RT], vb[2][2];
+    auto widen = [&](int k) {
+        const int p = k >> 1, w = 2 * (k & 1), to = k & 1;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) vb[to][j] = widen8<false>(rb[p][j][w], rb[p][j][w + 1], fb[j]);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) va[to][i] = widen8<E5M2A>(ra[p][i][w], ra[p][i][w + 1], fa[i]);
+    };
+    widen(0);
+    // Each slice is scheduled by itself, a product and its share of the next slice's widening in turn: left alone, the
+    // compiler gathers the widening before the products and chains the products of one tile.
+    constexpr int SHARE = (4 * (RT + 2) + 2 * RT - 1) / (2 * RT);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (k < 3) widen(k + 1);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[k], vb[j][k], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[k & 1][j], va[k & 1][i], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 2 * RT; ++e) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (k < 3) __builtin_amdgcn_sched_group_barrier(0x002, SHARE, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -175,22 +203,24 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
     // This wave's 1 KiB pieces of a stage: 16 rows of A or of B each, lane / 4 the row, lane % 4 the place in LDS. Rows
     // past the operand's end read its last row; their products are not stored.
     const uint8_t* base[LOADS];
+    int64_t step[LOADS];
     uint32_t off[LOADS];
     const int prow = lane >> 2, piece = (lane & 3) ^ ((prow >> 2) & 3);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
         const int p = wave * LOADS + j;  // a piece is all A or all B: TM / 16 pieces of A
         const bool is_a = p < TM / 16;
-        const int64_t row0 = is_a ? m0 : n0, rows = is_a ? g.m : g.n, ld = is_a ? g.lda : g.ldb;
+        const int64_t row0 = is_a ? m0 : n0, rows = is_a ? g.m : g.n, rs = is_a ? g.rsa : g.rsb;
         const int64_t row = (is_a ? p * 16 : p * 16 - TM) + prow;
-        base[j] = (is_a ? g.a : g.b) + row0 * ld + (int64_t)first * BK;
-        off[j] = (uint32_t)((row0 + row < rows ? row : rows - 1 - row0) * ld) + piece * 16;
+        step[j] = is_a ? g.hsa : g.hsb;
+        base[j] = (is_a ? g.a : g.b) + row0 * rs + 2 * first * step[j];
+        off[j] = (uint32_t)((row0 + row < rows ? row : rows - 1 - row0) * rs) + piece * 16;
     }
     const unsigned lds0 = lds_addr(lds);
     auto load = [&](int stage, int half) {
 #pragma unroll
         for (int j = 0; j < LOADS; ++j)
-            glds_x4(base[j] + (int64_t)half * HK, off[j], lds0 + stage * STAGE + (wave * LOADS + j) * 1024);
+            glds_x4(base[j] + half * step[j], off[j], lds0 + stage * STAGE + (wave * LOADS + j) * 1024);
     };
 
     // the scales of this lane's rows, eight blocks of k in two words
@@ -247,59 +277,39 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
         stage = stage == 2 ? 0 : stage + 1;
     }
 
-    // Register 4 k + e of a 32 x 32 tile is out[8 k + 4 (lane / 32) + e][lane % 32]: 32 lanes write 32 consecutive columns.
-    // (The other operand order, four columns a lane, stored 32 bytes a row at a time and cost HBM twice the requests.)
-    const int64_t rows_left = g.m - m0;
-    const int row0 = wm * RT * 32 + 4 * (lane >> 5), col0 = wn * 64 + (lane & 31);
-    const uint32_t n = (uint32_t)g.n;
-    if constexpr (SPLIT) {
-        float* tile_out = (float*)g.out + (split * g.m + m0) * g.n + n0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (n0 + col0 + 32 * j < g.n) {
-#pragma unroll
-                for (int i = 0; i < RT; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int row = row0 + 32 * i + 8 * (e >> 2) + (e & 3);
-                        if (row < rows_left) tile_out[row * n + col0 + 32 * j] = acc[i][j][e];
-                    }
-            }
-        return;
-    }
-    T* tile_out = (T*)g.out + m0 * g.n + n0;
-    __bf16* tile_deriv = g.deriv == nullptr ? nullptr : g.deriv + m0 * g.n + n0;
-    const bool whole = rows_left >= TM;
+    // B rows are the instruction's rows: registers 4 k .. 4 k + 3 of a 32 x 32 tile are out[lane % 32][8 k + 4 (lane / 32) ..].
+    // They pass through LDS (the wave's quarter of the stages, which no one reads any more), 32 columns at a time, so that
+    // 8 lanes store 128 bytes of one row: stored as they lie, 32 bytes a row, they cost HBM twice the requests. The loop
+    // over the rows also keeps the epilogue short; unrolled over the accumulators it outgrew the instruction cache.
+    constexpr int ES = 36;  // floats of an LDS row
+    static_assert(RT * 32 * ES * 4 * 4 <= 3 * STAGE, "the epilogue's rows fit the stages");
+    float* strip = (float*)lds + wave * (RT * 32 * ES);
+    __syncthreads();
+    const int64_t wave_m = m0 + wm * RT * 32;
+    const int sub = lane >> 3, quad = (lane & 7) * 4;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const bool inside = n0 + col0 + 32 * j < g.n;
-        const float bias = g.bias != nullptr && inside ? g.bias[n0 + col0 + 32 * j] : 0.f;
-        bool far = false;
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                acc[i][j][e] += bias;
-                far |= __builtin_fabsf(g.omega * acc[i][j][e]) > EXACT_PHASE;
+            for (int k = 0; k < 4; ++k)
+                *(f32x4*)(strip + (i * 32 + (lane & 31)) * ES + 8 * k + 4 * (lane >> 5)) =
+                    f32x4{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int64_t col = n0 + (wn * 2 + j) * 32 + quad;
+        if (col < g.n) {
+            const Finish<T> to(g, col);
+            for (int row = sub; row < RT * 32; row += 8) {
+                const int64_t m = wave_m + row;
+                if (m >= g.m) break;
+                const f32x4 v = *(const f32x4*)(strip + row * ES + quad);
+                if constexpr (SPLIT)
+                    put4((float*)g.out + (split * g.m + m) * g.n + col, v, to.valid, to.vec);
+                else
+                    to.store(g, m, v);
             }
-        const bool any_far = g.act == FP8_ACT_SINE && __any(far);
-        if (inside) {
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int row = row0 + 32 * i + 8 * (e >> 2) + (e & 3);
-                    if (whole || row < rows_left) {
-                        const uint32_t at = row * n + col0 + 32 * j;
-                        float v = acc[i][j][e];
-                        if (g.act == FP8_ACT_SINE) {
-                            const float cs = sine(g.omega * v, any_far, v);
-                            if (tile_deriv != nullptr) tile_deriv[at] = (__bf16)(g.omega * cs);
-                        }
-                        tile_out[at] = (T)v;
-                    }
-                }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
@@ -339,7 +349,7 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs g, const float* __re
             }
             __syncthreads();
         }
-        if (grp == 0 && i < total) finish<T>(g, row, col, v);
+        if (grp == 0 && i < total) Finish<T>(g, col).store(g, row, v);
     }
 }
 
@@ -393,7 +403,10 @@ void launch_fp8_product(hipStream_t stream, const Fp8Product& p) {
     g.b = p.b.data;
     g.sa = p.a.scale;
     g.sb = p.b.scale;
-    g.lda = g.ldb = fp8_padded(p.k);
+    g.rsa = p.a.panels ? HK : fp8_padded(p.k);
+    g.rsb = p.b.panels ? HK : fp8_padded(p.k);
+    g.hsa = p.a.panels ? p.a.rows * HK : HK;
+    g.hsb = p.b.panels ? p.b.rows * HK : HK;
     g.lsa = g.lsb = fp8_scale_cols(p.k);
     g.m = p.a.rows;
     g.n = p.b.rows;

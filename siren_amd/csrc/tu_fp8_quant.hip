@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
                                                     const __bf16* __restrict__ mult, uint8_t* __restrict__ q,
                                                     uint8_t* __restrict__ s, uint8_t* __restrict__ qt,
                                                     uint8_t* __restrict__ st, float* __restrict__ colsum, int tiles,
-                                                    int vec, int col_blocks) {
+                                                    int vec, int col_blocks, int panels) {
     __shared__ __align__(16) uint8_t tr[QT * QSTRIDE];
     __shared__ float part[8][QT];
     __shared__ float wmax[4];
@@ -160,7 +160,9 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
             }
             if (r0 + i < rows) {
                 const float inv = inverse_scale(byte);
-                *(uint32_t*)(q + (r0 + i) * ((int64_t)col_blocks * QT) + c0) =
+                uint8_t* dst = panels ? q + ((cb * 2 + (c4 >> 4)) * rows + r0 + i) * 64 + (c4 & 15) * 4
+                                      : q + (r0 + i) * ((int64_t)col_blocks * QT) + c0;
+                *(uint32_t*)dst =
                     pack4<E5M2>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
                 if (!tiles && c4 == 0) {
                     s[(r0 + i) * s_ld + cb] = (uint8_t)byte;
@@ -209,12 +211,22 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
             *(u32x4*)(tr + (c4 * 4 + k) * QSTRIDE + rg * 16) = w;
         }
         __syncthreads();
+        if (panels) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {  // 8 lanes a column: 128 contiguous bytes of the transpose
-            const int c = j * 32 + (t >> 3), piece = t & 7;
-            if ((int64_t)cb * QT + c < cols)
-                *(u32x4*)(qt + ((int64_t)cb * QT + c) * (row_blocks * QT) + rb * QT + piece * 16) =
-                    *(const u32x4*)(tr + c * QSTRIDE + piece * 16);
+            for (int j = 0; j < 4; ++j) {  // 4 lanes a column of each panel: a wave's 16 columns lie behind each other
+                const int c = (j & 1) * 64 + (t >> 2), piece = (j >> 1) * 4 + (t & 3);
+                if ((int64_t)cb * QT + c < cols)
+                    *(u32x4*)(qt + ((rb * 2 + (j >> 1)) * cols + (int64_t)cb * QT + c) * 64 + (t & 3) * 16) =
+                        *(const u32x4*)(tr + c * QSTRIDE + piece * 16);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // 8 lanes a column: 128 contiguous bytes of the transpose
+                const int c = j * 32 + (t >> 3), piece = t & 7;
+                if ((int64_t)cb * QT + c < cols)
+                    *(u32x4*)(qt + ((int64_t)cb * QT + c) * (row_blocks * QT) + rb * QT + piece * 16) =
+                        *(const u32x4*)(tr + c * QSTRIDE + piece * 16);
+            }
         }
     }
 }
@@ -247,7 +259,7 @@ void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
     const int vec = ((uintptr_t)a.x % (4 * size)) == 0 && (a.ld % 4 == 0 || a.rows == 1);
 #define SIREN_QUANT(T, E)                                                                                       \
     hipLaunchKernelGGL((quant_kernel<T, E>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
-                       a.cols, (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, vec, (int)col_blocks)
+                       a.cols, (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, vec, (int)col_blocks, a.panels)
     if (a.e5m2) {
         if (a.type == FP8_F32) SIREN_QUANT(float, true);
         if (a.type == FP8_BF16) SIREN_QUANT(__bf16, true);

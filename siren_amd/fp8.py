@@ -34,9 +34,18 @@ class Blocks(NamedTuple):
     cols: int
 
     @property
+    def rows(self):
+        return self.data.shape[-2]
+
+    @property
     def tiled(self):
         # one row is both: its tile is its row block
-        return self.scale.shape[0] != self.data.shape[0]
+        return self.scale.shape[0] != self.rows
+
+    @property
+    def layout(self):
+        # what _quantize(panels=True) makes for a product is (cols / 64, rows, 64)
+        return int(self.tiled) | (2 if self.data.dim() == 3 else 0)
 
 
 def _p(t):
@@ -88,25 +97,26 @@ def _words(n):
     return (n + 511) // 512 * 4
 
 
-def _quantize(x, tiles, straight=True, transposed=False, fmt=0, mult=None, colsum=False):
-    """(Blocks | None, Blocks | None of the transpose, column sums | None) of x (rows, cols) by one pass."""
+def _quantize(x, tiles, straight=True, transposed=False, fmt=0, mult=None, colsum=False, panels=False):
+    """(Blocks | None, Blocks | None of the transpose, column sums | None) of x (rows, cols) by one pass. panels: the
+    values as the products read them best, (cols / 64, rows, 64)."""
     x, ld = _rows_of(x)
     rows, cols = x.shape
     dev, dtype = x.device, torch.float8_e5m2 if fmt else torch.float8_e4m3fn
     q = s = qt = st = ws = sums = None
     if straight:
-        q = torch.empty(rows, _padded(cols), dtype=dtype, device=dev)
+        q = torch.empty(*((_padded(cols) // 64, rows, 64) if panels else (rows, _padded(cols))), dtype=dtype, device=dev)
         s = torch.empty((rows + 127) // 128 if tiles else rows, _words(cols), dtype=torch.uint8, device=dev)
     if transposed:
-        qt = torch.empty(cols, _padded(rows), dtype=dtype, device=dev)
+        qt = torch.empty(*((_padded(rows) // 64, cols, 64) if panels else (cols, _padded(rows))), dtype=dtype, device=dev)
         st = torch.empty((cols + 127) // 128 if tiles else cols, _words(rows), dtype=torch.uint8, device=dev)
     if colsum:
         ws = torch.empty((rows + 127) // 128, cols, device=dev)
         sums = torch.empty(cols, device=dev)
     lib = _lib.load()
     with _On(dev):
-        _lib.check(lib.siren_fp8_quantize(_p(x), _DTYPES[x.dtype], rows, cols, ld, _p(mult), fmt, int(tiles), _p(q), _p(s),
-                                          _p(qt), _p(st), _p(ws), _p(sums), _stream(dev)), 'siren_fp8_quantize')
+        _lib.check(lib.siren_fp8_quantize(_p(x), _DTYPES[x.dtype], rows, cols, ld, _p(mult), fmt, int(tiles), int(panels),
+                                          _p(q), _p(s), _p(qt), _p(st), _p(ws), _p(sums), _stream(dev)), 'siren_fp8_quantize')
     return (Blocks(q, s, cols) if straight else None), (Blocks(qt, st, rows) if transposed else None), sums
 
 
@@ -135,7 +145,7 @@ def dequantize(b):
 
 def _product(a, b, bias, act, omega, out_dtype, deriv=False):
     """act(a b^T + bias) of two Blocks quantised along the summed axis, and omega cos(omega z) in bf16 if asked for."""
-    m, n, dev = a.data.shape[0], b.data.shape[0], a.data.device
+    m, n, dev = a.rows, b.rows, a.data.device
     out = torch.empty(m, n, dtype=out_dtype, device=dev)
     # the sine's derivative meets a gradient that is rounded to 3 bits of mantissa next: 8 bits of it are enough
     d = torch.empty(m, n, dtype=torch.bfloat16, device=dev) if deriv else None
@@ -143,8 +153,8 @@ def _product(a, b, bias, act, omega, out_dtype, deriv=False):
     _lib.check(lib.siren_fp8_matmul_ws_bytes(m, n, a.cols, ctypes.byref(need)), 'siren_fp8_matmul_ws_bytes')
     ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
     with _On(dev):
-        _lib.check(lib.siren_fp8_matmul(_p(a.data), _p(a.scale), m, int(a.tiled), _FORMATS[a.data.dtype], _p(b.data),
-                                        _p(b.scale), n, int(b.tiled), a.cols, _p(bias), act, omega, _p(out),
+        _lib.check(lib.siren_fp8_matmul(_p(a.data), _p(a.scale), m, a.layout, _FORMATS[a.data.dtype], _p(b.data),
+                                        _p(b.scale), n, b.layout, a.cols, _p(bias), act, omega, _p(out),
                                         _DTYPES[out_dtype], _p(d), _p(ws), _stream(dev)), 'siren_fp8_matmul')
     return out, d
 
@@ -174,8 +184,8 @@ class _Linear(torch.autograd.Function):
         ctx.types = x.dtype, weight.dtype, None if bias is None else bias.dtype
         if not ctx.rows:  # an empty batch: no products, gradients of zero
             return x.new_empty(0, weight.shape[0])
-        qx, qxt, _ = _quantize(x, False, transposed=need_w)
-        qw, qwt, _ = _quantize(weight, True, transposed=need_x)
+        qx, qxt, _ = _quantize(x, False, transposed=need_w, panels=True)
+        qw, qwt, _ = _quantize(weight, True, transposed=need_x, panels=True)
         y, deriv = _product(qx, qw, _bias32(bias), act, omega, x.dtype, deriv=act == 1 and (need_x or need_w or need_b))
         ctx.save_for_backward(*(qxt[:2] if need_w else ()), *(qwt[:2] if need_x else ()),
                               *((deriv,) if deriv is not None else ()))
@@ -193,7 +203,8 @@ class _Linear(torch.autograd.Function):
         qxt = Blocks(saved.pop(0), saved.pop(0), ctx.rows) if need_w else None
         qwt = Blocks(saved.pop(0), saved.pop(0), n) if need_x else None
         deriv = saved.pop(0) if saved else None
-        qd, qdt, sums = _quantize(dy, False, straight=need_x, transposed=need_w, fmt=ctx.fmt, mult=deriv, colsum=need_b)
+        qd, qdt, sums = _quantize(dy, False, straight=need_x, transposed=need_w, fmt=ctx.fmt, mult=deriv, colsum=need_b,
+                                  panels=True)
         dx = _product(qd, qwt, None, 0, 0., xt)[0] if need_x else None
         dw = _product(qdt, qxt, None, 0, 0., wt)[0] if need_w else None
         return dx, dw, (sums.to(bt) if need_b else None), None, None, None

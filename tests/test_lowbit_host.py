@@ -21,7 +21,7 @@ OK, EINVAL = 0, 1
 def test_quantize_validates(lib):
     def call(x=P(64), dtype=0, rows=4, cols=8, ld=8, mult=None, fmt=0, tiles=0, q=P(64), s=P(64), qt=None, st=None,
              ws=None, sums=None):
-        return lib.siren_fp8_quantize(x, dtype, rows, cols, ld, mult, fmt, tiles, q, s, qt, st, ws, sums, None)
+        return lib.siren_fp8_quantize(x, dtype, rows, cols, ld, mult, fmt, tiles, 0, q, s, qt, st, ws, sums, None)
     assert call(rows=0) == OK and call(cols=0, ld=0) == OK
     for bad in (dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(cols=-1), dict(ld=7), dict(fmt=2), dict(s=None), dict(q=None),
                 dict(qt=P(64)), dict(st=P(64)), dict(sums=P(64)), dict(x=None), dict(q=None, s=None), dict(q=P(72)),

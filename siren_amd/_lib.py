@@ -104,7 +104,7 @@ _SIGS = {
     'siren_fp8_matmul': [_P, _P, _I64, _I32, _I32, _P, _P, _I64, _I32, _I64, _P, _I32, ctypes.c_float, _P, _I32, _P, _P,
                          _P],
     'siren_fp8_linear_ws_bytes': [_I64, _I64, _I64, ctypes.POINTER(_I64)],
-    'siren_fp8_linear': [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _I32, ctypes.c_float, _P, _P, _P],
+    'siren_fp8_linear': [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _I32, ctypes.c_float, _P, _P, _P, _P],
     'siren_adamw_scratch_bytes': [_I64, ctypes.POINTER(_I64)],
     'siren_adamw_step': [_I64, _P, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _F64, _F64, _F64, _F64, _F64, _F64,
                          ctypes.c_uint64, _P, _P],
@@ -136,6 +136,28 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_native = None
+
+
+def native():
+    """The 8-bit training operators on torch tensors (csrc/torch_binding.cpp, built beside the library), over the C ABI of
+    the library that load() loaded. As required as that library: there is no fallback."""
+    global _native
+    if _native is None:
+        lib = load()
+        import torch  # noqa: F401  (the module's own libraries)
+        try:
+            from . import _native as mod
+        except ImportError as e:
+            raise ImportError('siren_amd: the torch binding is missing or was built for another torch (%s) - build it with '
+                              '`python -c "import __graft_entry__ as g; g.build()"`' % e) from e
+        mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in
+                  ('siren_last_error', 'siren_fp8_quantize', 'siren_fp8_matmul_ws_bytes', 'siren_fp8_matmul',
+                   'siren_fp8_linear_ws_bytes', 'siren_fp8_linear', 'siren_adamw_scratch_bytes', 'siren_adamw_step')})
+        _native = mod
+    return _native
 
 
 def check(rc, what):

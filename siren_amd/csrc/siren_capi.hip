@@ -1752,26 +1752,33 @@ int32_t siren_fp8_matmul(const void* a, const void* sa, int64_t m, int32_t a_lay
 int32_t siren_fp8_linear_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes) {
     if (bytes == nullptr) return fail(SIREN_EINVAL, "bytes is NULL");
     if (int rc = check_fp8_product(m, n, k)) return rc;
-    *bytes = m == 0 || n == 0 ? 0
-                              : (m * siren::fp8_padded(k) + m * siren::fp8_scale_cols(k) + 15) / 16 * 16 +
+    *bytes = m == 0 || n == 0 || siren::fp8_few_rows(m)
+                 ? 0
+                 : (m * siren::fp8_padded(k) + m * siren::fp8_scale_cols(k) + 15) / 16 * 16 +
                                     siren::fp8_product_ws_bytes(m, n, k);
     return SIREN_OK;
 }
 
 int32_t siren_fp8_linear(const void* x, int32_t dtype, int64_t m, int64_t k, int64_t ld, const void* w, const void* sw,
-                         int64_t n, const float* bias, int32_t act, float omega, void* y, void* ws, void* stream) {
+                         int64_t n, const float* bias, int32_t act, float omega, void* y, void* deriv, void* ws, void* stream) {
     if (int rc = check_fp8_type(dtype)) return rc;
     if (int rc = check_fp8_product(m, n, k)) return rc;
-    if (int rc = check_fp8_act(act, omega, nullptr)) return rc;
+    if (int rc = check_fp8_act(act, omega, deriv)) return rc;
     if (m == 0 || n == 0) return SIREN_OK;
     if (int rc = check_fp8_source(x, dtype, m, k, ld)) return rc;
-    if (int rc = check_fp8_operands(ws, ws, w, sw, bias, y, nullptr)) return rc;
+    const bool few = siren::fp8_few_rows(m);
+    if (int rc = check_fp8_operands(few ? w : ws, few ? sw : ws, w, sw, bias, y, deriv)) return rc;
+    if (few) {
+        siren::launch_fp8_few_rows((hipStream_t)stream, x, dtype, ld, m, k, (const uint8_t*)w, (const uint8_t*)sw, n, bias,
+                                   act, omega, y, deriv);
+        return hip_status("siren_fp8_linear");
+    }
     uint8_t* q = (uint8_t*)ws;
     uint8_t* s = q + m * siren::fp8_padded(k);
     uint8_t* rest = q + (m * siren::fp8_padded(k) + m * siren::fp8_scale_cols(k) + 15) / 16 * 16;
     if (int rc = siren_fp8_quantize(x, dtype, m, k, ld, nullptr, 0, 0, 1, q, s, nullptr, nullptr, nullptr, nullptr, stream))
         return rc;
-    return siren_fp8_matmul(q, s, m, SIREN_FP8_PANELS, 0, w, sw, n, SIREN_FP8_TILES, k, bias, act, omega, y, dtype, nullptr, rest, stream);
+    return siren_fp8_matmul(q, s, m, SIREN_FP8_PANELS, 0, w, sw, n, SIREN_FP8_TILES, k, bias, act, omega, y, dtype, deriv, rest, stream);
 }
 
 int32_t siren_adamw_scratch_bytes(int64_t count, int64_t* bytes) {

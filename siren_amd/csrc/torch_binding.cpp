@@ -1,0 +1,427 @@
+// torch_binding.cpp — the 8-bit training operators on torch tensors (siren_amd/_native.so): argument checks, memory from
+// torch's caching allocator, the current stream, and the layer's autograd node, over the C ABI of libsiren_amd.so.
+//
+// Why not ctypes, as the other entry points: these calls are short. A layer's training step took 233 us of host time
+// through Python (of 110 us of kernels: the engine's own thread has to take the interpreter's lock for a Python node),
+// an AdamW step over ten tensors 29 us (of 9), a layer for one row 19 us. No kernel is here, and no copy of the C ABI: the
+// functions are taken from the library that siren_amd/_lib.py loaded (bind).
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/siren_amd.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef std::optional<Tensor> MaybeTensor;
+
+struct Library {
+    decltype(&siren_last_error) last_error;
+    decltype(&siren_fp8_quantize) quantize;
+    decltype(&siren_fp8_matmul_ws_bytes) matmul_ws_bytes;
+    decltype(&siren_fp8_matmul) matmul;
+    decltype(&siren_fp8_linear_ws_bytes) linear_ws_bytes;
+    decltype(&siren_fp8_linear) linear;
+    decltype(&siren_adamw_scratch_bytes) adamw_scratch_bytes;
+    decltype(&siren_adamw_step) adamw_step;
+} lib;
+
+void bind(const std::map<std::string, uintptr_t>& f) {
+#define SIREN_BIND(field, name) lib.field = reinterpret_cast<decltype(lib.field)>(f.at(name))
+    SIREN_BIND(last_error, "siren_last_error");
+    SIREN_BIND(quantize, "siren_fp8_quantize");
+    SIREN_BIND(matmul_ws_bytes, "siren_fp8_matmul_ws_bytes");
+    SIREN_BIND(matmul, "siren_fp8_matmul");
+    SIREN_BIND(linear_ws_bytes, "siren_fp8_linear_ws_bytes");
+    SIREN_BIND(linear, "siren_fp8_linear");
+    SIREN_BIND(adamw_scratch_bytes, "siren_adamw_scratch_bytes");
+    SIREN_BIND(adamw_step, "siren_adamw_step");
+#undef SIREN_BIND
+}
+
+// a status of the C ABI as the exception that siren_amd/_lib.py raises for it
+void check(int32_t rc, const char* what) {
+    if (rc == SIREN_OK) return;
+    TORCH_CHECK_VALUE(rc != SIREN_EINVAL, what, ": ", lib.last_error());
+    TORCH_CHECK(false, what, " failed (", rc, "): ", lib.last_error());
+}
+
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+int type_code(at::ScalarType t) {
+    return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1;
+}
+int format_code(at::ScalarType t) { return t == at::kFloat8_e4m3fn ? 0 : t == at::kFloat8_e5m2 ? 1 : -1; }
+
+void check_input(const Tensor& x, const char* what) {
+    TORCH_CHECK(x.is_cuda(), "siren_amd.fp8 runs on ROCm devices (MI355X) only; got a ", x.device().type(), " tensor as ", what);
+    TORCH_CHECK_TYPE(type_code(x.scalar_type()) >= 0, what, " must be fp32, bf16 or fp16; got ", x.scalar_type());
+    TORCH_CHECK_TYPE(x.layout() == at::kStrided, what, " must be a dense tensor");
+}
+
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+int64_t padded(int64_t n) { return blocks(n) * 128; }
+int64_t words(int64_t n) { return (blocks(n) + 3) / 4 * 4; }
+
+// A quantised (rows, cols) tensor: values in rows (rows, padded cols) or in panels (padded cols / 64, rows, 64)
+struct Blocks {
+    Tensor data, scale;
+    int64_t rows = 0, cols = 0;
+    int layout = 0;
+};
+
+// x as the kernels read it: columns one element apart, rows any distance that does not overlap
+Tensor rows_of(const Tensor& x, int64_t& ld) {
+    const int64_t r = x.size(0), c = x.size(1);
+    Tensor y = (c <= 1 || x.stride(1) == 1) && (r <= 1 || x.stride(0) >= c) ? x : x.contiguous();
+    ld = r > 1 ? y.stride(0) : c;
+    return y;
+}
+
+enum Want { STRAIGHT = 1, TRANSPOSED = 2, PANELS = 4, TRANSPOSED_PANELS = 8, TILES = 16 };
+
+// One pass over x (times mult): its rows, its transpose's rows, its column sums, as wanted. Rows and panels may differ
+// between the two directions: then the pass is made twice.
+void quantize_into(const Tensor& x0, int want, int fmt, const Tensor& mult, Blocks* q, Blocks* qt, Tensor* colsum) {
+    int64_t ld;
+    const Tensor x = rows_of(x0, ld);
+    const int64_t rows = x.size(0), cols = x.size(1);
+    const auto bytes = x.options().dtype(fmt ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn);
+    const auto u8 = x.options().dtype(at::kByte);
+    const bool tiles = want & TILES;
+    auto make = [&](Blocks* b, int64_t r, int64_t c, bool panels) {
+        b->data = panels ? at::empty({padded(c) / 64, r, 64}, bytes) : at::empty({r, padded(c)}, bytes);
+        b->scale = at::empty({tiles ? blocks(r) : r, words(c)}, u8);
+        b->rows = r;
+        b->cols = c;
+        b->layout = (tiles ? SIREN_FP8_TILES : 0) | (panels ? SIREN_FP8_PANELS : 0);
+    };
+    if (q) make(q, rows, cols, want & PANELS);
+    if (qt) make(qt, cols, rows, want & TRANSPOSED_PANELS);
+    Tensor ws;
+    if (colsum) {
+        const auto f32 = x.options().dtype(at::kFloat);
+        ws = at::empty({blocks(rows), cols}, f32);
+        *colsum = at::empty({cols}, f32);
+    }
+    auto pass = [&](Blocks* a, Blocks* t, Tensor* sums, bool panels) {
+        check(lib.quantize(x.data_ptr(), type_code(x.scalar_type()), rows, cols, ld, mult.defined() ? mult.data_ptr() : nullptr,
+                           fmt, tiles, panels, a ? a->data.data_ptr() : nullptr, a ? a->scale.data_ptr() : nullptr,
+                           t ? t->data.data_ptr() : nullptr, t ? t->scale.data_ptr() : nullptr,
+                           sums ? ws.data_ptr<float>() : nullptr, sums ? sums->data_ptr<float>() : nullptr, stream_of(x)),
+              "siren_fp8_quantize");
+    };
+    const bool same = !q || !qt || bool(want & PANELS) == bool(want & TRANSPOSED_PANELS);
+    if (same) {
+        pass(q, qt, colsum, q ? want & PANELS : want & TRANSPOSED_PANELS);
+    } else {
+        pass(q, nullptr, colsum, want & PANELS);
+        pass(nullptr, qt, nullptr, want & TRANSPOSED_PANELS);
+    }
+}
+
+Tensor product(const Blocks& a, const Blocks& b, const Tensor& bias, int act, double omega, at::ScalarType type, Tensor* deriv) {
+    const auto opt = a.scale.options();
+    Tensor out = at::empty({a.rows, b.rows}, opt.dtype(type));
+    // the sine's derivative meets a gradient that is rounded to 3 bits of mantissa next: 8 bits of it are enough
+    if (deriv) *deriv = at::empty({a.rows, b.rows}, opt.dtype(at::kBFloat16));
+    int64_t need = 0;
+    check(lib.matmul_ws_bytes(a.rows, b.rows, a.cols, &need), "siren_fp8_matmul_ws_bytes");
+    Tensor ws;
+    if (need) ws = at::empty({need}, opt);
+    check(lib.matmul(a.data.data_ptr(), a.scale.data_ptr(), a.rows, a.layout, format_code(a.data.scalar_type()),
+                     b.data.data_ptr(), b.scale.data_ptr(), b.rows, b.layout, a.cols,
+                     bias.defined() ? bias.data_ptr<float>() : nullptr, act, (float)omega, out.data_ptr(), type_code(type),
+                     deriv ? deriv->data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, stream_of(a.scale)),
+          "siren_fp8_matmul");
+    return out;
+}
+
+// act(x w^T + bias) in one call of the C ABI; w: rows, tiles
+Tensor serve(const Tensor& x0, const Blocks& w, const Tensor& bias, int act, double omega, Tensor* deriv) {
+    int64_t ld;
+    const Tensor x = rows_of(x0, ld);
+    const int64_t m = x.size(0), k = x.size(1);
+    Tensor y = at::empty({m, w.rows}, x.options());
+    if (deriv) *deriv = at::empty({m, w.rows}, x.options().dtype(at::kBFloat16));
+    int64_t need = 0;
+    check(lib.linear_ws_bytes(m, w.rows, k, &need), "siren_fp8_linear_ws_bytes");
+    Tensor ws;
+    if (need) ws = at::empty({need}, x.options().dtype(at::kByte));
+    check(lib.linear(x.data_ptr(), type_code(x.scalar_type()), m, k, ld, w.data.data_ptr(), w.scale.data_ptr(), w.rows,
+                     bias.defined() ? bias.data_ptr<float>() : nullptr, act, (float)omega, y.data_ptr(),
+                     deriv ? deriv->data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, stream_of(x)),
+          "siren_fp8_linear");
+    return y;
+}
+
+Tensor bias32(const Tensor& bias) { return bias.defined() ? bias.detach().to(at::kFloat).contiguous() : bias; }
+
+// Gradients of gradients: the values pass, a backward through them says why there is none
+struct NotTwice : torch::autograd::Function<NotTwice> {
+    static Tensor forward(AutogradContext*, const Tensor& g, const Tensor&) { return g.detach(); }
+    static variable_list backward(AutogradContext*, const variable_list&) {
+        TORCH_CHECK(false, "fp8.linear: its gradients are not differentiable again (second derivatives need the fp32 kernels)");
+    }
+};
+
+// y = act(x W^T + b) with gradients. x is read once in the forward and dy once in the backward, each quantised both along
+// its rows and along its columns in that pass; the weight's tiles serve both directions.
+struct Linear : torch::autograd::Function<Linear> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t act,
+                          double omega, int64_t fmt) {
+        const bool nx = x.requires_grad(), nw = weight.requires_grad(), nb = bias.defined() && bias.requires_grad();
+        const int64_t m = x.size(0), n = weight.size(0), k = weight.size(1);
+        ctx->saved_data["dims"] = std::vector<int64_t>{m, n, k, fmt, nx, nw, nb};
+        ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(),
+                                                        bias.defined() ? (int64_t)bias.scalar_type() : 0};
+        if (m == 0) return x.new_empty({0, n});  // no products, gradients of zero
+        const c10::DeviceGuard guard(x.device());
+        const Tensor xd = x.detach(), b32 = bias32(bias);
+        Blocks qx, qxt, qw, qwt;
+        Tensor deriv, y;
+        Tensor* want_deriv = act && (nx || nw || nb) ? &deriv : nullptr;
+        int64_t ws = 0;
+        check(lib.linear_ws_bytes(m, n, k, &ws), "siren_fp8_linear_ws_bytes");
+        if (ws == 0) {  // few rows: the product quantises them itself, and reads the weight in rows
+            quantize_into(weight.detach(), TILES | TRANSPOSED_PANELS, 0, Tensor(), &qw, nx ? &qwt : nullptr, nullptr);
+            y = serve(xd, qw, b32, (int)act, omega, want_deriv);
+            if (nw) quantize_into(xd, TRANSPOSED_PANELS, 0, Tensor(), nullptr, &qxt, nullptr);
+        } else {
+            quantize_into(xd, PANELS | TRANSPOSED_PANELS, 0, Tensor(), &qx, nw ? &qxt : nullptr, nullptr);
+            quantize_into(weight.detach(), TILES | PANELS | TRANSPOSED_PANELS, 0, Tensor(), &qw, nx ? &qwt : nullptr, nullptr);
+            y = product(qx, qw, b32, (int)act, omega, x.scalar_type(), want_deriv);
+        }
+        ctx->save_for_backward({qxt.data, qxt.scale, qwt.data, qwt.scale, deriv});
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const auto dims = ctx->saved_data["dims"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
+        const int64_t m = dims[0], n = dims[1], k = dims[2], fmt = dims[3];
+        const bool nx = dims[4], nw = dims[5], nb = dims[6];
+        const auto tx = (at::ScalarType)types[0], tw = (at::ScalarType)types[1], tb = (at::ScalarType)types[2];
+        Tensor dx, dw, db;
+        const Tensor dy = grads[0];
+        if (!dy.defined()) return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+        const auto opt = dy.options();
+        if (m == 0) {
+            if (nx) dx = at::empty({0, k}, opt.dtype(tx));
+            if (nw) dw = at::zeros({n, k}, opt.dtype(tw));
+            if (nb) db = at::zeros({n}, opt.dtype(tb));
+            return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+        }
+        const c10::DeviceGuard guard(dy.device());
+        const auto saved = ctx->get_saved_variables();
+        const bool create_graph = at::GradMode::is_enabled();
+        {
+            const at::NoGradGuard none;
+            Blocks q, qt;
+            Tensor sums;
+            quantize_into(dy.detach(), PANELS | TRANSPOSED_PANELS, (int)fmt, saved[4], nx ? &q : nullptr, nw ? &qt : nullptr,
+                          nb ? &sums : nullptr);
+            if (nx) dx = product(q, {saved[2], saved[3], k, n, SIREN_FP8_TILES | SIREN_FP8_PANELS}, Tensor(), 0, 0., tx, nullptr);
+            if (nw) dw = product(qt, {saved[0], saved[1], k, m, SIREN_FP8_PANELS}, Tensor(), 0, 0., tw, nullptr);
+            if (nb) db = sums.to(tb);
+        }
+        if (create_graph) {
+            const Tensor anchor = at::empty({0}, opt.dtype(at::kFloat)).requires_grad_(true);
+            for (Tensor* g : {&dx, &dw, &db})
+                if (g->defined()) *g = NotTwice::apply(*g, anchor);
+        }
+        return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor check_layer(const Tensor& x, const Tensor& bias, int64_t n, int64_t k, double omega) {
+    check_input(x, "x");
+    TORCH_CHECK_VALUE(x.dim() >= 1, "x must be (..., in)");
+    TORCH_CHECK_VALUE(n >= 1 && k >= 1, "weight must have rows and columns; got (", n, ", ", k, ")");
+    TORCH_CHECK_VALUE(x.size(-1) == k, "x must be (..., ", k, ") for this weight; got ", x.sizes());
+    TORCH_CHECK_VALUE(std::isfinite(omega), "omega must be finite");
+    if (bias.defined()) {
+        check_input(bias, "bias");
+        TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == n && bias.device() == x.device(), "bias must be (", n, ",) on ",
+                          x.device(), "; got ", bias.sizes(), " on ", bias.device());
+    }
+    return x.dim() == 2 ? x : x.reshape({-1, k});
+}
+
+Tensor like_input(const Tensor& x, const Tensor& y) {
+    if (x.dim() == 2) return y;
+    auto shape = x.sizes().vec();
+    shape.back() = y.size(1);
+    return y.view(shape);
+}
+
+Blocks packed_operand(const Tensor& data, const Tensor& scale, int64_t cols, const at::Device& dev, bool tiles_only) {
+    TORCH_CHECK(data.is_cuda(), "siren_amd.fp8 runs on ROCm devices (MI355X) only; got a ", data.device().type(), " tensor");
+    TORCH_CHECK_TYPE(format_code(data.scalar_type()) >= 0 && scale.scalar_type() == at::kByte,
+                     "Blocks are e4m3 or e5m2 with uint8 scales; got ", data.scalar_type(), " and ", scale.scalar_type());
+    TORCH_CHECK_VALUE(data.dim() == 2 && scale.dim() == 2 && cols >= 1 && data.size(1) == padded(cols) &&
+                          scale.size(1) == words(cols) &&
+                          (scale.size(0) == blocks(data.size(0)) || (!tiles_only && scale.size(0) == data.size(0))),
+                      "Blocks of ", cols, " columns are quantize()'s: data (rows, ", padded(cols), "), scale (rows or ceil(rows / 128), ",
+                      words(cols), ")", tiles_only ? "; a weight is quantize(weight, 'tile')" : "", "; got ", data.sizes(), " and ",
+                      scale.sizes());
+    TORCH_CHECK_VALUE(data.is_contiguous() && scale.is_contiguous() && (uintptr_t)data.data_ptr() % 16 == 0 &&
+                          (uintptr_t)scale.data_ptr() % 4 == 0,
+                      "Blocks must be contiguous, their data 16-byte and their scales 4-byte aligned");
+    TORCH_CHECK_VALUE(data.device() == dev && scale.device() == dev, "Blocks on ", data.device(), " but the other operand on ", dev);
+    // one row is both: its tile is its row block
+    return {data, scale, data.size(0), cols, tiles_only || scale.size(0) != data.size(0) ? SIREN_FP8_TILES : 0};
+}
+
+std::pair<Tensor, Tensor> quantize(const Tensor& x, bool tiles, int64_t fmt) {
+    check_input(x, "x");
+    TORCH_CHECK_VALUE(x.dim() == 2, "x must be (rows, cols); got ", x.sizes());
+    const c10::DeviceGuard guard(x.device());
+    Blocks q;
+    quantize_into(x.detach(), tiles ? TILES : 0, (int)fmt, Tensor(), &q, nullptr, nullptr);
+    return {q.data, q.scale};
+}
+
+std::vector<Tensor> quantize_both(const Tensor& x, bool tiles, int64_t fmt) {
+    check_input(x, "x");
+    TORCH_CHECK_VALUE(x.dim() == 2, "x must be (rows, cols); got ", x.sizes());
+    const c10::DeviceGuard guard(x.device());
+    Blocks q, qt;
+    quantize_into(x.detach(), tiles ? TILES : 0, (int)fmt, Tensor(), &q, &qt, nullptr);
+    return {q.data, q.scale, qt.data, qt.scale};
+}
+
+std::pair<Tensor, MaybeTensor> matmul(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, int64_t cols,
+                                      const MaybeTensor& bias, int64_t act, double omega, at::ScalarType type, bool derivative) {
+    const Blocks qa = packed_operand(a, sa, cols, a.device(), false), qb = packed_operand(b, sb, cols, a.device(), false);
+    TORCH_CHECK_TYPE(b.scalar_type() == at::kFloat8_e4m3fn, "the second operand must be e4m3; got ", b.scalar_type());
+    TORCH_CHECK_TYPE(type_code(type) >= 0, "dtype must be fp32, bf16 or fp16; got ", type);
+    TORCH_CHECK_VALUE(std::isfinite(omega), "omega must be finite");
+    Tensor b32;
+    if (bias) {
+        check_input(*bias, "bias");
+        TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == qb.rows && bias->device() == a.device(), "bias must be (", qb.rows, ",)");
+        b32 = bias32(*bias);
+    }
+    const c10::DeviceGuard guard(a.device());
+    Tensor d;
+    Tensor y = product(qa, qb, b32, (int)act, omega, type, derivative ? &d : nullptr);
+    return {y, derivative ? MaybeTensor(d) : std::nullopt};
+}
+
+Tensor linear_packed(const Tensor& x, const Tensor& data, const Tensor& scale, int64_t cols, const MaybeTensor& maybe_bias,
+                     int64_t act, double omega) {
+    const Tensor bias = maybe_bias.value_or(Tensor());
+    check_input(x, "x");
+    const Blocks w = packed_operand(data, scale, cols, x.device(), true);
+    TORCH_CHECK_TYPE(data.scalar_type() == at::kFloat8_e4m3fn, "a weight in 8 bits is e4m3; got ", data.scalar_type());
+    const Tensor x2 = check_layer(x, bias, w.rows, cols, omega);
+    TORCH_CHECK(!(at::GradMode::is_enabled() && (x.requires_grad() || (bias.defined() && bias.requires_grad()))),
+                "fp8.linear: a weight held in 8 bits is forward only; use torch.no_grad(), or pass the weight itself to train");
+    const c10::DeviceGuard guard(x.device());
+    return like_input(x, serve(x2.detach(), w, bias32(bias), (int)act, omega, nullptr));
+}
+
+Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& maybe_bias, int64_t act, double omega, int64_t fmt) {
+    const Tensor bias = maybe_bias.value_or(Tensor());
+    check_input(x, "x");
+    check_input(weight, "weight");
+    TORCH_CHECK_VALUE(weight.dim() == 2, "weight must be (out, in); got ", weight.sizes());
+    TORCH_CHECK_VALUE(weight.device() == x.device(), "weight on ", weight.device(), " but x on ", x.device());
+    const Tensor x2 = check_layer(x, bias, weight.size(0), weight.size(1), omega);
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad())))
+        return like_input(x, Linear::apply(x2, weight, bias, act, omega, fmt));
+    const c10::DeviceGuard guard(x.device());
+    Blocks w;
+    quantize_into(weight.detach(), TILES, 0, Tensor(), &w, nullptr, nullptr);
+    return like_input(x, serve(x2.detach(), w, bias32(bias), (int)act, omega, nullptr));
+}
+
+MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<MaybeTensor>& grads, const Tensor& m, const Tensor& v,
+                       const Tensor& step, double lr, double b1, double b2, double eps, double weight_decay,
+                       std::optional<double> max_norm, uint64_t seed, const MaybeTensor& sm, const MaybeTensor& sv) {
+    const size_t n = params.size();
+    TORCH_CHECK_VALUE(n >= 1 && grads.size() == n, "adamw_step needs as many gradients as parameters, one at least; got ",
+                      grads.size(), " and ", n);
+    const at::Device dev = params[0].device();
+    TORCH_CHECK(dev.is_cuda(), "adamw_step runs on ROCm devices (MI355X) only; got a ", dev.type(), " tensor");
+    std::vector<void*> ps(n);
+    std::vector<const void*> gs(n);
+    std::vector<int64_t> numels(n);
+    std::vector<int32_t> types(n);
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    spans.reserve(n);
+    std::vector<Tensor> keep;
+    int64_t size = 0;
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor& p = params[i];
+        types[i] = type_code(p.scalar_type());
+        TORCH_CHECK(types[i] >= 0 && p.device() == dev, "adamw_step needs fp32, bf16 or fp16 parameters on one device; got ",
+                    p.scalar_type(), " on ", p.device());
+        TORCH_CHECK_VALUE(p.is_contiguous(), "adamw_step needs contiguous parameters; parameter ", i, " has strides ", p.strides());
+        ps[i] = p.data_ptr();
+        gs[i] = nullptr;
+        if (grads[i]) {
+            const Tensor& g = *grads[i];
+            TORCH_CHECK_VALUE(g.layout() == at::kStrided && g.sizes() == p.sizes() && g.scalar_type() == p.scalar_type() &&
+                                  g.device() == dev,
+                              "gradient ", i, " must be ", p.sizes(), " ", p.scalar_type(), " on ", dev, "; got ", g.sizes(), " ",
+                              g.scalar_type(), " on ", g.device());
+            if (g.is_contiguous()) {
+                gs[i] = g.data_ptr();
+            } else {
+                keep.push_back(g.contiguous());
+                gs[i] = keep.back().data_ptr();
+            }
+        }
+        numels[i] = p.numel();
+        if (numels[i] > 0) spans.emplace_back((uintptr_t)ps[i], (uintptr_t)ps[i] + p.nbytes());
+        size += padded(numels[i]);
+    }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first, "adamw_step: parameters overlap (is one listed twice?)");
+    TORCH_CHECK_VALUE(bool(sm) == bool(sv), "scales must be two tensors");
+    const auto want = sm ? at::kFloat8_e4m3fn : at::kFloat;
+    const std::pair<const char*, const Tensor*> states[2] = {{"exp_avg", &m}, {"exp_avg_sq", &v}};
+    for (const auto& s : states)
+        TORCH_CHECK_VALUE(s.second->scalar_type() == want && s.second->numel() == size && s.second->device() == dev &&
+                              s.second->is_contiguous() && (uintptr_t)s.second->data_ptr() % 16 == 0,
+                          s.first, " must be ", size, " contiguous 16-byte aligned values of ", want, " on ", dev, "; got ",
+                          s.second->numel(), " of ", s.second->scalar_type(), " on ", s.second->device());
+    if (sm)
+        for (const Tensor* s : {&*sm, &*sv})
+            TORCH_CHECK_VALUE(s->scalar_type() == at::kByte && s->numel() == size / 128 && s->device() == dev && s->is_contiguous(),
+                              "scales must be two tensors of ", size / 128, " contiguous uint8 on ", dev);
+    TORCH_CHECK_VALUE(step.scalar_type() == at::kLong && step.numel() == 1 && step.device() == dev, "step must be one int64 on ", dev);
+    TORCH_CHECK_VALUE(!max_norm || *max_norm > 0., "max_norm must be positive or None; got ", max_norm.value_or(0.));
+    int64_t need = 0;
+    check(lib.adamw_scratch_bytes((int64_t)n, &need), "siren_adamw_scratch_bytes");
+    const c10::DeviceGuard guard(dev);
+    const Tensor scratch = at::empty({need / 4}, step.options().dtype(at::kFloat));
+    check(lib.adamw_step((int64_t)n, ps.data(), gs.data(), numels.data(), types.data(), sm ? 8 : 32, m.data_ptr(), v.data_ptr(),
+                         sm ? sm->data_ptr() : nullptr, sv ? sv->data_ptr() : nullptr, step.data_ptr<int64_t>(), lr, b1, b2, eps,
+                         weight_decay, max_norm.value_or(0.), seed, scratch.data_ptr(), stream_of(step)),
+          "siren_adamw_step");
+    return max_norm ? MaybeTensor(scratch.select(0, 8)) : std::nullopt;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_native, m) {
+    m.def("bind", &bind);
+    m.def("quantize", &quantize);
+    m.def("quantize_both", &quantize_both);
+    m.def("matmul", [](const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, int64_t cols, const MaybeTensor& bias,
+                       int64_t act, double omega, py::object dtype, bool derivative) {
+        return matmul(a, sa, b, sb, cols, bias, act, omega, torch::python::detail::py_object_to_dtype(dtype), derivative);
+    });
+    m.def("linear_packed", &linear_packed);
+    m.def("linear", &linear);
+    m.def("adamw_step", &adamw_step);
+}

@@ -15,15 +15,13 @@
 // lanes that read one piece of 16 rows hit distinct banks. The sums do not care in which order k is taken as long as both
 // operands agree, so a lane's 16 contiguous bytes serve two instructions of 8.
 #include "fp8.h"
+#include "fp8_device.h"
 #include "siren_common.h"
 
 namespace siren {
 
 namespace {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int TN = 128;  // columns of a workgroup's tile
@@ -44,21 +42,6 @@ struct GemmArgs {
     void* out;                   // split: fp32 partial products (splits, m, n)
     __bf16* deriv;
 };
-
-template <bool E5M2, int HI>
-__device__ __forceinline__ bf16x2 widen2(uint32_t w, float scale) {
-    if constexpr (E5M2)
-        return __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, scale, HI);
-    else
-        return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI);
-}
-// 8 bytes (two words) -> 8 bf16 numbers, times scale
-template <bool E5M2>
-__device__ __forceinline__ bf16x8 widen8(uint32_t w0, uint32_t w1, float scale) {
-    const bf16x2 p0 = widen2<E5M2, 0>(w0, scale), p1 = widen2<E5M2, 1>(w0, scale);
-    const bf16x2 p2 = widen2<E5M2, 0>(w1, scale), p3 = widen2<E5M2, 1>(w1, scale);
-    return bf16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
-}
 
 template <typename T>
 __device__ __forceinline__ void put4(T* dst, f32x4 v, int valid, bool vec) {
@@ -313,6 +296,94 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
     }
 }
 
+// A layer of a few rows (up to 32) in one launch: what it cannot do without is the weight's bytes. A workgroup owns 64
+// columns, a wave 16 of them: it asks for its weights of FEW_K k first, all waves round that much of x to 8 bits into LDS
+// while they travel (half a wave a block), then the wave's rows of the weight times the rows of x, 16 at a time.
+constexpr int FEW_ROWS = 32, FEW_K = 512, FEW_LD = FEW_K + 16;  // LDS rows 16 bytes apart from a bank period
+struct FewArgs {
+    const void* x;
+    int64_t ld, m, k;
+    const uint8_t *w, *sw;
+    int vec;
+    GemmArgs out;  // n, bias, act, omega, out
+};
+template <typename T, int MT>
+__global__ __launch_bounds__(256) void few_rows_kernel(FewArgs f) {
+    __shared__ __align__(16) uint8_t xq[MT * 16 * FEW_LD];
+    __shared__ uint8_t xs[MT * 16 * (FEW_K / 128)];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = lane & 15, q = lane >> 4;
+    const GemmArgs& g = f.out;
+    const int64_t n0 = (int64_t)blockIdx.x * 64 + wave * 16;
+    const int64_t wrow = n0 + r < g.n ? n0 + r : g.n - 1;  // rows past the end read the last one and store nothing
+    const int64_t kp = (f.k + 127) / 128 * 128;
+    const int blocks = (int)(kp / 128);
+    const uint8_t* w = f.w + wrow * kp + q * 16;
+    const uint8_t* sw = f.sw + (wrow >> 7) * ((blocks + 3) / 4 * 4);
+    f32x4 acc[MT] = {};
+    for (int b0 = 0; b0 < blocks; b0 += FEW_K / 128) {
+        const int here = blocks - b0 < FEW_K / 128 ? blocks - b0 : FEW_K / 128;
+        u32x4 wv[FEW_K / 128][2];
+        const uint32_t scales = *(const uint32_t*)(sw + b0);
+#pragma unroll
+        for (int b = 0; b < FEW_K / 128; ++b) {
+            const int at = (b0 + (b < here ? b : 0)) * 128;
+            wv[b][0] = *(const u32x4*)(w + at);
+            wv[b][1] = *(const u32x4*)(w + at + 64);
+        }
+        if (b0 > 0) __syncthreads();  // x of the chunk before has been read
+        const int c4 = threadIdx.x & 31, units = here * (int)f.m;
+        for (int u = threadIdx.x >> 5; u < MT * 16 * here; u += 8) {
+            const int row = u / here, b = u - row * here;
+            const int64_t c0 = (int64_t)(b0 + b) * 128 + c4 * 4, left = f.k - c0;
+            uint32_t codes = 0;
+            int byte = 127;
+            if (u < units) {
+                float v[4];
+                load_quad((const T*)f.x + row * f.ld + c0, left < 4 ? (left > 0 ? (int)left : 0) : 4, f.vec != 0, v);
+                byte = exponent_byte<false>(half_wave_max(fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])),
+                                                                fmaxf(finite_abs(v[2]), finite_abs(v[3])))));
+                const float inv = inverse_scale(byte);
+                codes = pack4<false>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+            }
+            *(uint32_t*)(xq + row * FEW_LD + b * 128 + c4 * 4) = codes;
+            if (c4 == 0) xs[row * (FEW_K / 128) + b] = (uint8_t)byte;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < FEW_K / 128; ++b) {
+            if (b < here) {
+                const float fw = __uint_as_float(((scales >> (8 * b)) & 0xFFu) << 23);
+                bf16x8 wf[4];
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    wf[2 * p] = widen8<false>(wv[b][p][0], wv[b][p][1], fw);
+                    wf[2 * p + 1] = widen8<false>(wv[b][p][2], wv[b][p][3], fw);
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const int row = t * 16 + r;
+                    const float fx = __uint_as_float((uint32_t)xs[row * (FEW_K / 128) + b] << 23);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const u32x4 c = *(const u32x4*)(xq + row * FEW_LD + b * 128 + p * 64 + q * 16);
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[2 * p], widen8<false>(c[0], c[1], fx), acc[t], 0, 0, 0);
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[2 * p + 1], widen8<false>(c[2], c[3], fx), acc[t], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    // the weight's rows are the instruction's rows: lane (r, q) holds y[r][n0 + 4 q ..]
+    const int64_t col = n0 + 4 * q;
+    if (col < g.n) {
+        const Finish<T> to(g, col);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            if (t * 16 + r < f.m) to.store(g, t * 16 + r, acc[t]);
+    }
+}
+
 // out = act(sum of the splits' partial products + bias), four columns a thread. GROUPS threads share an element's splits,
 // each its own contiguous run of them, and are added in order: few outputs with many splits (a reduction over 65536)
 // would otherwise leave most of the card idle behind one long chain of loads (33 us for 32 x 256 of 128 splits).
@@ -391,6 +462,39 @@ void launch_gemm(hipStream_t stream, GemmArgs& g, int splits, bool rows256) {
 }
 
 }  // namespace
+
+bool fp8_few_rows(int64_t m) { return m <= FEW_ROWS; }
+
+void launch_fp8_few_rows(hipStream_t stream, const void* x, int type, int64_t ld, int64_t m, int64_t k, const uint8_t* w,
+                         const uint8_t* sw, int64_t n, const float* bias, int act, float omega, void* y, void* deriv) {
+    FewArgs f = {};
+    f.x = x;
+    f.ld = ld;
+    f.m = m;
+    f.k = k;
+    f.w = w;
+    f.sw = sw;
+    f.vec = (uintptr_t)x % (type == FP8_F32 ? 16 : 8) == 0 && (ld % 4 == 0 || m == 1);
+    f.out.m = m;
+    f.out.n = n;
+    f.out.bias = bias;
+    f.out.act = act;
+    f.out.omega = omega;
+    f.out.out = y;
+    f.out.deriv = (__bf16*)deriv;
+    const dim3 grid((unsigned)((n + 63) / 64));
+#define SIREN_FEW(T)                                                                               \
+    do {                                                                                           \
+        if (m <= 16)                                                                               \
+            hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, dim3(256), 0, stream, f);            \
+        else                                                                                       \
+            hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, dim3(256), 0, stream, f);            \
+    } while (0)
+    if (type == FP8_F32) SIREN_FEW(float);
+    if (type == FP8_BF16) SIREN_FEW(__bf16);
+    if (type == FP8_F16) SIREN_FEW(_Float16);
+#undef SIREN_FEW
+}
 
 int64_t fp8_product_ws_bytes(int64_t m, int64_t n, int64_t k) {
     const int s = splits_of(m, n, k);

@@ -9,40 +9,15 @@
 // column sums of a bias's gradient on the way, so the tensor is read once. 64 values a thread: 16 rows x 4 columns, so
 // a row's maximum is a reduction over half a wave, a column's one over LDS, and the transpose leaves as 16-byte pieces.
 #include "fp8.h"
+#include "fp8_device.h"
 #include "siren_common.h"
 
 namespace siren {
 
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int QT = 128;           // tile edge
 constexpr int QSTRIDE = QT + 16;  // LDS row of the transposed bytes: 16-byte pieces on distinct banks
-
-__device__ __forceinline__ float finite_abs(float x) {
-    const float a = __builtin_fabsf(x);
-    return a < INFINITY ? a : 0.f;
-}
-
-// the exponent byte of a block whose largest finite magnitude is amax: 448 = 1.75 * 2^8, 57344 = 1.75 * 2^15
-template <bool E5M2>
-__device__ __forceinline__ int exponent_byte(float amax) {
-    const uint32_t b = __float_as_uint(amax);
-    const int e = (int)(b >> 23) - (E5M2 ? 15 : 8) + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-    return e < 1 ? 1 : e;
-}
-__device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
-
-template <bool E5M2>
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-    if constexpr (E5M2) {
-        const int lo = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false);
-        return (uint32_t)__builtin_amdgcn_cvt_pk_bf8_f32(c, d, lo, true);
-    } else {
-        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
-    }
-}
 
 template <typename T, bool E5M2>
 __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
@@ -154,9 +129,7 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
             if (!tiles) {
                 float m = fmaxf(fmaxf(finite_abs(v[i][0]), finite_abs(v[i][1])),
                                 fmaxf(finite_abs(v[i][2]), finite_abs(v[i][3])));
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-                byte = exponent_byte<E5M2>(m);
+                byte = exponent_byte<E5M2>(half_wave_max(m));
             }
             if (r0 + i < rows) {
                 const float inv = inverse_scale(byte);
@@ -231,6 +204,45 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
     }
 }
 
+// Rows alone, nothing transposed (a layer that is only evaluated): half a wave takes one block of a row, a workgroup one
+// block of 32 rows, 4 a half wave, all loaded before any is reduced. A few rows are a matter of latency here (the tile
+// kernel above is thousands of instructions long, 8 us for one row), many one of bytes.
+constexpr int ROWS_PER_GROUP = 32;
+template <typename T, bool E5M2>
+__global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                                         uint8_t* __restrict__ q, uint8_t* __restrict__ s, int vec,
+                                                         int col_blocks, int panels) {
+    const int c4 = threadIdx.x & 31, unit = threadIdx.x >> 5;
+    const int64_t rb = blockIdx.x / col_blocks;
+    const int cb = (int)(blockIdx.x % col_blocks);
+    const int64_t c0 = (int64_t)cb * QT + c4 * 4;
+    const int64_t left = cols - c0;
+    const int valid = left < 4 ? (left > 0 ? (int)left : 0) : 4;
+    const int64_t s_ld = (col_blocks + 3) / 4 * 4;
+    float v[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = rb * ROWS_PER_GROUP + i * 8 + unit;
+        load_quad(x + (r < rows ? r : rows - 1) * ld + c0, valid, vec != 0, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = rb * ROWS_PER_GROUP + i * 8 + unit;
+        const float m = half_wave_max(fmaxf(fmaxf(finite_abs(v[i][0]), finite_abs(v[i][1])),
+                                            fmaxf(finite_abs(v[i][2]), finite_abs(v[i][3]))));
+        const int byte = exponent_byte<E5M2>(m);
+        const float inv = inverse_scale(byte);
+        if (r < rows) {
+            uint8_t* dst = panels ? q + ((cb * 2 + (c4 >> 4)) * rows + r) * 64 + (c4 & 15) * 4
+                                  : q + r * ((int64_t)col_blocks * QT) + c0;
+            *(uint32_t*)dst = pack4<E5M2>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+            // the pad bytes of a row's last word stand for 1
+            if (c4 == 0) s[r * s_ld + cb] = (uint8_t)byte;
+            if (cb == col_blocks - 1 && c4 > 0 && cb + c4 < s_ld) s[r * s_ld + cb + c4] = 127;
+        }
+    }
+}
+
 // out[c] = sum_b colsum[b][c] in 64 bits: 32 columns x 32 groups of row blocks a workgroup, the groups joined in a fixed
 // order (4 groups of 64 columns left 16 workgroups for 1024 columns: 213 us for 2048 row blocks)
 __global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ colsum, int64_t blocks, int64_t cols,
@@ -257,6 +269,20 @@ void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
     const int64_t col_blocks = fp8_blocks(a.cols), grid = fp8_blocks(a.rows) * col_blocks;
     const int64_t size = a.type == FP8_F32 ? 4 : 2;
     const int vec = ((uintptr_t)a.x % (4 * size)) == 0 && (a.ld % 4 == 0 || a.rows == 1);
+    if (a.qt == nullptr && a.colsum == nullptr && a.mult == nullptr && !a.tiles) {
+        const int64_t groups = (a.rows + ROWS_PER_GROUP - 1) / ROWS_PER_GROUP * col_blocks;
+#define SIREN_QUANT_ROWS(T, E)                                                                                           \
+    hipLaunchKernelGGL((quant_rows_kernel<T, E>), dim3((unsigned)groups), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
+                       a.cols, a.q, a.s, vec, (int)col_blocks, a.panels)
+        if (a.type == FP8_F32 && a.e5m2) SIREN_QUANT_ROWS(float, true);
+        if (a.type == FP8_BF16 && a.e5m2) SIREN_QUANT_ROWS(__bf16, true);
+        if (a.type == FP8_F16 && a.e5m2) SIREN_QUANT_ROWS(_Float16, true);
+        if (a.type == FP8_F32 && !a.e5m2) SIREN_QUANT_ROWS(float, false);
+        if (a.type == FP8_BF16 && !a.e5m2) SIREN_QUANT_ROWS(__bf16, false);
+        if (a.type == FP8_F16 && !a.e5m2) SIREN_QUANT_ROWS(_Float16, false);
+#undef SIREN_QUANT_ROWS
+        return;
+    }
 #define SIREN_QUANT(T, E)                                                                                       \
     hipLaunchKernelGGL((quant_kernel<T, E>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
                        a.cols, (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, vec, (int)col_blocks, a.panels)

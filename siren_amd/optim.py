@@ -130,69 +130,11 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     step: int64, one element, on the device: the steps done so far; 1 is added.
 
     Returns the gradients' norm before clipping (a device tensor), or None without max_norm."""
-    params, grads = list(params), list(grads)
-    if not params or len(params) != len(grads):
-        raise ValueError('adamw_step needs as many gradients as parameters, one at least; got %d and %d'
-                         % (len(params), len(grads)))
-    dev = params[0].device
-    if dev.type != 'cuda':
-        raise RuntimeError('adamw_step runs on ROCm devices (MI355X) only; got a %s tensor' % dev.type)
-    n = len(params)
-    ps, gs = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)()
-    numels, types = (ctypes.c_int64 * n)(), (ctypes.c_int32 * n)()
-    spans, keep, size = [], [], 0
-    for i, (p, g) in enumerate(zip(params, grads)):
-        code = _DTYPES.get(p.dtype)
-        if code is None or p.device != dev:
-            raise RuntimeError('adamw_step needs fp32, bf16 or fp16 parameters on one device; got %s on %s'
-                               % (p.dtype, p.device))
-        if not p.is_contiguous():
-            raise ValueError('adamw_step needs contiguous parameters; parameter %d has strides %s' % (i, p.stride()))
-        k = p.numel()
-        if g is not None:
-            if g.shape != p.shape or g.dtype != p.dtype or g.device != dev or g.layout != torch.strided:
-                raise ValueError('gradient %d must be %s %s on %s; got %s %s on %s'
-                                 % (i, tuple(p.shape), p.dtype, dev, tuple(g.shape), g.dtype, g.device))
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)
-            gs[i] = g.data_ptr()
-        at = p.data_ptr()
-        ps[i], numels[i], types[i] = at, k, code
-        if k:
-            spans.append((at, at + k * p.element_size()))
-        size += (k + 127) // 128 * 128
-    spans.sort()
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-        raise ValueError('adamw_step: parameters overlap (is one listed twice?)')
-    bits = 32 if scales is None else 8
-    want = torch.float32 if scales is None else torch.float8_e4m3fn
-    for name, t in (('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq)):
-        if t.dtype != want or t.numel() != size or t.device != dev or not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError('%s must be %d contiguous 16-byte aligned values of %s on %s; got %d of %s on %s'
-                             % (name, size, want, dev, t.numel(), t.dtype, t.device))
-    sm, sv = (None, None) if scales is None else scales
-    if scales is not None:
-        for t in scales:
-            if t.dtype != torch.uint8 or t.numel() != size // 128 or t.device != dev or not t.is_contiguous():
-                raise ValueError('scales must be two tensors of %d contiguous uint8 on %s' % (size // 128, dev))
-    if step.dtype != torch.int64 or step.numel() != 1 or step.device != dev:
-        raise ValueError('step must be one int64 on %s' % dev)
-    if max_norm is not None and not float(max_norm) > 0.:
-        raise ValueError('max_norm must be positive or None; got %r' % (max_norm,))
     if not (0. <= betas[0] < 1. and 0. <= betas[1] < 1. and eps >= 0. and math.isfinite(lr) and math.isfinite(weight_decay)):
         raise ValueError('need 0 <= betas < 1, eps >= 0 and finite lr and weight_decay')
-    lib, need = _lib.load(), ctypes.c_int64()
-    _lib.check(lib.siren_adamw_scratch_bytes(n, ctypes.byref(need)), 'siren_adamw_scratch_bytes')
-    scratch = torch.empty(need.value // 4, device=dev)
-    with torch.cuda.device(dev):
-        st = torch.cuda.current_stream(dev).cuda_stream
-        _lib.check(lib.siren_adamw_step(n, ps, gs, numels, types, bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
-                                        sm.data_ptr() if sm is not None else None, sv.data_ptr() if sv is not None else None,
-                                        step.data_ptr(), lr, betas[0], betas[1], eps, weight_decay,
-                                        0. if max_norm is None else float(max_norm), seed & 0xFFFFFFFFFFFFFFFF,
-                                        scratch.data_ptr(), st), 'siren_adamw_step')
-    return None if max_norm is None else scratch[8]
+    sm, sv = (None, None) if scales is None else scales
+    return _lib.native().adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas[0], betas[1], eps, weight_decay,
+                                    max_norm, seed & 0xFFFFFFFFFFFFFFFF, sm, sv)
 
 
 class FusedAdamW:

@@ -119,22 +119,17 @@ def test_quantize_special_values(cuda):
         assert np.array_equal(np64(fp8.dequantize(b)), want, equal_nan=True)
 
 
-@pytest.mark.parametrize('rows,cols', [(1, 130), (200, 70), (128, 128), (129, 1)])
-@pytest.mark.parametrize('tiles', [False, True])
-def test_both_directions_in_one_pass(cuda, rows, cols, tiles):
-    """The transpose is the quantised transpose; the column sums are the unrounded ones'; mult multiplies first."""
+@pytest.mark.parametrize('rows,cols', [(1, 130), (200, 70), (128, 128), (129, 1), (1, 1), (300, 515)])
+@pytest.mark.parametrize('block', ['row', 'tile'])
+def test_both_directions_in_one_pass(cuda, rows, cols, block):
+    """The transpose is the quantised transpose."""
     from siren_amd import fp8
     x = values((rows, cols), 5)
-    mult = values((rows, cols), 6).bfloat16()
-    q, qt, sums = fp8._quantize(x.to(cuda), tiles, transposed=True, mult=mult.to(cuda), colsum=True)
-    y = (x * mult.float()).numpy()
-    for b, v in ((q, y), (qt, y.T)):
-        want, byte = held(v, E4M3, tiles)
-        assert np.array_equal(np64(fp8.dequantize(fp8.Blocks(b.data, b.scale, v.shape[1]))), want)
+    for b, v in zip(fp8.quantize(x.to(cuda), block, transposed=True), (x.numpy(), x.numpy().T)):
+        want, byte = held(v, E4M3, block == 'tile')
+        assert np.array_equal(np64(fp8.dequantize(b)), want)
         assert np.array_equal(b.scale.cpu().numpy()[:, :byte.shape[1]], byte)
-    # 128 values of a row block are added in 32 bits: 15 roundings in a thread, 7 across; the blocks in 64
-    y = y.astype(np.float64)
-    check(sums, y.sum(0), 23 * 2. ** -24 * np.abs(y).sum(0) + 2. ** -24 * np.abs(y.sum(0)) + 2. ** -149, 'column sums')
+        assert (b.scale[:, byte.shape[1]:] == 127).all() and (b.data[:, v.shape[1]:].float() == 0).all()
 
 
 @pytest.mark.parametrize('view', ['strided', 'offset', 'transposed', 'expanded', 'wide'])
@@ -205,6 +200,53 @@ def test_linear_not_finite(cuda):
     assert torch.isnan(z[~keep]).all() and torch.equal(z[keep], y[keep])
 
 
+@pytest.mark.parametrize('m,k,n', [(1, 1, 1), (70, 300, 130), (260, 1100, 257), (40, 5000, 30)])
+def test_matmul(cuda, m, k, n):
+    """Two quantised operands, either in rows or tiles, the first in either format."""
+    from siren_amd import fp8
+    a, b = values((m, k), 1).to(cuda), values((n, k), 2).to(cuda)
+    bias = values((1, n), 3)[0].to(cuda)
+    for fmt in (E4M3, E5M2):
+        for ba in ('row', 'tile'):
+            for bb in ('row', 'tile'):
+                aq, bq = held(np64(a), fmt, ba == 'tile')[0], held(np64(b), tiles=bb == 'tile')[0]
+                z = aq @ bq.T + np64(bias)
+                for dtype in (torch.float32, torch.bfloat16):
+                    y = fp8.matmul(fp8.quantize(a, ba, fmt), fp8.quantize(b, bb), bias, dtype=dtype)
+                    check(y, z, product_tol(aq, bq, z, dtype, np.abs(np64(bias))), (fmt, ba, bb))
+    with pytest.raises(ValueError):
+        fp8.matmul(fp8.quantize(a), fp8.quantize(torch.cat([b, b], 1)))
+    with pytest.raises(TypeError):
+        fp8.matmul(fp8.quantize(a), fp8.quantize(b, dtype=E5M2))
+    with pytest.raises(TypeError):
+        fp8.matmul(a, b)
+    with pytest.raises(ValueError):
+        fp8.matmul(fp8.quantize(a), fp8.quantize(b), derivative=True)
+
+
+def test_linear_refuses(cuda):
+    from siren_amd import fp8
+    from siren_amd._lib import SirenUnsupported
+    x, w, b = layer(5, 200, 300, torch.float32, cuda)
+    w8 = fp8.quantize(w, 'tile')
+    for bad in (dict(x=x[:, :100]), dict(bias=b[:4]), dict(bias=b.cpu()), dict(activation='relu'), dict(omega=float('nan')),
+                dict(weight=fp8.quantize(w)), dict(weight=fp8.Blocks(w8.data[:, :128], w8.scale, 200)),
+                dict(weight=fp8.Blocks(w8.data, w8.scale[:, :2], 200)), dict(weight=fp8.Blocks(w8.data, w8.scale, 100)),
+                dict(weight=fp8.Blocks(w8.data.t().contiguous().t(), w8.scale, 200))):
+        with pytest.raises((ValueError, RuntimeError)):
+            fp8.linear(**{**dict(x=x, weight=w8, bias=b), **bad})
+    for bad in (dict(x=x.double()), dict(x=x.int()), dict(weight=w.double()), dict(grad_dtype=torch.float16),
+                dict(weight=fp8.quantize(w, 'tile', E5M2)), dict(weight=fp8.Blocks(w8.data, w8.scale.int(), 200))):
+        with pytest.raises(TypeError):
+            fp8.linear(**{**dict(x=x, weight=w, bias=b), **bad})
+    with pytest.raises(SirenUnsupported):
+        fp8.linear(x, w[None])
+    with pytest.raises(ValueError):
+        fp8.quantize(x, 'column')
+    with pytest.raises(ValueError):
+        fp8.quantize(x[0])
+
+
 # ---- gradients ---------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('m,k,n', [(1, 1, 1), (1, 256, 300), (32, 256, 1024), (33, 130, 64), (129, 257, 130), (1500, 192, 320)])
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
@@ -242,7 +284,7 @@ def test_sine_gradients(cuda):
     dx, dw, db = torch.autograd.grad(fp8.linear(x, w, b, 'sine'), leaves, dy)
     xq, wq = held(np64(x))[0], held(np64(w), tiles=True)[0]
     z = xq @ wq.T + np64(b)
-    _, deriv = fp8._product(fp8.quantize(x), fp8.quantize(w, 'tile'), b.detach(), 1, 30., torch.float32, deriv=True)
+    _, deriv = fp8.matmul(fp8.quantize(x), fp8.quantize(w, 'tile'), b, 'sine', derivative=True)
     tol = 30 * (30 * product_tol(xq, wq, 0 * z, torch.float32, np.abs(np64(b))) + np.abs(30 * z) * 2. ** -23 + 2. ** -22)
     check(deriv, 30 * np.cos(30 * z), tol + 2. ** -8 * np.abs(30 * np.cos(30 * z)), 'derivative')
     g = (dy * deriv.float()).cpu().double().numpy()

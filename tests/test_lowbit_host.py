@@ -50,11 +50,11 @@ def test_products_validate(lib):
     assert lib.siren_fp8_matmul_ws_bytes(1 << 18, 1024, 1024, ctypes.byref(c)) == OK and c.value == 0
     assert lib.siren_fp8_matmul_ws_bytes(1024, 1024, 1 << 18, ctypes.byref(c)) == OK and c.value % (4 << 20) == 0 and c.value
 
-    def lin(x=P(64), m=4, k=8, ld=8, w=P(64), sw=P(64), n=4, y=P(64), ws=P(64)):
-        return lib.siren_fp8_linear(x, 0, m, k, ld, w, sw, n, None, 0, 30., y, ws, None)
+    def lin(x=P(64), m=40, k=8, ld=8, w=P(64), sw=P(64), n=4, y=P(64), ws=P(64), deriv=None):
+        return lib.siren_fp8_linear(x, 0, m, k, ld, w, sw, n, None, 0, 30., y, deriv, ws, None)
     assert lin(m=0) == OK and lin(n=0) == OK
     for bad in (dict(m=-1), dict(k=0), dict(x=None), dict(w=None), dict(sw=None), dict(y=None), dict(ws=None), dict(ws=P(8)),
-                dict(w=P(4)), dict(sw=P(1)), dict(ld=3), dict(x=P(66)), dict(y=P(4))):
+                dict(w=P(4)), dict(sw=P(1)), dict(ld=3), dict(x=P(66)), dict(y=P(4)), dict(deriv=P(64))):
         assert lin(**bad) == EINVAL, bad
 
 

@@ -33,9 +33,10 @@ def hyper_bias_init(m):
 
 class HyperNetwork(nn.Module):
     """HyperNetwork(hyper_in_features, hyper_hidden_layers, hyper_hidden_features, hypo_module): forward(z (B, in))
-    -> OrderedDict name -> (B, *param_shape), in hypo_module.meta_named_parameters() order."""
+    -> OrderedDict name -> (B, *param_shape), in hypo_module.meta_named_parameters() order. precision='fp8' (extra
+    keyword): its products, whose weights are some hyper_hidden_features times the hypo-network's, on 8-bit operands."""
 
-    def __init__(self, hyper_in_features, hyper_hidden_layers, hyper_hidden_features, hypo_module):
+    def __init__(self, hyper_in_features, hyper_hidden_layers, hyper_hidden_features, hypo_module, precision='fp32'):
         super().__init__()
         self.names, self.param_shapes = [], []
         self.nets = nn.ModuleList()
@@ -44,7 +45,7 @@ class HyperNetwork(nn.Module):
             self.param_shapes.append(param.size())
             hn = modules.FCBlock(in_features=hyper_in_features, out_features=int(param.numel()),
                                  num_hidden_layers=hyper_hidden_layers, hidden_features=hyper_hidden_features,
-                                 outermost_linear=True, nonlinearity='relu')
+                                 outermost_linear=True, nonlinearity='relu', precision=precision)
             self.nets.append(hn)
             last = self.nets[-1].net[-1]
             if 'weight' in name:

@@ -26,7 +26,7 @@ import numpy as np
 import torch
 from torch import nn
 
-from . import _lib
+from . import _lib, fp8
 from .autograd import JetState, SirenBatchedFunction, SirenFunction, SirenJetFunction, SirenSplitFunction
 from .engine import SirenEngine
 
@@ -80,14 +80,18 @@ class MetaSequential(nn.Sequential, MetaModule):
 # ----------------------------------------------------------------------------------------------------------
 class BatchLinear(nn.Linear, MetaModule):
     """nn.Linear that also takes (possibly batched, ...xOutxIn) weights through `params` (modules.py:11-25).
-    Used on its own (and by non-sine baselines); inside a sine FCBlock the fused engine evaluates it."""
+    Used on its own (and by non-sine baselines); inside a sine FCBlock the fused engine evaluates it.
+    precision = 'fp8' (an attribute; FCBlock sets it): the products of unbatched weights in 8 bits (fp8.linear)."""
     __doc__ = nn.Linear.__doc__
+    precision = 'fp32'
 
     def forward(self, input, params=None):
         if params is None:
             params = OrderedDict(self.named_parameters())
         bias = params.get('bias', None)
         weight = params['weight']
+        if self.precision == 'fp8':
+            return fp8.linear(input, weight, bias)
         out = input.matmul(weight.transpose(-1, -2))
         if bias is not None:
             out = out + bias.unsqueeze(-2)
@@ -157,7 +161,29 @@ def get_engine(d_in, hidden, n_hidden, d_out, omega_first=30., omega_hidden=30.,
     return eng
 
 
-PRECISIONS = ('fp32', 'bf16x6')
+PRECISIONS = ('fp32', 'bf16x6', 'fp8')
+FP8_MIN_FEATURES = 64  # a layer with fewer inputs or outputs stays in fp32: coordinates need their bits, and bytes save nothing
+
+
+def _fp8_sine_apply(coords, weights_biases, outermost_linear):
+    """A sine network with its hidden products in 8 bits (fp8.linear with the sine in its epilogue), activations between
+    them in bf16 (8 bits of mantissa for values that the next layer rounds to 4). The first layer, and a last one with
+    fewer than FP8_MIN_FEATURES outputs, are plain fp32. Trains on values; its gradients are not differentiable again."""
+    if coords.device.type != 'cuda':
+        raise RuntimeError('siren_amd runs on ROCm devices (MI355X) only; move the model and coords to "cuda". '
+                           'The CPU restatement of the reference lives in oracle/ (test infrastructure).')
+    if any(W.dim() != 2 for W, _ in weights_biases):
+        raise _lib.SirenUnsupported("precision='fp8' takes unbatched weights")
+    a = coords
+    for i, (W, b) in enumerate(weights_biases):
+        last = i == len(weights_biases) - 1
+        sine = not last or not outermost_linear
+        if min(W.shape) >= FP8_MIN_FEATURES:
+            a = fp8.linear(a if a.dtype == torch.bfloat16 else a.to(torch.bfloat16), W, b, 'sine' if sine else None)
+        else:
+            z = nn.functional.linear(a.float(), W, b)
+            a = torch.sin(30 * z) if sine else z
+    return a.float()
 
 
 def _fused_apply(engine, jet, coords, weights_biases, precision='fp32'):
@@ -260,6 +286,10 @@ class FCBlock(MetaModule):
             layers.append(MetaSequential(BatchLinear(hidden_features, out_features)))
         else:
             layers.append(MetaSequential(BatchLinear(hidden_features, out_features), nl))
+        if precision == 'fp8' and nonlinearity != 'sine':
+            for layer in layers:
+                if min(layer[0].in_features, layer[0].out_features) >= FP8_MIN_FEATURES:
+                    layer[0].precision = 'fp8'
         self.net = MetaSequential(*layers)
         if self.weight_init is not None:
             self.net.apply(self.weight_init)
@@ -278,6 +308,8 @@ class FCBlock(MetaModule):
         if self.nonlinearity != 'sine':
             return self.net(coords, params=params)
         wb = [(params['%d.0.weight' % i], params.get('%d.0.bias' % i)) for i in range(len(self.net))]
+        if self.precision == 'fp8':
+            return _fp8_sine_apply(coords, wb, self.outermost_linear)
         return _fused_apply(self._engine(), self._jet, coords, wb, self.precision)
 
     def forward_with_activations(self, coords, params=None, retain_grad=False):
@@ -313,6 +345,9 @@ class SingleBVPNet(MetaModule):
     W0 kernel (1.85x), and a step whose loss needs parameter gradients of model_out only (image fitting) on the
     split W0 forward plus the bf16x6 W2 backward (siren_backward_split: split-bf16 recompute + reverse, fp32 MFMA
     wgrad). A backward through the jet node recomputes on the fp32 kernels.
+    precision='fp8' runs the products of every layer with 64 inputs and outputs at least on 8-bit operands with a scale
+    per block of 128, forward and backward (fp8.linear): values to some 2^-5 a layer, any hidden width, losses on
+    model_out only (a loss on gradient() raises in its backward).
     """
 
     def __init__(self, out_features=1, type='sine', in_features=2, mode='mlp', hidden_features=256,

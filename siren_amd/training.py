@@ -40,10 +40,19 @@ def _coord_count(model_input):
 
 def train(model, train_dataloader, epochs, lr, steps_til_summary, epochs_til_checkpoint, model_dir, loss_fn,
           summary_fn=None, val_dataloader=None, double_precision=False, clip_grad=False, use_lbfgs=False,
-          loss_schedules=None, device='cuda', log=print, writer=None, fused_adam=False):
+          loss_schedules=None, device='cuda', log=print, writer=None, fused_adam=False, optimizer=None):
+    """optimizer: steps instead of Adam, e.g. optim.FusedAdamW(model.parameters(), lr=lr, state_bits=8); lr is then its own.
+    One with a max_norm attribute clips by itself: clip_grad sets it."""
     if double_precision:
         raise NotImplementedError('siren_amd computes in fp32 (the reference default)')
-    if use_lbfgs:
+    if optimizer is not None and (use_lbfgs or fused_adam):
+        raise ValueError('train: optimizer, use_lbfgs and fused_adam exclude each other')
+    clips_itself = fused_adam or hasattr(optimizer, 'max_norm')
+    if optimizer is not None:
+        optim = optimizer
+        if clip_grad and clips_itself:
+            optim.max_norm = 1. if clip_grad is True else clip_grad
+    elif use_lbfgs:
         optim = torch.optim.LBFGS(lr=lr, params=model.parameters(), max_iter=50000, max_eval=50000,
                                   history_size=50, line_search_fn='strong_wolfe')
     elif fused_adam:  # clip + Adam in two HIP launches over one flat bucket, norm kept on the device (optim.py)
@@ -109,7 +118,7 @@ def train(model, train_dataloader, epochs, lr, steps_til_summary, epochs_til_che
                     optim.allreduce_grad(world, count)  # the bucket itself is the all-reduce buffer: no gather / scatter
                 else:
                     distributed.allreduce_gradients(list(model.parameters()), world, count)
-                if clip_grad and not fused_adam:
+                if clip_grad and not clips_itself:
                     max_norm = 1. if isinstance(clip_grad, bool) else clip_grad
                     torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=max_norm)
                 optim.step()

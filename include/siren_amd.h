@@ -427,7 +427,7 @@ int32_t siren_laplace_backward_stored(const siren_cfg* cfg, const float* ws, con
 #define SIREN_FP8_PANELS 2 /* its values in panels instead of rows                              */
 
 /* x (rows, cols) of row stride ld -> q, s: quantised along the columns; qt, st: the transpose (cols, rows), quantised
- * along the rows, laid out as a (cols, rows) tensor. Either pair may be NULL. mult (rows, cols) bf16, contiguous,
+ * along the rows, laid out as a (cols, rows) tensor. Either pair may be NULL. panels: 1 for q, 2 for qt, 3 for both. mult (rows, cols) bf16, contiguous,
  * nullable: x is multiplied by it first. colsum (cols) fp32, nullable: the column sums of what is quantised, before
  * rounding (a bias's gradient), through colsum_ws of ceil(rows / 128) * cols floats. With rows == 0 nothing is
  * written. */

@@ -24,7 +24,7 @@ struct Fp8Quant {
     const void* mult;
     uint8_t *q, *s, *qt, *st;
     float* colsum;
-    int type, e5m2, tiles, panels;  // panels: of q and of qt, as in Fp8Operand
+    int type, e5m2, tiles, panels;  // panels, as in Fp8Operand: 1 of q, 2 of qt
 };
 void launch_fp8_quant(hipStream_t st, const Fp8Quant& a);
 // out[c] = sum over the row blocks of colsum (blocks, cols), in order

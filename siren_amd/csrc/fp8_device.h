@@ -21,18 +21,22 @@ __device__ __forceinline__ int exponent_byte(float amax) {
     const int e = (int)(b >> 23) - (E5M2 ? 15 : 8) + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
     return e < 1 ? 1 : e;
 }
-__device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
+__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float((uint32_t)byte << 23); }
 
-// four values to four codes, to the nearest, ties to even; NaN and (e4m3) infinities become NaN
+// four values over scale to four codes, to the nearest, ties to even; NaN and (e4m3) infinities become NaN. The scale is a
+// power of two, so the division inside the instruction is exact.
 template <bool E5M2>
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float scale) {
+    typedef short i16x2 __attribute__((ext_vector_type(2)));
+    i16x2 r = {0, 0};
     if constexpr (E5M2) {
-        const int lo = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false);
-        return (uint32_t)__builtin_amdgcn_cvt_pk_bf8_f32(c, d, lo, true);
+        r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(r, a, b, scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(r, c, d, scale, true);
     } else {
-        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
     }
+    return __builtin_bit_cast(uint32_t, r);
 }
 
 // two codes to bf16, times scale (a power of two: exact)
@@ -64,10 +68,31 @@ __device__ __forceinline__ void load_quad(const T* src, int valid, bool vec, flo
     }
 }
 
-// the maximum over the 32 lanes of a half wave
+// the maximum over the 16 lanes of a row of the wave, and over the 32 of its half, by data-parallel moves (a shuffle
+// through LDS costs an instruction of its own and the LDS' time for each step)
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float m) {
+    return fmaxf(m, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(m), CTRL, 0xF, 0xF, true)));
+}
+__device__ __forceinline__ float row16_max(float m) {
+    m = dpp_max<0xB1>(m);   // lanes 1 apart
+    m = dpp_max<0x4E>(m);   // 2 apart
+    m = dpp_max<0x124>(m);  // rotated by 4
+    return dpp_max<0x128>(m);  // by 8
+}
 __device__ __forceinline__ float half_wave_max(float m) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    m = row16_max(m);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// the largest finite magnitude of a half wave's quads: where the plain maximum of any in the wave is not finite (fmaxf
+// drops a NaN beside a number), the quads are looked through again
+__device__ __forceinline__ float half_wave_amax(float a, float b, float c, float d) {
+    float m = half_wave_max(fmaxf(fmaxf(__builtin_fabsf(a), __builtin_fabsf(b)),
+                                  fmaxf(__builtin_fabsf(c), __builtin_fabsf(d))));
+    if (__builtin_expect(__any(!(m < INFINITY)), 0))
+        m = half_wave_max(fmaxf(fmaxf(finite_abs(a), finite_abs(b)), fmaxf(finite_abs(c), finite_abs(d))));
     return m;
 }
 

@@ -1702,8 +1702,8 @@ int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t c
                            int32_t format, int32_t tiles, int32_t panels, void* q, void* s, void* qt, void* st,
                            float* colsum_ws, float* colsum, void* stream) {
     if (int rc = check_fp8_type(dtype)) return rc;
-    if (rows < 0 || cols < 0 || (format != 0 && format != 1))
-        return fail(SIREN_EINVAL, "siren_fp8_quantize: need rows, cols >= 0 and format 0 (e4m3) or 1 (e5m2)");
+    if (rows < 0 || cols < 0 || (format != 0 && format != 1) || (panels & ~3) != 0)
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: need rows, cols >= 0, format 0 (e4m3) or 1 (e5m2) and panels in 0..3");
     if (siren::fp8_blocks(cols) > kMaxGrid / std::max<int64_t>(1, siren::fp8_blocks(rows)))
         return fail(SIREN_EINVAL, "siren_fp8_quantize: too many tiles");
     if ((q == nullptr) != (s == nullptr) || (qt == nullptr) != (st == nullptr))
@@ -1715,7 +1715,7 @@ int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t c
     if (!aligned(q, 16) || !aligned(qt, 16) || !aligned(s, 4) || !aligned(st, 4) || !aligned(mult, 2))
         return fail(SIREN_EINVAL, "siren_fp8_quantize: q and qt must be 16-byte aligned, scales 4-byte aligned");
     siren::Fp8Quant a{x, ld, rows, cols, mult, (uint8_t*)q, (uint8_t*)s, (uint8_t*)qt, (uint8_t*)st,
-                      colsum != nullptr ? colsum_ws : nullptr, dtype, format, tiles != 0, panels != 0};
+                      colsum != nullptr ? colsum_ws : nullptr, dtype, format, tiles != 0, panels};
     siren::launch_fp8_quant((hipStream_t)stream, a);
     if (colsum != nullptr)
         siren::launch_fp8_colsum((hipStream_t)stream, colsum_ws, siren::fp8_blocks(rows), cols, colsum);

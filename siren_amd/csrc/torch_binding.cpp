@@ -84,10 +84,9 @@ Tensor rows_of(const Tensor& x, int64_t& ld) {
     return y;
 }
 
-enum Want { STRAIGHT = 1, TRANSPOSED = 2, PANELS = 4, TRANSPOSED_PANELS = 8, TILES = 16 };
+enum Want { PANELS = 1, TRANSPOSED_PANELS = 2, TILES = 4 };
 
-// One pass over x (times mult): its rows, its transpose's rows, its column sums, as wanted. Rows and panels may differ
-// between the two directions: then the pass is made twice.
+// One pass over x (times mult): its rows, its transpose's rows, its column sums, as wanted
 void quantize_into(const Tensor& x0, int want, int fmt, const Tensor& mult, Blocks* q, Blocks* qt, Tensor* colsum) {
     int64_t ld;
     const Tensor x = rows_of(x0, ld);
@@ -110,20 +109,12 @@ void quantize_into(const Tensor& x0, int want, int fmt, const Tensor& mult, Bloc
         ws = at::empty({blocks(rows), cols}, f32);
         *colsum = at::empty({cols}, f32);
     }
-    auto pass = [&](Blocks* a, Blocks* t, Tensor* sums, bool panels) {
-        check(lib.quantize(x.data_ptr(), type_code(x.scalar_type()), rows, cols, ld, mult.defined() ? mult.data_ptr() : nullptr,
-                           fmt, tiles, panels, a ? a->data.data_ptr() : nullptr, a ? a->scale.data_ptr() : nullptr,
-                           t ? t->data.data_ptr() : nullptr, t ? t->scale.data_ptr() : nullptr,
-                           sums ? ws.data_ptr<float>() : nullptr, sums ? sums->data_ptr<float>() : nullptr, stream_of(x)),
-              "siren_fp8_quantize");
-    };
-    const bool same = !q || !qt || bool(want & PANELS) == bool(want & TRANSPOSED_PANELS);
-    if (same) {
-        pass(q, qt, colsum, q ? want & PANELS : want & TRANSPOSED_PANELS);
-    } else {
-        pass(q, nullptr, colsum, want & PANELS);
-        pass(nullptr, qt, nullptr, want & TRANSPOSED_PANELS);
-    }
+    const int panels = (want & PANELS ? 1 : 0) | (want & TRANSPOSED_PANELS ? 2 : 0);
+    check(lib.quantize(x.data_ptr(), type_code(x.scalar_type()), rows, cols, ld, mult.defined() ? mult.data_ptr() : nullptr, fmt,
+                       tiles, panels, q ? q->data.data_ptr() : nullptr, q ? q->scale.data_ptr() : nullptr,
+                       qt ? qt->data.data_ptr() : nullptr, qt ? qt->scale.data_ptr() : nullptr,
+                       colsum ? ws.data_ptr<float>() : nullptr, colsum ? colsum->data_ptr<float>() : nullptr, stream_of(x)),
+          "siren_fp8_quantize");
 }
 
 Tensor product(const Blocks& a, const Blocks& b, const Tensor& bias, int act, double omega, at::ScalarType type, Tensor* deriv) {

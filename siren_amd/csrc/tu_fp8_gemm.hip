@@ -341,10 +341,8 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs f) {
             if (u < units) {
                 float v[4];
                 load_quad((const T*)f.x + row * f.ld + c0, left < 4 ? (left > 0 ? (int)left : 0) : 4, f.vec != 0, v);
-                byte = exponent_byte<false>(half_wave_max(fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])),
-                                                                fmaxf(finite_abs(v[2]), finite_abs(v[3])))));
-                const float inv = inverse_scale(byte);
-                codes = pack4<false>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                byte = exponent_byte<false>(half_wave_amax(v[0], v[1], v[2], v[3]));
+                codes = pack4<false>(v[0], v[1], v[2], v[3], scale_of(byte));
             }
             *(uint32_t*)(xq + row * FEW_LD + b * 128 + c4 * 4) = codes;
             if (c4 == 0) xs[row * (FEW_K / 128) + b] = (uint8_t)byte;

@@ -19,7 +19,7 @@ namespace {
 constexpr int QT = 128;           // tile edge
 constexpr int QSTRIDE = QT + 16;  // LDS row of the transposed bytes: 16-byte pieces on distinct banks
 
-template <typename T, bool E5M2>
+template <typename T, bool E5M2, bool MULT>
 __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
                                                     const __bf16* __restrict__ mult, uint8_t* __restrict__ q,
                                                     uint8_t* __restrict__ s, uint8_t* __restrict__ qt,
@@ -36,19 +36,36 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
     const int64_t row_blocks = (rows + QT - 1) / QT;
     const int64_t s_ld = (col_blocks + 3) / 4 * 4, st_ld = (row_blocks + 3) / 4 * 4;
 
-    // Every load is issued before any is waited for: rows past the end read the last row and are zeroed afterwards (a
-    // branch around each row's load made 16 round trips of them: 8 us for one row).
+    // Every load is issued before any is waited for (a branch around each row's load made 16 round trips of them: 8 us for
+    // one row). A tile on the edge reads the last row or column again and zeroes what does not exist.
     f32x4 v[16];
-    const bool wide = vec && c0 + 4 <= cols;
-    if (wide) {
-        typedef T T4 __attribute__((ext_vector_type(4)));
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    typedef __bf16 B4 __attribute__((ext_vector_type(4)));
+    if (vec && (rb + 1) * QT <= rows && (int64_t)(cb + 1) * QT <= cols) {
         T4 h[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) h[i] = *(const T4*)(x + (r0 + i < rows ? r0 + i : rows - 1) * ld + c0);
+        for (int i = 0; i < 16; ++i) h[i] = *(const T4*)(x + (r0 + i) * ld + c0);
+        if constexpr (MULT) {
+            const bool wide = (cols & 3) == 0;
+            B4 f[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 16; ++i) {
+                const __bf16* src = mult + (r0 + i) * cols + c0;
+                if (wide)
+                    f[i] = *(const B4*)src;
+                else
+                    f[i] = B4{src[0], src[1], src[2], src[3]};
+            }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] = r0 + i < rows ? (float)h[i][k] : 0.f;
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[i][k] = (float)h[i][k] * (float)f[i][k];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[i][k] = (float)h[i][k];
+        }
     } else {
         T h[16][4];
 #pragma unroll
@@ -59,26 +76,11 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 #pragma unroll
         for (int i = 0; i < 16; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] = r0 + i < rows && c0 + k < cols ? (float)h[i][k] : 0.f;
-    }
-    if (mult != nullptr) {
-        const bool mwide = (cols & 3) == 0 && c0 + 4 <= cols;
-        typedef __bf16 B4 __attribute__((ext_vector_type(4)));
-        if (mwide) {
-            B4 h[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) h[i] = *(const B4*)(mult + (r0 + i < rows ? r0 + i : rows - 1) * cols + c0);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[i][k] *= r0 + i < rows ? (float)h[i][k] : 0.f;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (r0 + i < rows && c0 + k < cols) v[i][k] *= (float)mult[(r0 + i) * cols + c0 + k];
-        }
+            for (int k = 0; k < 4; ++k) {
+                const bool in = r0 + i < rows && c0 + k < cols;
+                v[i][k] = in ? (float)h[i][k] : 0.f;
+                if (MULT && in) v[i][k] *= (float)mult[(r0 + i) * cols + c0 + k];
+            }
     }
 
     if (colsum != nullptr) {  // 16 rows a thread, then the 8 row groups in order
@@ -103,9 +105,16 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 #pragma unroll
         for (int i = 0; i < 16; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) m = fmaxf(m, finite_abs(v[i][k]));
+            for (int k = 0; k < 4; ++k) m = fmaxf(m, __builtin_fabsf(v[i][k]));
+        if (__builtin_expect(__any(m == INFINITY), 0)) {  // fmaxf drops NaN; infinities are dropped here
+            m = 0.f;
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) m = fmaxf(m, finite_abs(v[i][k]));
+        }
+        m = half_wave_max(m);
+        m = fmaxf(m, __shfl_xor(m, 32));
         if ((t & 63) == 0) wmax[t >> 6] = m;
         __syncthreads();
         tile_byte = exponent_byte<E5M2>(fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3])));
@@ -126,17 +135,12 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             int byte = tile_byte;
-            if (!tiles) {
-                float m = fmaxf(fmaxf(finite_abs(v[i][0]), finite_abs(v[i][1])),
-                                fmaxf(finite_abs(v[i][2]), finite_abs(v[i][3])));
-                byte = exponent_byte<E5M2>(half_wave_max(m));
-            }
+            if (!tiles) byte = exponent_byte<E5M2>(half_wave_amax(v[i][0], v[i][1], v[i][2], v[i][3]));
             if (r0 + i < rows) {
-                const float inv = inverse_scale(byte);
-                uint8_t* dst = panels ? q + ((cb * 2 + (c4 >> 4)) * rows + r0 + i) * 64 + (c4 & 15) * 4
+                uint8_t* dst = (panels & 1) ? q + ((cb * 2 + (c4 >> 4)) * rows + r0 + i) * 64 + (c4 & 15) * 4
                                       : q + (r0 + i) * ((int64_t)col_blocks * QT) + c0;
                 *(uint32_t*)dst =
-                    pack4<E5M2>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+                    pack4<E5M2>(v[i][0], v[i][1], v[i][2], v[i][3], scale_of(byte));
                 if (!tiles && c4 == 0) {
                     s[(r0 + i) * s_ld + cb] = (uint8_t)byte;
                     if (cb == col_blocks - 1)
@@ -147,16 +151,21 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
     }
 
     if (qt != nullptr) {
-        float inv[4];
+        float scale[4];
         if (tiles) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) inv[k] = inverse_scale(tile_byte);
+            for (int k = 0; k < 4; ++k) scale[k] = scale_of(tile_byte);
         } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 float m = 0.f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) m = fmaxf(m, finite_abs(v[i][k]));
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, __builtin_fabsf(v[i][k]));
+                if (__builtin_expect(__any(m == INFINITY), 0)) {
+                    m = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) m = fmaxf(m, finite_abs(v[i][k]));
+                }
                 part[rg][c4 * 4 + k] = m;
             }
             __syncthreads();
@@ -166,7 +175,7 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 #pragma unroll
                 for (int g = 1; g < 8; ++g) m = fmaxf(m, part[g][c4 * 4 + k]);
                 const int byte = exponent_byte<E5M2>(m);
-                inv[k] = inverse_scale(byte);
+                scale[k] = scale_of(byte);
                 if (rg == 0 && c0 + k < cols) {
                     st[(c0 + k) * st_ld + rb] = (uint8_t)byte;
                     if (rb == row_blocks - 1)
@@ -179,12 +188,11 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
             u32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                w[j] = pack4<E5M2>(v[4 * j][k] * inv[k], v[4 * j + 1][k] * inv[k], v[4 * j + 2][k] * inv[k],
-                                   v[4 * j + 3][k] * inv[k]);
+                w[j] = pack4<E5M2>(v[4 * j][k], v[4 * j + 1][k], v[4 * j + 2][k], v[4 * j + 3][k], scale[k]);
             *(u32x4*)(tr + (c4 * 4 + k) * QSTRIDE + rg * 16) = w;
         }
         __syncthreads();
-        if (panels) {
+        if (panels & 2) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // 4 lanes a column of each panel: a wave's 16 columns lie behind each other
                 const int c = (j & 1) * 64 + (t >> 2), piece = (j >> 1) * 4 + (t & 3);
@@ -228,14 +236,11 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t r = rb * ROWS_PER_GROUP + i * 8 + unit;
-        const float m = half_wave_max(fmaxf(fmaxf(finite_abs(v[i][0]), finite_abs(v[i][1])),
-                                            fmaxf(finite_abs(v[i][2]), finite_abs(v[i][3]))));
-        const int byte = exponent_byte<E5M2>(m);
-        const float inv = inverse_scale(byte);
+        const int byte = exponent_byte<E5M2>(half_wave_amax(v[i][0], v[i][1], v[i][2], v[i][3]));
         if (r < rows) {
-            uint8_t* dst = panels ? q + ((cb * 2 + (c4 >> 4)) * rows + r) * 64 + (c4 & 15) * 4
+            uint8_t* dst = (panels & 1) ? q + ((cb * 2 + (c4 >> 4)) * rows + r) * 64 + (c4 & 15) * 4
                                   : q + r * ((int64_t)col_blocks * QT) + c0;
-            *(uint32_t*)dst = pack4<E5M2>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+            *(uint32_t*)dst = pack4<E5M2>(v[i][0], v[i][1], v[i][2], v[i][3], scale_of(byte));
             // the pad bytes of a row's last word stand for 1
             if (c4 == 0) s[r * s_ld + cb] = (uint8_t)byte;
             if (cb == col_blocks - 1 && c4 > 0 && cb + c4 < s_ld) s[r * s_ld + cb + c4] = 127;
@@ -283,18 +288,24 @@ void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
 #undef SIREN_QUANT_ROWS
         return;
     }
-#define SIREN_QUANT(T, E)                                                                                       \
-    hipLaunchKernelGGL((quant_kernel<T, E>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
-                       a.cols, (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, vec, (int)col_blocks, a.panels)
-    if (a.e5m2) {
-        if (a.type == FP8_F32) SIREN_QUANT(float, true);
-        if (a.type == FP8_BF16) SIREN_QUANT(__bf16, true);
-        if (a.type == FP8_F16) SIREN_QUANT(_Float16, true);
-    } else {
-        if (a.type == FP8_F32) SIREN_QUANT(float, false);
-        if (a.type == FP8_BF16) SIREN_QUANT(__bf16, false);
-        if (a.type == FP8_F16) SIREN_QUANT(_Float16, false);
-    }
+#define SIREN_QUANT(T, E, M)                                                                                            \
+    hipLaunchKernelGGL((quant_kernel<T, E, M>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, a.cols, \
+                       (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, vec, (int)col_blocks, a.panels)
+#define SIREN_QUANT_TYPES(E, M)                     \
+    do {                                            \
+        if (a.type == FP8_F32) SIREN_QUANT(float, E, M);     \
+        if (a.type == FP8_BF16) SIREN_QUANT(__bf16, E, M);   \
+        if (a.type == FP8_F16) SIREN_QUANT(_Float16, E, M);  \
+    } while (0)
+    if (a.e5m2 && a.mult != nullptr)
+        SIREN_QUANT_TYPES(true, true);
+    else if (a.e5m2)
+        SIREN_QUANT_TYPES(true, false);
+    else if (a.mult != nullptr)
+        SIREN_QUANT_TYPES(false, true);
+    else
+        SIREN_QUANT_TYPES(false, false);
+#undef SIREN_QUANT_TYPES
 #undef SIREN_QUANT
 }
 

@@ -43,14 +43,16 @@ struct GemmArgs {
     __bf16* deriv;
 };
 
+// Nontemporal: a result is read by a later kernel, after the operands that it would push out of L2 (262144 x 1024 x 1024
+// fp32 out: 620 -> 550 us).
 template <typename T>
 __device__ __forceinline__ void put4(T* dst, f32x4 v, int valid, bool vec) {
     if (vec && valid >= 4) {
         if constexpr (sizeof(T) == 4) {
-            *(f32x4*)dst = v;
+            __builtin_nontemporal_store(v, (f32x4*)dst);
         } else {
             typedef T T4 __attribute__((ext_vector_type(4)));
-            *(T4*)dst = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+            __builtin_nontemporal_store((T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}), (T4*)dst);
         }
     } else {
 #pragma unroll
@@ -106,8 +108,8 @@ struct Finish {
 };
 
 // The products of one half block (64 k) of a wave's RT x 2 tiles of 32 x 32, bytes to bf16 and scaled on the way, in four
-// slices of 16 k: a wave issues in order, so the next slice's widening (3 instructions a product at RT = 4) has to stand
-// between this one's products for the matrix pipe not to wait for it.
+// slices of 16 k: the next slice's widening (3 instructions a product at RT = 4) stands beside this one's products. (Placing
+// them one by one with scheduling barriers was 2 % slower than the compiler's own order.)
 template <bool E5M2A, int RT>
 __device__ __forceinline__ void half_block(const uint8_t* la, const uint8_t* lb, int lane, const uint32_t (&ba)[RT],
                                            const uint32_t (&bb)[2], f32x16 (&acc)[RT][2]) {
@@ -136,10 +138,6 @@ __device__ __forceinline__ void half_block(const uint8_t* la, const uint8_t* lb,
         for (int i = 0; i < RT; ++i) va[to][i] = widen8<E5M2A>(ra[p][i][w], ra[p][i][w + 1], fa[i]);
     };
     widen(0);
-    // Each slice is scheduled by itself, a product and its share of the next slice's widening in turn: left alone, the
-    // compiler gathers the widening before the products and chains the products of one tile.
-    constexpr int SHARE = (4 * (RT + 2) + 2 * RT - 1) / (2 * RT);
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         if (k < 3) widen(k + 1);
@@ -148,12 +146,6 @@ __device__ __forceinline__ void half_block(const uint8_t* la, const uint8_t* lb,
 #pragma unroll
             for (int j = 0; j < 2; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[k & 1][j], va[k & 1][i], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 2 * RT; ++e) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (k < 3) __builtin_amdgcn_sched_group_barrier(0x002, SHARE, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -168,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
 
     // Workgroups go round-robin to the 8 dies: give each die a contiguous run of the (split, tile) list, columns fastest, so
     // that the tiles that share rows of A, or a split's k of both operands, meet in one L2 (the splits of a 1024 x 1024
-    // product over 262144, dealt out tile by tile, read B from HBM on every die: 540 us instead of XXX)
+    // product over 262144, dealt out tile by tile, read B from HBM on every die: 550 us instead of 455)
     const int tiles = g.tiles_m * g.tiles_n;
     int tile = blockIdx.x;
     {
@@ -282,23 +274,31 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
         const int64_t col = n0 + (wn * 2 + j) * 32 + quad;
         if (col < g.n) {
             const Finish<T> to(g, col);
-            for (int row = sub; row < RT * 32; row += 8) {
-                const int64_t m = wave_m + row;
-                if (m >= g.m) break;
-                const f32x4 v = *(const f32x4*)(strip + row * ES + quad);
-                if constexpr (SPLIT)
-                    put4((float*)g.out + (split * g.m + m) * g.n + col, v, to.valid, to.vec);
-                else
-                    to.store(g, m, v);
+            for (int row = sub; row < RT * 32; row += 32) {  // four rows' reads before the first is stored
+                f32x4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = *(const f32x4*)(strip + (row + 8 * u) * ES + quad);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int64_t m = wave_m + row + 8 * u;
+                    if (m < g.m) {
+                        if constexpr (SPLIT)
+                            put4((float*)g.out + (split * g.m + m) * g.n + col, v[u], to.valid, to.vec);
+                        else
+                            to.store(g, m, v[u]);
+                    }
+                }
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
-// A layer of a few rows (up to 32) in one launch: what it cannot do without is the weight's bytes. A workgroup owns 64
-// columns, a wave 16 of them: it asks for its weights of FEW_K k first, all waves round that much of x to 8 bits into LDS
-// while they travel (half a wave a block), then the wave's rows of the weight times the rows of x, 16 at a time.
+// A layer of a few rows (up to 32) in one launch: what it cannot do without is the weight's bytes. A wave owns NT x 16
+// columns, a workgroup four times as many: it asks for its weights of FEW_K k first, all waves round that much of x to 8
+// bits into LDS while they travel (half a wave a block), then the wave's rows of the weight times the rows of x, 16 at a
+// time. Rows of x that do not exist are whatever LDS holds: an output depends on its own row only. 65536 columns of 256:
+// 6 us for one row (16.8 MB: 2.8 TB/s), 9 for 32 (8.4 MB of results more).
 constexpr int FEW_ROWS = 32, FEW_K = 512, FEW_LD = FEW_K + 16;  // LDS rows 16 bytes apart from a bank period
 struct FewArgs {
     const void* x;
@@ -307,78 +307,103 @@ struct FewArgs {
     int vec;
     GemmArgs out;  // n, bias, act, omega, out
 };
-template <typename T, int MT>
+template <typename T, int MT, int NT>
 __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs f) {
+    constexpr int CHUNK = FEW_K / 128;
     __shared__ __align__(16) uint8_t xq[MT * 16 * FEW_LD];
-    __shared__ uint8_t xs[MT * 16 * (FEW_K / 128)];
+    __shared__ uint8_t xs[MT * 16 * CHUNK];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, q = lane >> 4;
     const GemmArgs& g = f.out;
-    const int64_t n0 = (int64_t)blockIdx.x * 64 + wave * 16;
-    const int64_t wrow = n0 + r < g.n ? n0 + r : g.n - 1;  // rows past the end read the last one and store nothing
+    const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * (NT * 16);
     const int64_t kp = (f.k + 127) / 128 * 128;
     const int blocks = (int)(kp / 128);
-    const uint8_t* w = f.w + wrow * kp + q * 16;
-    const uint8_t* sw = f.sw + (wrow >> 7) * ((blocks + 3) / 4 * 4);
-    f32x4 acc[MT] = {};
-    for (int b0 = 0; b0 < blocks; b0 += FEW_K / 128) {
-        const int here = blocks - b0 < FEW_K / 128 ? blocks - b0 : FEW_K / 128;
-        u32x4 wv[FEW_K / 128][2];
-        const uint32_t scales = *(const uint32_t*)(sw + b0);
+    const uint8_t *w[NT], *sw[NT];
 #pragma unroll
-        for (int b = 0; b < FEW_K / 128; ++b) {
-            const int at = (b0 + (b < here ? b : 0)) * 128;
-            wv[b][0] = *(const u32x4*)(w + at);
-            wv[b][1] = *(const u32x4*)(w + at + 64);
+    for (int j = 0; j < NT; ++j) {  // columns past the end read the last one's weights and store nothing
+        const int64_t row = n0 + j * 16 + r < g.n ? n0 + j * 16 + r : g.n - 1;
+        w[j] = f.w + row * kp + q * 16;
+        sw[j] = f.sw + (row >> 7) * ((blocks + 3) / 4 * 4);
+    }
+    f32x4 acc[MT][NT] = {};
+    for (int b0 = 0; b0 < blocks; b0 += CHUNK) {
+        const int here = blocks - b0 < CHUNK ? blocks - b0 : CHUNK;
+        u32x4 wv[NT][CHUNK][2];
+        uint32_t scales[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            scales[j] = *(const uint32_t*)(sw[j] + b0);
+#pragma unroll
+            for (int b = 0; b < CHUNK; ++b)
+                if (b < here) {
+                    wv[j][b][0] = *(const u32x4*)(w[j] + (b0 + b) * 128);
+                    wv[j][b][1] = *(const u32x4*)(w[j] + (b0 + b) * 128 + 64);
+                }
         }
         if (b0 > 0) __syncthreads();  // x of the chunk before has been read
-        const int c4 = threadIdx.x & 31, units = here * (int)f.m;
-        for (int u = threadIdx.x >> 5; u < MT * 16 * here; u += 8) {
-            const int row = u / here, b = u - row * here;
-            const int64_t c0 = (int64_t)(b0 + b) * 128 + c4 * 4, left = f.k - c0;
-            uint32_t codes = 0;
-            int byte = 127;
-            if (u < units) {
-                float v[4];
-                load_quad((const T*)f.x + row * f.ld + c0, left < 4 ? (left > 0 ? (int)left : 0) : 4, f.vec != 0, v);
-                byte = exponent_byte<false>(half_wave_amax(v[0], v[1], v[2], v[3]));
-                codes = pack4<false>(v[0], v[1], v[2], v[3], scale_of(byte));
+        // units of one block of one row, BATCH of a half wave's loaded before the first is rounded
+        constexpr int BATCH = MT == 1 ? 2 : 8;
+        const int c4 = threadIdx.x & 31, half = threadIdx.x >> 5, all = (int)f.m * here;
+        for (int u0 = half; u0 < all; u0 += 8 * BATCH) {
+            float v[BATCH][4];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int u = u0 + 8 * i, row = u / here, b = u - row * here;
+                const int64_t c0 = (int64_t)(b0 + b) * 128 + c4 * 4, left = f.k - c0;
+                load_quad((const T*)f.x + row * f.ld + c0, u < all && left > 0 ? (left < 4 ? (int)left : 4) : 0, f.vec != 0, v[i]);
             }
-            *(uint32_t*)(xq + row * FEW_LD + b * 128 + c4 * 4) = codes;
-            if (c4 == 0) xs[row * (FEW_K / 128) + b] = (uint8_t)byte;
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int u = u0 + 8 * i, row = u / here, b = u - row * here;
+                const int byte = exponent_byte<false>(half_wave_amax(v[i][0], v[i][1], v[i][2], v[i][3]));
+                if (u < all) {
+                    *(uint32_t*)(xq + row * FEW_LD + b * 128 + c4 * 4) =
+                        pack4<false>(v[i][0], v[i][1], v[i][2], v[i][3], scale_of(byte));
+                    if (c4 == 0) xs[row * CHUNK + b] = (uint8_t)byte;
+                }
+            }
         }
         __syncthreads();
 #pragma unroll
-        for (int b = 0; b < FEW_K / 128; ++b) {
+        for (int b = 0; b < CHUNK; ++b) {
             if (b < here) {
-                const float fw = __uint_as_float(((scales >> (8 * b)) & 0xFFu) << 23);
-                bf16x8 wf[4];
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    wf[2 * p] = widen8<false>(wv[b][p][0], wv[b][p][1], fw);
-                    wf[2 * p + 1] = widen8<false>(wv[b][p][2], wv[b][p][3], fw);
-                }
+                bf16x8 xf[MT][4];
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     const int row = t * 16 + r;
-                    const float fx = __uint_as_float((uint32_t)xs[row * (FEW_K / 128) + b] << 23);
+                    const float fx = scale_of(xs[row * CHUNK + b]);
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
                         const u32x4 c = *(const u32x4*)(xq + row * FEW_LD + b * 128 + p * 64 + q * 16);
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[2 * p], widen8<false>(c[0], c[1], fx), acc[t], 0, 0, 0);
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[2 * p + 1], widen8<false>(c[2], c[3], fx), acc[t], 0, 0, 0);
+                        xf[t][2 * p] = widen8<false>(c[0], c[1], fx);
+                        xf[t][2 * p + 1] = widen8<false>(c[2], c[3], fx);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const float fw = scale_of((scales[j] >> (8 * b)) & 0xFFu);
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        const u32x4& c = wv[j][b][p >> 1];
+                        const bf16x8 wf = widen8<false>(c[2 * (p & 1)], c[2 * (p & 1) + 1], fw);
+#pragma unroll
+                        for (int t = 0; t < MT; ++t)
+                            acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[t][p], acc[t][j], 0, 0, 0);
                     }
                 }
             }
         }
     }
-    // the weight's rows are the instruction's rows: lane (r, q) holds y[r][n0 + 4 q ..]
-    const int64_t col = n0 + 4 * q;
-    if (col < g.n) {
-        const Finish<T> to(g, col);
+    // the weight's rows are the instruction's rows: lane (r, q) holds y[r][n0 + 16 j + 4 q ..]
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-            if (t * 16 + r < f.m) to.store(g, t * 16 + r, acc[t]);
+    for (int j = 0; j < NT; ++j) {
+        const int64_t col = n0 + j * 16 + 4 * q;
+        if (col < g.n) {
+            const Finish<T> to(g, col);
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                if (t * 16 + r < f.m) to.store(g, t * 16 + r, acc[t][j]);
+        }
     }
 }
 
@@ -425,22 +450,32 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs g, const float* __re
 template <typename T>
 void launch_join(hipStream_t stream, const GemmArgs& g, const void* part, int splits) {
     const int64_t quads = g.m * ((g.n + 3) / 4);
-    // 8 waves a CU of one thread an element is 131072 elements; below that, threads share them
-    const bool share = quads < 131072 && splits >= 16;
-    const int64_t want = share ? (quads + 15) / 16 : (quads + 255) / 256;
+    // 8 waves a CU of one thread a quad are 131072 quads; below that, threads share them
+    const int groups = quads >= 131072 || splits < 4 ? 1 : quads >= 16384 || splits < 16 ? 4 : 16;
+    const int64_t want = (quads + 256 / groups - 1) / (256 / groups);
     const dim3 grid((unsigned)(want < 8192 ? want : 8192));
-    if (share)
+    if (groups == 16)
         hipLaunchKernelGGL((join_kernel<T, 16>), grid, dim3(256), 0, stream, g, (const float*)part, splits);
+    else if (groups == 4)
+        hipLaunchKernelGGL((join_kernel<T, 4>), grid, dim3(256), 0, stream, g, (const float*)part, splits);
     else
         hipLaunchKernelGGL((join_kernel<T, 1>), grid, dim3(256), 0, stream, g, (const float*)part, splits);
 }
 
-// 256 rows a tile where that leaves the card two workgroups a CU, 128 otherwise
-bool tall(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + TN - 1) / TN) >= 512; }
+// Tiles of 256 rows need a third less of the operands' bytes; those of 128 leave less of a tile outside the result, and three
+// workgroups of them share a CU, which hides a short sum's beginning and end.
+int64_t tiles_of(int64_t m, int64_t n, int rows) { return (m + rows - 1) / rows * ((n + TN - 1) / TN); }
+bool less_waste(int64_t m) { return 10 * ((m + 255) / 256 * 256) > 11 * ((m + 127) / 128 * 128); }  // by 128 rows, over 10 %
 
-// splits of the k axis: enough workgroups to fill 256 CUs twice, at least 4 blocks each
+// 262144 x 1024 x 1024: 590 us with 256 rows, 607 with 128; 16384 x 4096 x 4096: 453 and 491; 50001 x 832 x 320: 48 and 43
+bool tall(int64_t m, int64_t n, int64_t k) { return k >= 1024 && tiles_of(m, n, 256) >= 512 && !less_waste(m); }
+
+// A product whose tiles do not fill the card splits its k axis: 1024 x 1024 over 262144 takes 458 us with 256 rows a tile, 525
+// with 128
+bool split_tall(int64_t m) { return m > 128 && !less_waste(m); }
+// enough workgroups to fill 256 CUs twice, at least 4 blocks each
 int splits_of(int64_t m, int64_t n, int64_t k) {
-    const int64_t tm = m > 128 ? 256 : 128, tiles = ((m + tm - 1) / tm) * ((n + TN - 1) / TN), steps = fp8_blocks(k);
+    const int64_t tiles = tiles_of(m, n, split_tall(m) ? 256 : 128), steps = fp8_blocks(k);
     if (tiles >= 256 || steps < 8) return 1;
     int64_t s = (512 + tiles - 1) / tiles;
     if (s > steps / 4) s = steps / 4;
@@ -480,13 +515,19 @@ void launch_fp8_few_rows(hipStream_t stream, const void* x, int type, int64_t ld
     f.out.omega = omega;
     f.out.out = y;
     f.out.deriv = (__bf16*)deriv;
-    const dim3 grid((unsigned)((n + 63) / 64));
-#define SIREN_FEW(T)                                                                               \
-    do {                                                                                           \
-        if (m <= 16)                                                                               \
-            hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, dim3(256), 0, stream, f);            \
-        else                                                                                       \
-            hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, dim3(256), 0, stream, f);            \
+    // 32 columns a wave where that still is a workgroup a CU: half the rounding of x
+    const bool two = n >= 128 * 256;
+    const dim3 grid((unsigned)((n + (two ? 127 : 63)) / (two ? 128 : 64)));
+#define SIREN_FEW(T)                                                                                \
+    do {                                                                                            \
+        if (m <= 16 && two)                                                                         \
+            hipLaunchKernelGGL((few_rows_kernel<T, 1, 2>), grid, dim3(256), 0, stream, f);          \
+        else if (m <= 16)                                                                           \
+            hipLaunchKernelGGL((few_rows_kernel<T, 1, 1>), grid, dim3(256), 0, stream, f);          \
+        else if (two)                                                                               \
+            hipLaunchKernelGGL((few_rows_kernel<T, 2, 2>), grid, dim3(256), 0, stream, f);          \
+        else                                                                                        \
+            hipLaunchKernelGGL((few_rows_kernel<T, 2, 1>), grid, dim3(256), 0, stream, f);          \
     } while (0)
     if (type == FP8_F32) SIREN_FEW(float);
     if (type == FP8_BF16) SIREN_FEW(__bf16);
@@ -524,16 +565,16 @@ void launch_fp8_product(hipStream_t stream, const Fp8Product& p) {
     g.out = splits > 1 ? p.ws : p.out;
     if (splits > 1) {
         if (p.e5m2_a)
-            launch_gemm<float, true, true>(stream, g, splits, g.m > 128);
+            launch_gemm<float, true, true>(stream, g, splits, split_tall(g.m));
         else
-            launch_gemm<float, false, true>(stream, g, splits, g.m > 128);
+            launch_gemm<float, false, true>(stream, g, splits, split_tall(g.m));
         g.out = p.out;
         if (p.type == FP8_F32) launch_join<float>(stream, g, p.ws, splits);
         if (p.type == FP8_BF16) launch_join<__bf16>(stream, g, p.ws, splits);
         if (p.type == FP8_F16) launch_join<_Float16>(stream, g, p.ws, splits);
         return;
     }
-    const bool rows256 = tall(g.m, g.n);
+    const bool rows256 = tall(g.m, g.n, p.k);
     if (p.e5m2_a) {
         if (p.type == FP8_F32) launch_gemm<float, true, false>(stream, g, 1, rows256);
         if (p.type == FP8_BF16) launch_gemm<__bf16, true, false>(stream, g, 1, rows256);

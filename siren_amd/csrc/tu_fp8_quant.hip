@@ -66,6 +66,24 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[i][k] = (float)h[i][k];
         }
+    } else if (vec && (cols & 3) == 0) {
+        const bool in = c0 < cols;  // a quad is inside or outside
+        const int64_t c = in ? c0 : 0;
+        T4 h[16];
+        B4 f[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t r = r0 + i < rows ? r0 + i : rows - 1;
+            h[i] = *(const T4*)(x + r * ld + c);
+            if constexpr (MULT) f[i] = *(const B4*)(mult + r * cols + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[i][k] = in && r0 + i < rows ? (float)h[i][k] : 0.f;
+                if constexpr (MULT) v[i][k] *= in && r0 + i < rows ? (float)f[i][k] : 0.f;
+            }
     } else {
         T h[16][4];
 #pragma unroll

@@ -429,7 +429,7 @@ int32_t siren_laplace_backward_stored(const siren_cfg* cfg, const float* ws, con
 /* x (rows, cols) of row stride ld -> q, s: quantised along the columns; qt, st: the transpose (cols, rows), quantised
  * along the rows, laid out as a (cols, rows) tensor. Either pair may be NULL. panels: 1 for q, 2 for qt, 3 for both. mult (rows, cols) bf16, contiguous,
  * nullable: x is multiplied by it first. colsum (cols) fp32, nullable: the column sums of what is quantised, before
- * rounding (a bias's gradient), through colsum_ws of ceil(rows / 128) * cols floats. With rows == 0 nothing is
+ * rounding (a bias's gradient), through colsum_ws of ceil(rows / 128) * cols floats (NULL for up to 128 rows). With rows == 0 nothing is
  * written. */
 int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, const void* mult,
                            int32_t format, int32_t tiles, int32_t panels, void* q, void* s, void* qt, void* st,

@@ -1708,16 +1708,18 @@ int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t c
         return fail(SIREN_EINVAL, "siren_fp8_quantize: too many tiles");
     if ((q == nullptr) != (s == nullptr) || (qt == nullptr) != (st == nullptr))
         return fail(SIREN_EINVAL, "siren_fp8_quantize: values and scales go together");
-    if (colsum != nullptr && colsum_ws == nullptr) return fail(SIREN_EINVAL, "siren_fp8_quantize: colsum needs colsum_ws");
+    if (colsum != nullptr && colsum_ws == nullptr && rows > 128) return fail(SIREN_EINVAL, "siren_fp8_quantize: colsum needs colsum_ws");
     if (rows == 0 || cols == 0) return SIREN_OK;
     if (int rc = check_fp8_source(x, dtype, rows, cols, ld)) return rc;
     if (q == nullptr && qt == nullptr && colsum == nullptr) return fail(SIREN_EINVAL, "siren_fp8_quantize: nothing to write");
     if (!aligned(q, 16) || !aligned(qt, 16) || !aligned(s, 4) || !aligned(st, 4) || !aligned(mult, 2))
         return fail(SIREN_EINVAL, "siren_fp8_quantize: q and qt must be 16-byte aligned, scales 4-byte aligned");
+    // one row block's column sums are the sums
+    const bool one = rows <= 128;
     siren::Fp8Quant a{x, ld, rows, cols, mult, (uint8_t*)q, (uint8_t*)s, (uint8_t*)qt, (uint8_t*)st,
-                      colsum != nullptr ? colsum_ws : nullptr, dtype, format, tiles != 0, panels};
+                      colsum == nullptr || one ? colsum : colsum_ws, dtype, format, tiles != 0, panels};
     siren::launch_fp8_quant((hipStream_t)stream, a);
-    if (colsum != nullptr)
+    if (colsum != nullptr && !one)
         siren::launch_fp8_colsum((hipStream_t)stream, colsum_ws, siren::fp8_blocks(rows), cols, colsum);
     return hip_status("siren_fp8_quantize");
 }

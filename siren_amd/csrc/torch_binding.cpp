@@ -69,11 +69,15 @@ int64_t blocks(int64_t n) { return (n + 127) / 128; }
 int64_t padded(int64_t n) { return blocks(n) * 128; }
 int64_t words(int64_t n) { return (blocks(n) + 3) / 4 * 4; }
 
-// A quantised (rows, cols) tensor: values in rows (rows, padded cols) or in panels (padded cols / 64, rows, 64)
+// A quantised (rows, cols) tensor: values in rows (rows, padded cols) or in panels (padded cols / 64, rows, 64). What the
+// layer makes for itself is one allocation, values before scales (hold); what the user holds is two tensors.
 struct Blocks {
-    Tensor data, scale;
+    Tensor hold, data, scale;
     int64_t rows = 0, cols = 0;
-    int layout = 0;
+    int layout = 0, fmt = 0;
+    char* values() const { return (char*)(hold.defined() ? hold : data).data_ptr(); }
+    char* scales() const { return hold.defined() ? values() + rows * padded(cols) : (char*)scale.data_ptr(); }
+    const Tensor& any() const { return hold.defined() ? hold : data; }
 };
 
 // x as the kernels read it: columns one element apart, rows any distance that does not overlap
@@ -84,41 +88,46 @@ Tensor rows_of(const Tensor& x, int64_t& ld) {
     return y;
 }
 
-enum Want { PANELS = 1, TRANSPOSED_PANELS = 2, TILES = 4 };
+enum Want { PANELS = 1, TRANSPOSED_PANELS = 2, TILES = 4, TENSORS = 8 };
 
 // One pass over x (times mult): its rows, its transpose's rows, its column sums, as wanted
 void quantize_into(const Tensor& x0, int want, int fmt, const Tensor& mult, Blocks* q, Blocks* qt, Tensor* colsum) {
     int64_t ld;
     const Tensor x = rows_of(x0, ld);
     const int64_t rows = x.size(0), cols = x.size(1);
-    const auto bytes = x.options().dtype(fmt ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn);
     const auto u8 = x.options().dtype(at::kByte);
     const bool tiles = want & TILES;
     auto make = [&](Blocks* b, int64_t r, int64_t c, bool panels) {
-        b->data = panels ? at::empty({padded(c) / 64, r, 64}, bytes) : at::empty({r, padded(c)}, bytes);
-        b->scale = at::empty({tiles ? blocks(r) : r, words(c)}, u8);
+        const int64_t scale_rows = tiles ? blocks(r) : r;
+        if (want & TENSORS) {
+            b->data = at::empty({r, padded(c)}, x.options().dtype(fmt ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn));
+            b->scale = at::empty({scale_rows, words(c)}, u8);
+        } else {
+            b->hold = at::empty({r * padded(c) + scale_rows * words(c)}, u8);
+        }
         b->rows = r;
         b->cols = c;
         b->layout = (tiles ? SIREN_FP8_TILES : 0) | (panels ? SIREN_FP8_PANELS : 0);
+        b->fmt = fmt;
     };
     if (q) make(q, rows, cols, want & PANELS);
     if (qt) make(qt, cols, rows, want & TRANSPOSED_PANELS);
     Tensor ws;
     if (colsum) {
         const auto f32 = x.options().dtype(at::kFloat);
-        ws = at::empty({blocks(rows), cols}, f32);
+        if (rows > 128) ws = at::empty({blocks(rows), cols}, f32);
         *colsum = at::empty({cols}, f32);
     }
     const int panels = (want & PANELS ? 1 : 0) | (want & TRANSPOSED_PANELS ? 2 : 0);
     check(lib.quantize(x.data_ptr(), type_code(x.scalar_type()), rows, cols, ld, mult.defined() ? mult.data_ptr() : nullptr, fmt,
-                       tiles, panels, q ? q->data.data_ptr() : nullptr, q ? q->scale.data_ptr() : nullptr,
-                       qt ? qt->data.data_ptr() : nullptr, qt ? qt->scale.data_ptr() : nullptr,
-                       colsum ? ws.data_ptr<float>() : nullptr, colsum ? colsum->data_ptr<float>() : nullptr, stream_of(x)),
+                       tiles, panels, q ? q->values() : nullptr, q ? q->scales() : nullptr, qt ? qt->values() : nullptr,
+                       qt ? qt->scales() : nullptr, ws.defined() ? ws.data_ptr<float>() : nullptr,
+                       colsum ? colsum->data_ptr<float>() : nullptr, stream_of(x)),
           "siren_fp8_quantize");
 }
 
 Tensor product(const Blocks& a, const Blocks& b, const Tensor& bias, int act, double omega, at::ScalarType type, Tensor* deriv) {
-    const auto opt = a.scale.options();
+    const auto opt = a.any().options().dtype(at::kByte);
     Tensor out = at::empty({a.rows, b.rows}, opt.dtype(type));
     // the sine's derivative meets a gradient that is rounded to 3 bits of mantissa next: 8 bits of it are enough
     if (deriv) *deriv = at::empty({a.rows, b.rows}, opt.dtype(at::kBFloat16));
@@ -126,10 +135,9 @@ Tensor product(const Blocks& a, const Blocks& b, const Tensor& bias, int act, do
     check(lib.matmul_ws_bytes(a.rows, b.rows, a.cols, &need), "siren_fp8_matmul_ws_bytes");
     Tensor ws;
     if (need) ws = at::empty({need}, opt);
-    check(lib.matmul(a.data.data_ptr(), a.scale.data_ptr(), a.rows, a.layout, format_code(a.data.scalar_type()),
-                     b.data.data_ptr(), b.scale.data_ptr(), b.rows, b.layout, a.cols,
+    check(lib.matmul(a.values(), a.scales(), a.rows, a.layout, a.fmt, b.values(), b.scales(), b.rows, b.layout, a.cols,
                      bias.defined() ? bias.data_ptr<float>() : nullptr, act, (float)omega, out.data_ptr(), type_code(type),
-                     deriv ? deriv->data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, stream_of(a.scale)),
+                     deriv ? deriv->data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, stream_of(a.any())),
           "siren_fp8_matmul");
     return out;
 }
@@ -145,7 +153,7 @@ Tensor serve(const Tensor& x0, const Blocks& w, const Tensor& bias, int act, dou
     check(lib.linear_ws_bytes(m, w.rows, k, &need), "siren_fp8_linear_ws_bytes");
     Tensor ws;
     if (need) ws = at::empty({need}, x.options().dtype(at::kByte));
-    check(lib.linear(x.data_ptr(), type_code(x.scalar_type()), m, k, ld, w.data.data_ptr(), w.scale.data_ptr(), w.rows,
+    check(lib.linear(x.data_ptr(), type_code(x.scalar_type()), m, k, ld, w.values(), w.scales(), w.rows,
                      bias.defined() ? bias.data_ptr<float>() : nullptr, act, (float)omega, y.data_ptr(),
                      deriv ? deriv->data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, stream_of(x)),
           "siren_fp8_linear");
@@ -189,7 +197,7 @@ struct Linear : torch::autograd::Function<Linear> {
             quantize_into(weight.detach(), TILES | PANELS | TRANSPOSED_PANELS, 0, Tensor(), &qw, nx ? &qwt : nullptr, nullptr);
             y = product(qx, qw, b32, (int)act, omega, x.scalar_type(), want_deriv);
         }
-        ctx->save_for_backward({qxt.data, qxt.scale, qwt.data, qwt.scale, deriv});
+        ctx->save_for_backward({qxt.hold, qwt.hold, deriv});
         return y;
     }
 
@@ -212,13 +220,14 @@ struct Linear : torch::autograd::Function<Linear> {
         const auto saved = ctx->get_saved_variables();
         const bool create_graph = at::GradMode::is_enabled();
         {
-            const at::NoGradGuard none;
+            const at::NoGradGuard no_grad;
             Blocks q, qt;
             Tensor sums;
-            quantize_into(dy.detach(), PANELS | TRANSPOSED_PANELS, (int)fmt, saved[4], nx ? &q : nullptr, nw ? &qt : nullptr,
+            quantize_into(dy.detach(), PANELS | TRANSPOSED_PANELS, (int)fmt, saved[2], nx ? &q : nullptr, nw ? &qt : nullptr,
                           nb ? &sums : nullptr);
-            if (nx) dx = product(q, {saved[2], saved[3], k, n, SIREN_FP8_TILES | SIREN_FP8_PANELS}, Tensor(), 0, 0., tx, nullptr);
-            if (nw) dw = product(qt, {saved[0], saved[1], k, m, SIREN_FP8_PANELS}, Tensor(), 0, 0., tw, nullptr);
+            const Tensor none;
+            if (nx) dx = product(q, {saved[1], none, none, k, n, SIREN_FP8_TILES | SIREN_FP8_PANELS}, none, 0, 0., tx, nullptr);
+            if (nw) dw = product(qt, {saved[0], none, none, k, m, SIREN_FP8_PANELS}, none, 0, 0., tw, nullptr);
             if (nb) db = sums.to(tb);
         }
         if (create_graph) {
@@ -266,7 +275,8 @@ Blocks packed_operand(const Tensor& data, const Tensor& scale, int64_t cols, con
                       "Blocks must be contiguous, their data 16-byte and their scales 4-byte aligned");
     TORCH_CHECK_VALUE(data.device() == dev && scale.device() == dev, "Blocks on ", data.device(), " but the other operand on ", dev);
     // one row is both: its tile is its row block
-    return {data, scale, data.size(0), cols, tiles_only || scale.size(0) != data.size(0) ? SIREN_FP8_TILES : 0};
+    return {Tensor(), data, scale, data.size(0), cols, tiles_only || scale.size(0) != data.size(0) ? SIREN_FP8_TILES : 0,
+            format_code(data.scalar_type())};
 }
 
 std::pair<Tensor, Tensor> quantize(const Tensor& x, bool tiles, int64_t fmt) {
@@ -274,7 +284,7 @@ std::pair<Tensor, Tensor> quantize(const Tensor& x, bool tiles, int64_t fmt) {
     TORCH_CHECK_VALUE(x.dim() == 2, "x must be (rows, cols); got ", x.sizes());
     const c10::DeviceGuard guard(x.device());
     Blocks q;
-    quantize_into(x.detach(), tiles ? TILES : 0, (int)fmt, Tensor(), &q, nullptr, nullptr);
+    quantize_into(x.detach(), TENSORS | (tiles ? TILES : 0), (int)fmt, Tensor(), &q, nullptr, nullptr);
     return {q.data, q.scale};
 }
 
@@ -283,7 +293,7 @@ std::vector<Tensor> quantize_both(const Tensor& x, bool tiles, int64_t fmt) {
     TORCH_CHECK_VALUE(x.dim() == 2, "x must be (rows, cols); got ", x.sizes());
     const c10::DeviceGuard guard(x.device());
     Blocks q, qt;
-    quantize_into(x.detach(), tiles ? TILES : 0, (int)fmt, Tensor(), &q, &qt, nullptr);
+    quantize_into(x.detach(), TENSORS | (tiles ? TILES : 0), (int)fmt, Tensor(), &q, &qt, nullptr);
     return {q.data, q.scale, qt.data, qt.scale};
 }
 

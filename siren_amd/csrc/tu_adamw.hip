@@ -17,6 +17,7 @@
 #include <cmath>
 
 #include "adamw.h"
+#include "fp8_device.h"
 #include "rng.h"
 #include "siren_common.h"
 
@@ -117,14 +118,25 @@ template <typename T>
 __global__ __launch_bounds__(NORM_THREADS) void adamw_norm_kernel(AdamwTable tab, double* __restrict__ partial,
                                                                   int64_t* step, AdamwScalars* out, AdamwHyper h) {
     if (step != nullptr && blockIdx.x == 0 && threadIdx.x == 0) write_scalars(step, out, h);
+    // four chunks' loads before the first is squared
     double acc = 0.0;
-    for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-        const int k = find_tensor(tab, c);
-        const T* g = (const T*)tab.g[k];
-        const int64_t n = tab.n[k], i = (int64_t)(c - tab.first[k]) * CHUNK + threadIdx.x * 4;
-        const f32x4 v = load4(g, i, n, ((uintptr_t)g & (4 * sizeof(T) - 1)) == 0);
+    for (uint32_t c0 = blockIdx.x; c0 < tab.chunks; c0 += 4 * gridDim.x) {
+        f32x4 v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc = fma((double)v[e], (double)v[e], acc);
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t c = c0 + u * gridDim.x;
+            v[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (c < tab.chunks) {
+                const int k = find_tensor(tab, c);
+                const T* g = (const T*)tab.g[k];
+                v[u] = load4(g, (int64_t)(c - tab.first[k]) * CHUNK + threadIdx.x * 4, tab.n[k],
+                             ((uintptr_t)g & (4 * sizeof(T) - 1)) == 0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = fma((double)v[u][e], (double)v[u][e], acc);
     }
     __shared__ double red[NORM_THREADS / 64];
 #pragma unroll
@@ -168,13 +180,15 @@ __device__ __forceinline__ float apply(float p, float m, float u, float decay, f
     return __builtin_fmaf(-step_size * m, __builtin_amdgcn_rcpf(__builtin_fmaf(u, inv_root, eps)), p * decay);
 }
 
+// A workgroup's first chunk is asked for before the clip factor is made of the partial sums (one round trip less; the 8-bit
+// kernel's registers would lose a workgroup a CU for it).
 template <typename T>
 __global__ __launch_bounds__(256) void adamw32_kernel(AdamwTable tab, float* __restrict__ em, float* __restrict__ ev,
                                                       const AdamwScalars* __restrict__ sc, AdamwHyper h,
                                                       const double* __restrict__ partial, int parts,
                                                       float* __restrict__ norm_out) {
     __shared__ double red[4];
-    const float c = parts > 0 ? clip_factor(partial, parts, h.max_norm, norm_out, red) : 1.f;
+    float c = 1.f;
     const float step_size = sc->step_size, inv_root = 1.f / sc->root;
     for (uint32_t ch = blockIdx.x; ch < tab.chunks; ch += gridDim.x) {
         const int k = find_tensor(tab, ch);
@@ -193,6 +207,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwTable tab, float* __r
             mv[q] = *(const f32x4*)(em + off + i);  // the pad behind a tensor's end may be read, never written
             vv[q] = *(const f32x4*)(ev + off + i);
         }
+        if (ch == blockIdx.x && parts > 0) c = clip_factor(partial, parts, h.max_norm, norm_out, red);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int64_t i = base + q * (CHUNK / 2);
@@ -210,19 +225,6 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwTable tab, float* __r
             store4(ev + off, i, n, true, vv[q]);
         }
     }
-}
-
-__device__ __forceinline__ float max16(float v) {  // over the 16 lanes that hold one block
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
-    return v;
-}
-
-// the block's exponent byte: smallest power of two with which amax is at most 448 = 1.75 * 2^8 (amax finite)
-__device__ __forceinline__ int scale_byte(float amax) {
-    const uint32_t b = __float_as_uint(amax);
-    const int e = (int)(b >> 23) - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-    return e < 1 ? 1 : e;
 }
 
 // e4m3's code of |x| / scale, rounded up where the 16 bits r say so: the scaled magnitude times 2^-120 is an fp32
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamwTable tab, uint8_t* __
             gv[q] = load4(g, i + 4 * q, n, vec);
         }
         const u32x2 mc = *(const u32x2*)(em + off + i), uc = *(const u32x2*)(eu + off + i);
-        const float ms = __uint_as_float((uint32_t)sm[blk] << 23), us = __uint_as_float((uint32_t)su[blk] << 23);
+        const float ms = scale_of(sm[blk]), us = scale_of(su[blk]);
         float m[8], u[8];
         float mmax = 0.f, umax = 0.f;
         bool mok = true, uok = true;
@@ -289,11 +291,11 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamwTable tab, uint8_t* __
             }
         }
         // a block with an infinity or a NaN is held as a NaN (byte 255, codes 0); the maximum carries the fact
-        mmax = max16(mok ? mmax : INFINITY);
-        umax = max16(uok ? umax : INFINITY);
+        mmax = row16_max(mok ? mmax : INFINITY);
+        umax = row16_max(uok ? umax : INFINITY);
         const bool mbad = !finite(mmax), ubad = !finite(umax);
-        const int mb = scale_byte(mmax), ub = scale_byte(umax);
-        const float mi = __uint_as_float((uint32_t)(254 - mb) << 23), ui = __uint_as_float((uint32_t)(254 - ub) << 23);
+        const int mb = exponent_byte<false>(mmax), ub = exponent_byte<false>(umax);
+        const float mi = scale_of(254 - mb), ui = scale_of(254 - ub);
         u32x2 mo = {0u, 0u}, uo = {0u, 0u};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {

@@ -24,7 +24,7 @@ def test_quantize_validates(lib):
         return lib.siren_fp8_quantize(x, dtype, rows, cols, ld, mult, fmt, tiles, 0, q, s, qt, st, ws, sums, None)
     assert call(rows=0) == OK and call(cols=0, ld=0) == OK
     for bad in (dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(cols=-1), dict(ld=7), dict(fmt=2), dict(s=None), dict(q=None),
-                dict(qt=P(64)), dict(st=P(64)), dict(sums=P(64)), dict(x=None), dict(q=None, s=None), dict(q=P(72)),
+                dict(qt=P(64)), dict(st=P(64)), dict(rows=129, sums=P(64)), dict(x=None), dict(q=None, s=None), dict(q=P(72)),
                 dict(x=P(66)), dict(dtype=1, x=P(65)), dict(qt=P(8), st=P(64)),
                 dict(rows=1 << 40, cols=1 << 30, ld=1 << 30)):
         assert call(**bad) == EINVAL, bad

@@ -6,6 +6,7 @@
 // an AdamW step over ten tensors 29 us (of 9), a layer for one row 19 us. No kernel is here, and no copy of the C ABI: the
 // functions are taken from the library that siren_amd/_lib.py loaded (bind).
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
@@ -169,6 +170,20 @@ struct NotTwice : torch::autograd::Function<NotTwice> {
         TORCH_CHECK(false, "fp8.linear: its gradients are not differentiable again (second derivatives need the fp32 kernels)");
     }
 };
+
+// A backward that is captured while an eager graph of the same leaf lives would make the engine wait for that graph's
+// stream, which a capture may not: the process ends. The leaf's accumulator tells, so the call is refused instead.
+void check_capture(std::initializer_list<const Tensor*> leaves) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor* t : leaves) {
+        if (!t->defined() || !t->requires_grad() || t->grad_fn()) continue;
+        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto stream = accumulator ? accumulator->stream() : std::nullopt;
+        TORCH_CHECK(!stream || stream->id() == c10::hip::getCurrentHIPStream(t->device().index()).id(),
+                    "fp8.linear: this capture uses a leaf that an eager graph made on another stream still holds; its backward "
+                    "cannot be captured. Delete what that graph returned first, or warm up on the stream that captures");
+    }
+}
 
 // y = act(x W^T + b) with gradients. x is read once in the forward and dy once in the backward, each quantised both along
 // its rows and along its columns in that pass; the weight's tiles serve both directions.
@@ -335,8 +350,12 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& maybe_bi
     TORCH_CHECK_VALUE(weight.dim() == 2, "weight must be (out, in); got ", weight.sizes());
     TORCH_CHECK_VALUE(weight.device() == x.device(), "weight on ", weight.device(), " but x on ", x.device());
     const Tensor x2 = check_layer(x, bias, weight.size(0), weight.size(1), omega);
-    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad())))
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()))) {
+        TORCH_CHECK_VALUE(!weight.requires_grad() || x2.size(0) < (1 << 24), "a weight's gradient sums over fewer than 2^24 rows; got ",
+                          x2.size(0));
+        check_capture({&x, &weight, &bias});
         return like_input(x, Linear::apply(x2, weight, bias, act, omega, fmt));
+    }
     const c10::DeviceGuard guard(x.device());
     Blocks w;
     quantize_into(weight.detach(), TILES, 0, Tensor(), &w, nullptr, nullptr);
@@ -409,6 +428,9 @@ MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Mayb
                          sm ? sm->data_ptr() : nullptr, sv ? sv->data_ptr() : nullptr, step.data_ptr<int64_t>(), lr, b1, b2, eps,
                          weight_decay, max_norm.value_or(0.), seed, scratch.data_ptr(), stream_of(step)),
           "siren_adamw_step");
+    // written behind autograd's back: a graph that saved a parameter must notice
+    for (size_t i = 0; i < n; ++i)
+        if (gs[i]) torch::autograd::impl::bump_version(params[i]);
     return max_norm ? MaybeTensor(scratch.select(0, 8)) : std::nullopt;
 }
 

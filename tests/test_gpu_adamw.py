@@ -328,6 +328,23 @@ def test_state_dict_resumes(cuda):
         assert all(torch.equal(p, q) for p, q in zip(*runs))
 
 
+def test_autograd_notices_a_step(cuda):
+    """A graph that saved a parameter refuses its backward after a step, as with torch's optimisers; a parameter without a
+    gradient was not touched."""
+    from siren_amd.optim import FusedAdamW
+    p, q = (torch.ones(5, device=cuda, requires_grad=True) for _ in range(2))
+    opt = FusedAdamW([p, q], max_norm=1.)
+    opt.step()  # nothing has a gradient
+    assert float(opt.grad_norm()) == 0. and (p == 1).all() and int(opt.steps) == 1
+    p.grad = torch.ones_like(p)
+    saved, other = (p * p).sum(), (q * q).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        saved.backward()
+    other.backward()
+    assert torch.equal(q.grad, 2 * torch.ones_like(q))
+
+
 def test_refusals(cuda):
     from siren_amd.optim import FusedAdamW, adamw_step
     p = torch.ones(300, device=cuda)

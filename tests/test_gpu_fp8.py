@@ -412,6 +412,28 @@ def test_captured_training_step(cuda):
         assert all(torch.equal(p, q) for p, q in zip(want, got))
 
 
+def test_capture_beside_an_eager_graph_is_refused(cuda):
+    """A capture whose leaf an eager graph still holds is refused before the engine could meet it, and works once that graph
+    is gone. (A graph made on the capturing stream itself is no obstacle.)"""
+    from siren_amd import fp8
+    x, w, b = layer(40, 64, 64, torch.float32, cuda)
+    w.requires_grad_(True)
+    eager = fp8.linear(x, w, b)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match='eager graph'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            fp8.linear(x, w, b)
+    want, = torch.autograd.grad(eager.sum(), w)
+    del eager
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = fp8.linear(x, w, b) + fp8.linear(x, w, b)  # the capture's own graph of the leaf is no obstacle
+        got, = torch.autograd.grad(y, w, torch.ones_like(y))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, 2 * want)
+
+
 def test_offsets_past_32_bits(cuda):
     """Rows whose bytes, and outputs whose elements, begin past 2^32."""
     from siren_amd import fp8

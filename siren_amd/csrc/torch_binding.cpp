@@ -424,13 +424,14 @@ MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Mayb
     check(lib.adamw_scratch_bytes((int64_t)n, &need), "siren_adamw_scratch_bytes");
     const c10::DeviceGuard guard(dev);
     const Tensor scratch = at::empty({need / 4}, step.options().dtype(at::kFloat));
+    // Written behind autograd's back: a graph that saved a parameter must notice. Before the launch: this is what refuses
+    // a parameter made in inference mode
+    for (size_t i = 0; i < n; ++i)
+        if (gs[i]) torch::autograd::impl::bump_version(params[i]);
     check(lib.adamw_step((int64_t)n, ps.data(), gs.data(), numels.data(), types.data(), sm ? 8 : 32, m.data_ptr(), v.data_ptr(),
                          sm ? sm->data_ptr() : nullptr, sv ? sv->data_ptr() : nullptr, step.data_ptr<int64_t>(), lr, b1, b2, eps,
                          weight_decay, max_norm.value_or(0.), seed, scratch.data_ptr(), stream_of(step)),
           "siren_adamw_step");
-    // written behind autograd's back: a graph that saved a parameter must notice
-    for (size_t i = 0; i < n; ++i)
-        if (gs[i]) torch::autograd::impl::bump_version(params[i]);
     return max_norm ? MaybeTensor(scratch.select(0, 8)) : std::nullopt;
 }
 

@@ -173,8 +173,9 @@ __device__ __forceinline__ void moments(float g, float& m, float& v, float omb1,
     v = v * b2 + (g * g) * omb2;
 }
 
-// p (1 - lr wd) - step m / (u / root + eps); reciprocals of one unit in the last place: the update's own error is
-// far below p's rounding
+// p (1 - lr wd) - step m / (u / root + eps); a reciprocal of one unit in the last place: the update's own error is far
+// below p's rounding. u comes from the full square root: the card's own takes a subnormal v for zero, and with a small eps
+// the step would be infinite.
 __device__ __forceinline__ float apply(float p, float m, float u, float decay, float step_size, float inv_root,
                                        float eps) {
     return __builtin_fmaf(-step_size * m, __builtin_amdgcn_rcpf(__builtin_fmaf(u, inv_root, eps)), p * decay);
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwTable tab, float* __r
                 moments(c * gv[q][e], m, v, h.omb1, h.b2f, h.omb2);
                 mv[q][e] = m;
                 vv[q][e] = v;
-                pv[q][e] = apply(pv[q][e], m, __builtin_amdgcn_sqrtf(v), h.decay, step_size, inv_root, h.epsf);
+                pv[q][e] = apply(pv[q][e], m, __builtin_sqrtf(v), h.decay, step_size, inv_root, h.epsf);
             }
             store4(p, i, n, vec, pv[q]);
             store4(em + off, i, n, true, mv[q]);

@@ -369,3 +369,28 @@ def test_refusals(cuda):
         FusedAdamW([p], state_bits=16)
     with pytest.raises(ValueError):
         opt.load_state_dict(FusedAdamW([p], state_bits=8).state_dict())
+
+
+@pytest.mark.parametrize('eps', [0., 1e-25, 1e-8])
+def test_subnormal_second_moments(cuda, eps):
+    """Gradients of 1e-19 to 1e-20: v is a subnormal number, its root is not, and the step is lr all the same."""
+    from siren_amd.optim import FusedAdamW
+    p = torch.ones(700, device=cuda).requires_grad_(True)
+    opt = FusedAdamW([p], lr=1e-2, eps=eps, weight_decay=0.)
+    p.grad = torch.logspace(-19, -20, 700).to(cuda)
+    opt.step()
+    m, v = opt.exp_avg[:700].cpu().numpy(), opt.exp_avg_sq[:700].cpu().numpy()
+    assert (v > 0).all() and (v < 2. ** -126).all()
+    want, step = update(np.ones(700), m, np.sqrt(v.astype(np.float64)), 1, 1e-2, 0.9, 0.999, eps, 0.)
+    check_params(p.detach().cpu().numpy().astype(np.float64), want, step, torch.float32)
+
+
+def test_inference_parameters_are_refused_unchanged(cuda):
+    from siren_amd import optim
+    with torch.inference_mode():
+        p = torch.ones(300, device=cuda)
+        g = torch.ones(300, device=cuda)
+    opt = optim.FusedAdamW([torch.ones(300, device=cuda)])
+    with pytest.raises(RuntimeError, match='nference'):
+        optim.adamw_step([p], [g], opt.exp_avg, opt.exp_avg_sq, opt.steps)
+    assert bool((p == 1).all()) and int(opt.steps) == 0

@@ -427,25 +427,26 @@ int32_t siren_laplace_backward_stored(const siren_cfg* cfg, const float* ws, con
 #define SIREN_FP8_PANELS 2 /* its values in panels instead of rows                              */
 
 /* x (rows, cols) of row stride ld -> q, s: quantised along the columns; qt, st: the transpose (cols, rows), quantised
- * along the rows, laid out as a (cols, rows) tensor. Either pair may be NULL. panels: 1 for q, 2 for qt, 3 for both. mult (rows, cols) bf16, contiguous,
- * nullable: x is multiplied by it first. colsum (cols) fp32, nullable: the column sums of what is quantised, before
- * rounding (a bias's gradient), through colsum_ws of ceil(rows / 128) * cols floats (NULL for up to 128 rows). With rows == 0 nothing is
- * written. */
+ * along the rows, laid out as a (cols, rows) tensor. Either pair may be NULL. panels: 1 for q, 2 for qt, 3 for both.
+ * mult (rows, cols) bf16, contiguous, 16-byte aligned, nullable: x is multiplied by it first.
+ * colsum (cols) fp32, nullable: the column sums of what is quantised, before rounding (a bias's gradient), through
+ * colsum_ws of ceil(rows / 128) * cols floats (NULL for up to 128 rows).
+ * With rows == 0 nothing is written. */
 int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, const void* mult,
                            int32_t format, int32_t tiles, int32_t panels, void* q, void* s, void* qt, void* st,
                            float* colsum_ws, float* colsum, void* stream);
 
-/* out (m, n) = act(a b^T + bias) of a (m, k) and b (n, k) quantised along k (k < 2^24, n < 2^22), sums in 32 bits. a may be e4m3 or e5m2,
- * b is e4m3. act 0: none, 1: sin(omega z), with deriv (m, n) bf16, nullable, = omega cos(omega z). bias (n) fp32,
- * nullable. ws: siren_fp8_matmul_ws_bytes(m, n, k) bytes. */
+/* out (m, n) = act(a b^T + bias) of a (m, k) and b (n, k) quantised along k (k < 2^24, n < 2^22), sums in 32 bits.
+ * a may be e4m3 or e5m2, b is e4m3. act 0: none, 1: sin(omega z), with deriv (m, n) bf16, nullable, = omega cos(omega z).
+ * bias (n) fp32, nullable. ws: siren_fp8_matmul_ws_bytes(m, n, k) bytes. */
 int32_t siren_fp8_matmul_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes);
 int32_t siren_fp8_matmul(const void* a, const void* sa, int64_t m, int32_t a_layout, int32_t a_format, const void* b,
                          const void* sb, int64_t n, int32_t b_layout, int64_t k, const float* bias, int32_t act,
                          float omega, void* out, int32_t dtype, void* deriv, void* ws, void* stream);
 
 /* y (m, n) = act(x w^T + bias), the layer of siren_fp8_quantize (rows of x, e4m3) and siren_fp8_matmul in one call:
- * x (m, k) of row stride ld, w (n, k) in 8 bits, tiles, in rows, y in x's dtype, deriv
- * as above. ws: siren_fp8_linear_ws_bytes (0 for up to 32 rows, which are one launch). */
+ * x (m, k) of row stride ld, w (n, k) in 8 bits, tiles, in rows, y in x's dtype, deriv as
+ * above. ws: siren_fp8_linear_ws_bytes (0 for up to 32 rows, which are one launch). */
 int32_t siren_fp8_linear_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes);
 int32_t siren_fp8_linear(const void* x, int32_t dtype, int64_t m, int64_t k, int64_t ld, const void* w, const void* sw,
                          int64_t n, const float* bias, int32_t act, float omega, void* y, void* deriv, void* ws, void* stream);

@@ -1662,7 +1662,7 @@ int32_t siren_backward_stored_batched(const siren_cfg* cfg, const float* ws, con
 // ---- 8-bit training: block quantisation, products of 8-bit operands, AdamW over many tensors ------------------------
 namespace {
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
-constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+constexpr int64_t kMaxGrid = 0xFFFFFF;  // workgroups of 256 threads: a launch holds fewer than 2^32 threads
 
 int check_fp8_type(int32_t dtype) {
     return dtype >= siren::FP8_F32 && dtype <= siren::FP8_F16 ? SIREN_OK : fail(SIREN_EINVAL, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
@@ -1704,16 +1704,18 @@ int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t c
     if (int rc = check_fp8_type(dtype)) return rc;
     if (rows < 0 || cols < 0 || (format != 0 && format != 1) || (panels & ~3) != 0)
         return fail(SIREN_EINVAL, "siren_fp8_quantize: need rows, cols >= 0, format 0 (e4m3) or 1 (e5m2) and panels in 0..3");
-    if (siren::fp8_blocks(cols) > kMaxGrid / std::max<int64_t>(1, siren::fp8_blocks(rows)))
-        return fail(SIREN_EINVAL, "siren_fp8_quantize: too many tiles");
+    // in the order of their sizes in threads: the column sums' launch, a tile a workgroup, 32 rows of a block a workgroup
+    if ((colsum != nullptr && siren::fp8_blocks(cols) > kMaxGrid / 16) ||
+        siren::fp8_blocks(cols) > kMaxGrid / std::max<int64_t>(1, siren::fp8_blocks(rows) * (qt == nullptr ? 4 : 1)))
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: too many tiles for one launch");
     if ((q == nullptr) != (s == nullptr) || (qt == nullptr) != (st == nullptr))
         return fail(SIREN_EINVAL, "siren_fp8_quantize: values and scales go together");
     if (colsum != nullptr && colsum_ws == nullptr && rows > 128) return fail(SIREN_EINVAL, "siren_fp8_quantize: colsum needs colsum_ws");
     if (rows == 0 || cols == 0) return SIREN_OK;
     if (int rc = check_fp8_source(x, dtype, rows, cols, ld)) return rc;
     if (q == nullptr && qt == nullptr && colsum == nullptr) return fail(SIREN_EINVAL, "siren_fp8_quantize: nothing to write");
-    if (!aligned(q, 16) || !aligned(qt, 16) || !aligned(s, 4) || !aligned(st, 4) || !aligned(mult, 2))
-        return fail(SIREN_EINVAL, "siren_fp8_quantize: q and qt must be 16-byte aligned, scales 4-byte aligned");
+    if (!aligned(q, 16) || !aligned(qt, 16) || !aligned(s, 4) || !aligned(st, 4) || !aligned(mult, 16))
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: q, qt and mult must be 16-byte aligned, scales 4-byte aligned");
     // one row block's column sums are the sums
     const bool one = rows <= 128;
     siren::Fp8Quant a{x, ld, rows, cols, mult, (uint8_t*)q, (uint8_t*)s, (uint8_t*)qt, (uint8_t*)st,

@@ -460,3 +460,16 @@ def test_rows_of_a_batch_do_not_depend_on_it(cuda):
     tol = 2 * product_tol(xq, wq, np64(y), torch.float32, np.abs(np64(b)))
     for m in (1, 2, 5, 16, 17, 31, 32, 33, 64, 65, 128, 129, 257):
         check(fp8.linear(x[:m], w8, b), np64(y)[:m], tol[:m], m)
+
+
+@pytest.mark.parametrize('m', [3, 40, 600])
+def test_sine_of_what_is_not_finite(cuda, m):
+    """sin(omega z) and its derivative of an infinite or NaN z are NaN, and a huge one's stay within 1 and omega."""
+    from siren_amd import fp8
+    w = torch.ones(5, 70, device=cuda)
+    bias = torch.tensor([math.inf, -math.inf, math.nan, 1e38, 0.], device=cuda)
+    x = torch.full((m, 70), 0.01, device=cuda)
+    y, d = fp8.matmul(fp8.quantize(x), fp8.quantize(w, 'tile'), bias, 'sine', omega=2., derivative=True)
+    for got, top in ((y, 1.), (d.float(), 2.), (fp8.linear(x, fp8.quantize(w, 'tile'), bias, 'sine', omega=2.), 1.)):
+        assert bool(got[:, :3].isnan().all())
+        assert bool((got[:, 3:].abs() <= top).all())

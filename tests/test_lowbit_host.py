@@ -26,7 +26,8 @@ def test_quantize_validates(lib):
     for bad in (dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(cols=-1), dict(ld=7), dict(fmt=2), dict(s=None), dict(q=None),
                 dict(qt=P(64)), dict(st=P(64)), dict(rows=129, sums=P(64)), dict(x=None), dict(q=None, s=None), dict(q=P(72)),
                 dict(x=P(66)), dict(dtype=1, x=P(65)), dict(qt=P(8), st=P(64)),
-                dict(rows=1 << 40, cols=1 << 30, ld=1 << 30)):
+                dict(rows=1 << 40, cols=1 << 30, ld=1 << 30), dict(rows=1 << 29, cols=128, ld=128), dict(mult=P(72)),
+                dict(rows=1 << 31, qt=P(64), st=P(64)), dict(rows=2, cols=1 << 27, ld=1 << 27, sums=P(64))):
         assert call(**bad) == EINVAL, bad
         assert lib.siren_last_error()
 

@@ -8,6 +8,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -185,64 +186,48 @@ void check_capture(std::initializer_list<const Tensor*> leaves) {
     }
 }
 
-// y = act(x W^T + b) with gradients. x is read once in the forward and dy once in the backward, each quantised both along
-// its rows and along its columns in that pass; the weight's tiles serve both directions.
-struct Linear : torch::autograd::Function<Linear> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t act,
-                          double omega, int64_t fmt) {
-        const bool nx = x.requires_grad(), nw = weight.requires_grad(), nb = bias.defined() && bias.requires_grad();
-        const int64_t m = x.size(0), n = weight.size(0), k = weight.size(1);
-        ctx->saved_data["dims"] = std::vector<int64_t>{m, n, k, fmt, nx, nw, nb};
-        ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(),
-                                                        bias.defined() ? (int64_t)bias.scalar_type() : 0};
-        if (m == 0) return x.new_empty({0, n});  // no products, gradients of zero
-        const c10::DeviceGuard guard(x.device());
-        const Tensor xd = x.detach(), b32 = bias32(bias);
-        Blocks qx, qxt, qw, qwt;
-        Tensor deriv, y;
-        Tensor* want_deriv = act && (nx || nw || nb) ? &deriv : nullptr;
-        int64_t ws = 0;
-        check(lib.linear_ws_bytes(m, n, k, &ws), "siren_fp8_linear_ws_bytes");
-        if (ws == 0) {  // few rows: the product quantises them itself, and reads the weight in rows
-            quantize_into(weight.detach(), TILES | TRANSPOSED_PANELS, 0, Tensor(), &qw, nx ? &qwt : nullptr, nullptr);
-            y = serve(xd, qw, b32, (int)act, omega, want_deriv);
-            if (nw) quantize_into(xd, TRANSPOSED_PANELS, 0, Tensor(), nullptr, &qxt, nullptr);
-        } else {
-            quantize_into(xd, PANELS | TRANSPOSED_PANELS, 0, Tensor(), &qx, nw ? &qxt : nullptr, nullptr);
-            quantize_into(weight.detach(), TILES | PANELS | TRANSPOSED_PANELS, 0, Tensor(), &qw, nx ? &qwt : nullptr, nullptr);
-            y = product(qx, qw, b32, (int)act, omega, x.scalar_type(), want_deriv);
-        }
-        ctx->save_for_backward({qxt.hold, qwt.hold, deriv});
-        return y;
+// The backward of y = act(x W^T + b): x was read once in the forward, dy is read once here, each quantised both along its
+// rows and along its columns in that pass; the weight's tiles serve both directions. A Node of its own rather than a
+// torch::autograd::Function, whose dictionary and bookkeeping cost 4 us of the 88 of a training step of 8 x 128 x 128 (all of
+// it host time, half the engine's own).
+struct LinearBackward : torch::autograd::Node {
+    int64_t m = 0, n = 0, k = 0, fmt = 0;
+    at::ScalarType tx = at::kFloat, tw = at::kFloat, tb = at::kFloat;
+    torch::autograd::SavedVariable qxt, qwt, deriv;  // saved as torch saves, so that its hooks (checkpointing) see them
+
+    std::string name() const override { return "Fp8LinearBackward"; }
+
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        qxt.reset_data();
+        qwt.reset_data();
+        deriv.reset_data();
     }
 
-    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-        const auto dims = ctx->saved_data["dims"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
-        const int64_t m = dims[0], n = dims[1], k = dims[2], fmt = dims[3];
-        const bool nx = dims[4], nw = dims[5], nb = dims[6];
-        const auto tx = (at::ScalarType)types[0], tw = (at::ScalarType)types[1], tb = (at::ScalarType)types[2];
+    variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1), nb = task_should_compute_output(2);
         Tensor dx, dw, db;
-        const Tensor dy = grads[0];
-        if (!dy.defined()) return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+        const Tensor& dy = grads[0];
+        if (!dy.defined()) return {dx, dw, db};
         const auto opt = dy.options();
         if (m == 0) {
             if (nx) dx = at::empty({0, k}, opt.dtype(tx));
             if (nw) dw = at::zeros({n, k}, opt.dtype(tw));
             if (nb) db = at::zeros({n}, opt.dtype(tb));
-            return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+            return {dx, dw, db};
         }
         const c10::DeviceGuard guard(dy.device());
-        const auto saved = ctx->get_saved_variables();
         const bool create_graph = at::GradMode::is_enabled();
         {
             const at::NoGradGuard no_grad;
             Blocks q, qt;
             Tensor sums;
-            quantize_into(dy.detach(), PANELS | TRANSPOSED_PANELS, (int)fmt, saved[2], nx ? &q : nullptr, nw ? &qt : nullptr,
+            quantize_into(dy.detach(), PANELS | TRANSPOSED_PANELS, (int)fmt, deriv.unpack(), nx ? &q : nullptr, nw ? &qt : nullptr,
                           nb ? &sums : nullptr);
             const Tensor none;
-            if (nx) dx = product(q, {saved[1], none, none, k, n, SIREN_FP8_TILES | SIREN_FP8_PANELS}, none, 0, 0., tx, nullptr);
-            if (nw) dw = product(qt, {saved[0], none, none, k, m, SIREN_FP8_PANELS}, none, 0, 0., tw, nullptr);
+            if (nx) dx = product(q, {qwt.unpack(), none, none, k, n, SIREN_FP8_TILES | SIREN_FP8_PANELS}, none, 0, 0., tx, nullptr);
+            if (nw) dw = product(qt, {qxt.unpack(), none, none, k, m, SIREN_FP8_PANELS}, none, 0, 0., tw, nullptr);
             if (nb) db = sums.to(tb);
         }
         if (create_graph) {
@@ -250,9 +235,52 @@ struct Linear : torch::autograd::Function<Linear> {
             for (Tensor* g : {&dx, &dw, &db})
                 if (g->defined()) *g = NotTwice::apply(*g, anchor);
         }
-        return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+        return {dx, dw, db};
     }
 };
+
+// y = act(x W^T + b) with gradients
+Tensor train(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t act, double omega, int64_t fmt) {
+    const bool nx = x.requires_grad(), nw = weight.requires_grad();
+    const std::shared_ptr<LinearBackward> node(new LinearBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
+    node->m = x.size(0);
+    node->n = weight.size(0);
+    node->k = weight.size(1);
+    node->fmt = fmt;
+    node->tx = x.scalar_type();
+    node->tw = weight.scalar_type();
+    if (bias.defined()) node->tb = bias.scalar_type();
+    Tensor y;
+    {
+        const at::NoGradGuard no_grad;
+        if (node->m == 0) {  // no products, gradients of zero
+            y = x.new_empty({0, node->n});
+        } else {
+            const c10::DeviceGuard guard(x.device());
+            const Tensor b32 = bias32(bias);
+            Blocks qx, qxt, qw, qwt;
+            Tensor d;
+            Tensor* deriv = act ? &d : nullptr;
+            int64_t ws = 0;
+            check(lib.linear_ws_bytes(node->m, node->n, node->k, &ws), "siren_fp8_linear_ws_bytes");
+            if (ws == 0) {  // few rows: the product quantises them itself, and reads the weight in rows
+                quantize_into(weight, TILES | TRANSPOSED_PANELS, 0, Tensor(), &qw, nx ? &qwt : nullptr, nullptr);
+                y = serve(x, qw, b32, (int)act, omega, deriv);
+                if (nw) quantize_into(x, TRANSPOSED_PANELS, 0, Tensor(), nullptr, &qxt, nullptr);
+            } else {
+                quantize_into(x, PANELS | TRANSPOSED_PANELS, 0, Tensor(), &qx, nw ? &qxt : nullptr, nullptr);
+                quantize_into(weight, TILES | PANELS | TRANSPOSED_PANELS, 0, Tensor(), &qw, nx ? &qwt : nullptr, nullptr);
+                y = product(qx, qw, b32, (int)act, omega, x.scalar_type(), deriv);
+            }
+            node->qxt = torch::autograd::SavedVariable(qxt.hold, false);
+            node->qwt = torch::autograd::SavedVariable(qwt.hold, false);
+            node->deriv = torch::autograd::SavedVariable(d, false);
+        }
+    }
+    torch::autograd::set_history(y, node);
+    return y;
+}
 
 Tensor check_layer(const Tensor& x, const Tensor& bias, int64_t n, int64_t k, double omega) {
     check_input(x, "x");
@@ -354,7 +382,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& maybe_bi
         TORCH_CHECK_VALUE(!weight.requires_grad() || x2.size(0) < (1 << 24), "a weight's gradient sums over fewer than 2^24 rows; got ",
                           x2.size(0));
         check_capture({&x, &weight, &bias});
-        return like_input(x, Linear::apply(x2, weight, bias, act, omega, fmt));
+        return like_input(x, train(x2, weight, bias, act, omega, fmt));
     }
     const c10::DeviceGuard guard(x.device());
     Blocks w;

@@ -473,3 +473,31 @@ def test_sine_of_what_is_not_finite(cuda, m):
     for got, top in ((y, 1.), (d.float(), 2.), (fp8.linear(x, fp8.quantize(w, 'tile'), bias, 'sine', omega=2.), 1.)):
         assert bool(got[:, :3].isnan().all())
         assert bool((got[:, 3:].abs() <= top).all())
+
+
+@pytest.mark.parametrize('m', [5, 200])
+@pytest.mark.parametrize('act', [None, 'sine'])
+def test_graph_is_used_as_any_other(cuda, m, act):
+    """Parts of the gradients, a graph kept for two backward passes and refused a third, leaves that accumulate, hooks on what
+    is saved and recomputation: the same bytes each time."""
+    from torch.utils.checkpoint import checkpoint
+    from siren_amd import fp8
+    x, w, b = (torch.randn(*s, device=cuda, requires_grad=True) for s in ((m, 130), (70, 130), (70,)))
+    dy = torch.randn(m, 70, device=cuda)
+    y = fp8.linear(x, w, b, act)
+    want = torch.autograd.grad(y, (x, w, b), dy, retain_graph=True)
+    for i, leaf in enumerate((x, w, b)):
+        assert torch.equal(torch.autograd.grad(y, (leaf,), dy, retain_graph=True)[0], want[i])
+    y.backward(dy)
+    with pytest.raises(RuntimeError, match='second time'):
+        y.backward(dy)
+    assert all(torch.equal(leaf.grad, g) for leaf, g in zip((x, w, b), want))
+    fp8.linear(x, w, b, act).backward(dy)
+    assert all(torch.equal(leaf.grad, 2 * g) for leaf, g in zip((x, w, b), want))
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.numel()) or t, lambda t: t):
+        y = fp8.linear(x, w, b, act)
+    assert len(seen) == (3 if act else 2)
+    assert all(torch.equal(p, g) for p, g in zip(torch.autograd.grad(y, (x, w, b), dy), want))
+    y = checkpoint(lambda *a: fp8.linear(*a, act), x, w, b, use_reentrant=False)
+    assert all(torch.equal(p, g) for p, g in zip(torch.autograd.grad(y, (x, w, b), dy), want))

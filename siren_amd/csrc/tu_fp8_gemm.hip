@@ -10,8 +10,11 @@
 //
 // A workgroup of 4 waves owns 256 x 128 of out (128 x 128 where rows are few), each wave 128 x 64 (64 x 64) in tiles of
 // 32 x 32. Half a block, 64 k of both operands, is one stage of LDS: 24 KiB by direct global-to-LDS loads, three stages, so
-// the loads run two half blocks ahead; two workgroups share a CU, and one's stores run behind the other's products. An
-// LDS row is 64 bytes of one operand row; its 16-byte pieces are permuted by (row >> 2) & 3 on the way in, so that the 16
+// the loads run two half blocks ahead; two workgroups share a CU, and one's stores run behind the other's products. With 128
+// rows two stages of 16 KiB, so that four workgroups share a CU (50001 x 832 x 320: 44 us with three stages, 42 with two).
+// A half block of padding alone, and a wave whose rows or columns do not exist, take no products (42 -> 37 us).
+//
+// An LDS row is 64 bytes of one operand row; its 16-byte pieces are permuted by (row >> 2) & 3 on the way in, so that the 16
 // lanes that read one piece of 16 rows hit distinct banks. The sums do not care in which order k is taken as long as both
 // operands agree, so a lane's 16 contiguous bytes serve two instructions of 8.
 #include "fp8.h"
@@ -35,6 +38,7 @@ struct GemmArgs {
     int64_t m, n;
     int sha, shb;                // scales per row (0) or per 128 rows (7)
     int steps, steps_per_split;  // blocks of k, and of one split
+    int halves;                  // half blocks with k in them
     int tiles_m, tiles_n;
     const float* bias;
     int act;
@@ -154,7 +158,10 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
     constexpr int TM = RT * 64;                 // rows of the workgroup's tile: 2 waves of RT x 32
     constexpr int STAGE = (TM + TN) * HK;       // bytes of one half block
     constexpr int LOADS = (TM + TN) / 16 / 4;   // 1 KiB pieces of it a wave loads
-    __shared__ __align__(16) uint8_t lds[3 * STAGE];
+    constexpr int STAGES = RT == 2 ? 2 : 3;
+    constexpr int ES = 36;                      // floats of an LDS row of the epilogue
+    constexpr int STRIP = RT * 32 * ES;         // floats of a wave's
+    __shared__ __align__(16) uint8_t lds[STAGES * STAGE > STRIP * 16 ? STAGES * STAGE : STRIP * 16];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave & 1, wn = wave >> 1;
 
@@ -173,7 +180,8 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
     const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
     const int first = split * g.steps_per_split;
     const int last = first + g.steps_per_split < g.steps ? first + g.steps_per_split : g.steps;
-    const int halves = 2 * (last - first);
+    const int halves = (2 * last < g.halves ? 2 * last : g.halves) - 2 * first;
+    const bool idle = m0 + wm * RT * 32 >= g.m || n0 + wn * 64 >= g.n;
 
     // This wave's 1 KiB pieces of a stage: 16 rows of A or of B each, lane / 4 the row, lane % 4 the place in LDS. Rows
     // past the operand's end read its last row; their products are not stored.
@@ -214,7 +222,7 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
     f32x16 acc[RT][2] = {};
     uint64_t wa[RT], wb[2];
     load(0, 0);
-    load(1, 1);
+    if (STAGES == 3) load(1, 1);
     int stage = 0;
     for (int half = 0; half < halves; ++half) {
         const int block = first + (half >> 1);
@@ -230,16 +238,16 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
             // the loop's body would be for all of those, every half block
             __builtin_amdgcn_s_waitcnt(0x0F70);
         }
-        // Everything but the newest stage's loads is in: they return in order, and this stage's were issued before those.
-        // At the last stage there are no newer ones. This wave's own reads of the stage before are done too.
-        if (half + 1 < halves)
+        // This stage's loads are in. With three stages the next one's, issued later, may be under way: loads return in order,
+        // and at the last stage there are no newer ones. This wave's own reads of the stage before are done too.
+        if (STAGES == 3 && half + 1 < halves)
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
         else
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         // every wave's are in, and every wave has read the stage before this one, which the next loads overwrite
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (half + 2 < halves) load(stage == 0 ? 2 : stage - 1, half + 2);
+        if (half + STAGES - 1 < halves) load(stage == 0 ? STAGES - 1 : stage - 1, half + STAGES - 1);
         const int shift = 8 * (block & 7);
         uint32_t ba[RT], bb[2];
 #pragma unroll
@@ -248,17 +256,15 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
         for (int j = 0; j < 2; ++j) bb[j] = (uint32_t)(wb[j] >> shift) & 0xFFu;
         const uint8_t* la = lds + stage * STAGE + wm * RT * 32 * HK;
         const uint8_t* lb = lds + stage * STAGE + (TM + wn * 64) * HK;
-        half_block<E5M2A, RT>(la, lb, lane, ba, bb, acc);
-        stage = stage == 2 ? 0 : stage + 1;
+        if (!idle) half_block<E5M2A, RT>(la, lb, lane, ba, bb, acc);
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
 
     // B rows are the instruction's rows: registers 4 k .. 4 k + 3 of a 32 x 32 tile are out[lane % 32][8 k + 4 (lane / 32) ..].
     // They pass through LDS (the wave's quarter of the stages, which no one reads any more), 32 columns at a time, so that
     // 8 lanes store 128 bytes of one row: stored as they lie, 32 bytes a row, they cost HBM twice the requests. The loop
     // over the rows also keeps the epilogue short; unrolled over the accumulators it outgrew the instruction cache.
-    constexpr int ES = 36;  // floats of an LDS row
-    static_assert(RT * 32 * ES * 4 * 4 <= 3 * STAGE, "the epilogue's rows fit the stages");
-    float* strip = (float*)lds + wave * (RT * 32 * ES);
+    float* strip = (float*)lds + wave * STRIP;
     __syncthreads();
     const int64_t wave_m = m0 + wm * RT * 32;
     const int sub = lane >> 3, quad = (lane & 7) * 4;
@@ -462,12 +468,12 @@ void launch_join(hipStream_t stream, const GemmArgs& g, const void* part, int sp
         hipLaunchKernelGGL((join_kernel<T, 1>), grid, dim3(256), 0, stream, g, (const float*)part, splits);
 }
 
-// Tiles of 256 rows need a third less of the operands' bytes; those of 128 leave less of a tile outside the result, and three
+// Tiles of 256 rows need a third less of the operands' bytes; those of 128 leave less of a tile outside the result, and four
 // workgroups of them share a CU, which hides a short sum's beginning and end.
 int64_t tiles_of(int64_t m, int64_t n, int rows) { return (m + rows - 1) / rows * ((n + TN - 1) / TN); }
 bool less_waste(int64_t m) { return 10 * ((m + 255) / 256 * 256) > 11 * ((m + 127) / 128 * 128); }  // by 128 rows, over 10 %
 
-// 262144 x 1024 x 1024: 590 us with 256 rows, 607 with 128; 16384 x 4096 x 4096: 453 and 491; 50001 x 832 x 320: 48 and 43
+// 262144 x 1024 x 1024: 590 us with 256 rows, 607 with 128; 16384 x 4096 x 4096: 453 and 491; 50001 x 832 x 320: 48 and 37
 bool tall(int64_t m, int64_t n, int64_t k) { return k >= 1024 && tiles_of(m, n, 256) >= 512 && !less_waste(m); }
 
 // A product whose tiles do not fill the card splits its k axis: 1024 x 1024 over 262144 takes 458 us with 256 rows a tile, 525
@@ -556,6 +562,7 @@ void launch_fp8_product(hipStream_t stream, const Fp8Product& p) {
     g.sha = p.a.shift;
     g.shb = p.b.shift;
     g.steps = (int)fp8_blocks(p.k);
+    g.halves = (int)((p.k + HK - 1) / HK);
     g.bias = p.bias;
     g.act = p.act;
     g.omega = p.omega;

@@ -54,12 +54,18 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t w0, uint32_t w1, float scale) 
     return bf16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 }
 
-// src[0 .. 3] as fp32, of which valid exist (the rest zero). vec: src is aligned for one access
+// four elements that lie as they may: one access at the element's own alignment (the card splits what crosses a line), so
+// that odd widths and views read and write as wide as others
 template <typename T>
-__device__ __forceinline__ void load_quad(const T* src, int valid, bool vec, float (&v)[4]) {
-    if (vec && valid >= 4) {
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        const T4 h = *(const T4*)src;
+struct Quad {
+    typedef T Type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
+
+// src[0 .. 3] as fp32, of which valid exist (the rest zero)
+template <typename T>
+__device__ __forceinline__ void load_quad(const T* src, int valid, float (&v)[4]) {
+    if (valid >= 4) {
+        const typename Quad<T>::Type h = *(const typename Quad<T>::Type*)src;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = (float)h[k];
     } else {

@@ -310,7 +310,6 @@ struct FewArgs {
     const void* x;
     int64_t ld, m, k;
     const uint8_t *w, *sw;
-    int vec;
     GemmArgs out;  // n, bias, act, omega, out
 };
 template <typename T, int MT, int NT>
@@ -356,7 +355,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs f) {
             for (int i = 0; i < BATCH; ++i) {
                 const int u = u0 + 8 * i, row = u / here, b = u - row * here;
                 const int64_t c0 = (int64_t)(b0 + b) * 128 + c4 * 4, left = f.k - c0;
-                load_quad((const T*)f.x + row * f.ld + c0, u < all && left > 0 ? (left < 4 ? (int)left : 4) : 0, f.vec != 0, v[i]);
+                load_quad((const T*)f.x + row * f.ld + c0, u < all && left > 0 ? (left < 4 ? (int)left : 4) : 0, v[i]);
             }
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
@@ -513,7 +512,6 @@ void launch_fp8_few_rows(hipStream_t stream, const void* x, int type, int64_t ld
     f.k = k;
     f.w = w;
     f.sw = sw;
-    f.vec = (uintptr_t)x % (type == FP8_F32 ? 16 : 8) == 0 && (ld % 4 == 0 || m == 1);
     f.out.m = m;
     f.out.n = n;
     f.out.bias = bias;

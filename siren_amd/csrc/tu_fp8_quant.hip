@@ -20,11 +20,11 @@ constexpr int QT = 128;           // tile edge
 constexpr int QSTRIDE = QT + 16;  // LDS row of the transposed bytes: 16-byte pieces on distinct banks
 
 template <typename T, bool E5M2, bool MULT>
-__global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+__global__ __launch_bounds__(256, 4) void quant_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
                                                     const __bf16* __restrict__ mult, uint8_t* __restrict__ q,
                                                     uint8_t* __restrict__ s, uint8_t* __restrict__ qt,
                                                     uint8_t* __restrict__ st, float* __restrict__ colsum, int tiles,
-                                                    int vec, int col_blocks, int panels) {
+                                                    int near, int col_blocks, int panels) {
     __shared__ __align__(16) uint8_t tr[QT * QSTRIDE];
     __shared__ float part[8][QT];
     __shared__ float wmax[4];
@@ -37,25 +37,25 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
     const int64_t s_ld = (col_blocks + 3) / 4 * 4, st_ld = (row_blocks + 3) / 4 * 4;
 
     // Every load is issued before any is waited for (a branch around each row's load made 16 round trips of them: 8 us for
-    // one row). A tile on the edge reads the last row or column again and zeroes what does not exist.
+    // one row), by the wave's uniform address and a 32-bit offset of the lane (64-bit addresses of 16 rows cost the fourth
+    // wave of a SIMD). A tile on the edge reads the last row again, and columns up to the last, and zeroes what does not exist.
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int64_t wr = rb * QT + wave * 32;  // the wave's first row
     f32x4 v[16];
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    typedef __bf16 B4 __attribute__((ext_vector_type(4)));
-    if (vec && (rb + 1) * QT <= rows && (int64_t)(cb + 1) * QT <= cols) {
+    typedef typename Quad<T>::Type T4;
+    typedef typename Quad<__bf16>::Type B4;
+    if (near && (rb + 1) * QT <= rows && (int64_t)(cb + 1) * QT <= cols) {
+        const uint32_t row = (rg & 1) * 16, at = (row * (uint32_t)ld + c4 * 4) * (uint32_t)sizeof(T);
+        const T* src = x + wr * ld + (int64_t)cb * QT;
         T4 h[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) h[i] = *(const T4*)(x + (r0 + i) * ld + c0);
+        for (int i = 0; i < 16; ++i) h[i] = *(const T4*)((const char*)(src + i * ld) + at);
         if constexpr (MULT) {
-            const bool wide = (cols & 3) == 0;
+            const uint32_t mat = (row * (uint32_t)cols + c4 * 4) * 2u;
+            const __bf16* msrc = mult + wr * cols + (int64_t)cb * QT;
             B4 f[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const __bf16* src = mult + (r0 + i) * cols + c0;
-                if (wide)
-                    f[i] = *(const B4*)src;
-                else
-                    f[i] = B4{src[0], src[1], src[2], src[3]};
-            }
+            for (int i = 0; i < 16; ++i) f[i] = *(const B4*)((const char*)(msrc + i * cols) + mat);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
 #pragma unroll
@@ -66,39 +66,63 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[i][k] = (float)h[i][k];
         }
-    } else if (vec && (cols & 3) == 0) {
-        const bool in = c0 < cols;  // a quad is inside or outside
-        const int64_t c = in ? c0 : 0;
+    } else if (wr >= rows) {  // nothing of this wave's rows exists
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    } else if (near && cols >= 4) {
+        // the quad that crosses the end is read up to the end and shifted
+        const int64_t cs = c0 < cols - 4 ? c0 : cols - 4;
+        const int shift = c0 - cs < 4 ? (int)(c0 - cs) : 4, left = (int)(rows - 1 - wr < 31 ? rows - 1 - wr : 31);
+        const T* src = x + wr * ld + (int64_t)cb * QT;
+        const __bf16* msrc = mult + wr * cols + (int64_t)cb * QT;
+        const int c = (int)(cs - (int64_t)cb * QT);  // may be negative: the address below is taken in 64 bits then
         T4 h[16];
         B4 f[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int64_t r = r0 + i < rows ? r0 + i : rows - 1;
-            h[i] = *(const T4*)(x + r * ld + c);
-            if constexpr (MULT) f[i] = *(const B4*)(mult + r * cols + c);
+            const int r = (rg & 1) * 16 + i < left ? (rg & 1) * 16 + i : left;
+            h[i] = *(const T4*)((const char*)(src + c) + (uint32_t)r * (uint32_t)ld * (uint32_t)sizeof(T));
+            if constexpr (MULT) f[i] = *(const B4*)((const char*)(msrc + c) + (uint32_t)r * (uint32_t)cols * 2u);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 16; ++i) {
+            float p[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                v[i][k] = in && r0 + i < rows ? (float)h[i][k] : 0.f;
-                if constexpr (MULT) v[i][k] *= in && r0 + i < rows ? (float)f[i][k] : 0.f;
+                p[k] = (float)h[i][k];
+                if constexpr (MULT) p[k] *= (float)f[i][k];
             }
+            const bool in = r0 + i < rows;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i][k] = in ? p[k] : 0.f;
+        }
+        if ((int64_t)(cb + 1) * QT > cols) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const f32x4 p = v[i];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float u = shift == 0 ? p[k] : 0.f;
+#pragma unroll
+                    for (int d = 1; d < 4 - k; ++d) u = shift == d ? p[k + d] : u;
+                    v[i][k] = u;
+                }
+            }
+        }
     } else {
-        T h[16][4];
+        // fewer than 4 columns, or rows 2^25 elements apart: four rows at a time
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int b = 0; b < 4; ++b) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                h[i][k] = x[(r0 + i < rows ? r0 + i : rows - 1) * ld + (c0 + k < cols ? c0 + k : cols - 1)];
+            for (int i = 4 * b; i < 4 * b + 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool in = r0 + i < rows && c0 + k < cols;
-                v[i][k] = in ? (float)h[i][k] : 0.f;
-                if (MULT && in) v[i][k] *= (float)mult[(r0 + i) * cols + c0 + k];
-            }
+                for (int k = 0; k < 4; ++k) {
+                    const bool in = r0 + i < rows && c0 + k < cols;
+                    v[i][k] = in ? (float)x[(r0 + i) * ld + c0 + k] : 0.f;
+                    if (MULT && in) v[i][k] *= (float)mult[(r0 + i) * cols + c0 + k];
+                }
+            asm volatile("" ::: "memory");
+        }
     }
 
     if (colsum != nullptr) {  // 16 rows a thread, then the 8 row groups in order
@@ -214,9 +238,9 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // 4 lanes a column of each panel: a wave's 16 columns lie behind each other
                 const int c = (j & 1) * 64 + (t >> 2), piece = (j >> 1) * 4 + (t & 3);
-                if ((int64_t)cb * QT + c < cols)
-                    *(u32x4*)(qt + ((rb * 2 + (j >> 1)) * cols + (int64_t)cb * QT + c) * 64 + (t & 3) * 16) =
-                        *(const u32x4*)(tr + c * QSTRIDE + piece * 16);
+                if ((int64_t)cb * QT + c < cols)  // nontemporal: 262144 x 1024 fp32 313 -> 301 us
+                    __builtin_nontemporal_store(*(const u32x4*)(tr + c * QSTRIDE + piece * 16),
+                                                (u32x4*)(qt + ((rb * 2 + (j >> 1)) * cols + (int64_t)cb * QT + c) * 64 + (t & 3) * 16));
             }
         } else {
 #pragma unroll
@@ -236,7 +260,7 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 constexpr int ROWS_PER_GROUP = 32;
 template <typename T, bool E5M2>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
-                                                         uint8_t* __restrict__ q, uint8_t* __restrict__ s, int vec,
+                                                         uint8_t* __restrict__ q, uint8_t* __restrict__ s,
                                                          int col_blocks, int panels) {
     const int c4 = threadIdx.x & 31, unit = threadIdx.x >> 5;
     const int64_t rb = blockIdx.x / col_blocks;
@@ -249,7 +273,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t r = rb * ROWS_PER_GROUP + i * 8 + unit;
-        load_quad(x + (r < rows ? r : rows - 1) * ld + c0, valid, vec != 0, v[i]);
+        load_quad(x + (r < rows ? r : rows - 1) * ld + c0, valid, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -290,13 +314,12 @@ __global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ 
 
 void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
     const int64_t col_blocks = fp8_blocks(a.cols), grid = fp8_blocks(a.rows) * col_blocks;
-    const int64_t size = a.type == FP8_F32 ? 4 : 2;
-    const int vec = ((uintptr_t)a.x % (4 * size)) == 0 && (a.ld % 4 == 0 || a.rows == 1);
+    const int near = a.rows == 1 || a.ld < 1 << 25;  // 31 rows are less than 2^32 bytes apart
     if (a.qt == nullptr && a.colsum == nullptr && a.mult == nullptr && !a.tiles) {
         const int64_t groups = (a.rows + ROWS_PER_GROUP - 1) / ROWS_PER_GROUP * col_blocks;
 #define SIREN_QUANT_ROWS(T, E)                                                                                           \
     hipLaunchKernelGGL((quant_rows_kernel<T, E>), dim3((unsigned)groups), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
-                       a.cols, a.q, a.s, vec, (int)col_blocks, a.panels)
+                       a.cols, a.q, a.s, (int)col_blocks, a.panels)
         if (a.type == FP8_F32 && a.e5m2) SIREN_QUANT_ROWS(float, true);
         if (a.type == FP8_BF16 && a.e5m2) SIREN_QUANT_ROWS(__bf16, true);
         if (a.type == FP8_F16 && a.e5m2) SIREN_QUANT_ROWS(_Float16, true);
@@ -308,7 +331,7 @@ void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
     }
 #define SIREN_QUANT(T, E, M)                                                                                            \
     hipLaunchKernelGGL((quant_kernel<T, E, M>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, a.cols, \
-                       (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, vec, (int)col_blocks, a.panels)
+                       (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, near, (int)col_blocks, a.panels)
 #define SIREN_QUANT_TYPES(E, M)                     \
     do {                                            \
         if (a.type == FP8_F32) SIREN_QUANT(float, E, M);     \

@@ -59,19 +59,14 @@ __device__ __forceinline__ int find_tensor(const AdamwTable& t, uint32_t c) {
     return lo;
 }
 
-// four consecutive elements of src at i; those at or past n are zero. vec: src is aligned for one wide access
+// four consecutive elements of src at i, however they are aligned; those at or past n are zero
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* src, int64_t i, int64_t n, bool vec) {
+__device__ __forceinline__ f32x4 load4(const T* src, int64_t i, int64_t n) {
     f32x4 r = {0.f, 0.f, 0.f, 0.f};
-    if (vec && i + 4 <= n) {
-        if constexpr (sizeof(T) == 4) {
-            r = *(const f32x4*)(src + i);
-        } else {
-            typedef T T4 __attribute__((ext_vector_type(4)));
-            const T4 v = *(const T4*)(src + i);
+    if (i + 4 <= n) {
+        const typename Quad<T>::Type v = *(const typename Quad<T>::Type*)(src + i);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) r[k] = (float)v[k];
-        }
+        for (int k = 0; k < 4; ++k) r[k] = (float)v[k];
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -80,17 +75,9 @@ __device__ __forceinline__ f32x4 load4(const T* src, int64_t i, int64_t n, bool 
     return r;
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* dst, int64_t i, int64_t n, bool vec, f32x4 v) {
-    if (vec && i + 4 <= n) {
-        if constexpr (sizeof(T) == 4) {
-            *(f32x4*)(dst + i) = v;
-        } else {
-            typedef T T4 __attribute__((ext_vector_type(4)));
-            T4 o;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = (T)v[k];
-            *(T4*)(dst + i) = o;
-        }
+__device__ __forceinline__ void store4(T* dst, int64_t i, int64_t n, f32x4 v) {
+    if (i + 4 <= n) {
+        *(typename Quad<T>::Type*)(dst + i) = typename Quad<T>::Type{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -128,9 +115,7 @@ __global__ __launch_bounds__(NORM_THREADS) void adamw_norm_kernel(AdamwTable tab
             v[u] = f32x4{0.f, 0.f, 0.f, 0.f};
             if (c < tab.chunks) {
                 const int k = find_tensor(tab, c);
-                const T* g = (const T*)tab.g[k];
-                v[u] = load4(g, (int64_t)(c - tab.first[k]) * CHUNK + threadIdx.x * 4, tab.n[k],
-                             ((uintptr_t)g & (4 * sizeof(T) - 1)) == 0);
+                v[u] = load4((const T*)tab.g[k], (int64_t)(c - tab.first[k]) * CHUNK + threadIdx.x * 4, tab.n[k]);
             }
         }
 #pragma unroll
@@ -196,15 +181,14 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwTable tab, float* __r
         T* p = (T*)tab.p[k];
         const T* g = (const T*)tab.g[k];
         const int64_t n = tab.n[k], off = (int64_t)tab.block[k] * 128;
-        const bool vec = (((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) == 0;
         const int64_t base = (int64_t)(ch - tab.first[k]) * CHUNK + threadIdx.x * 4;
         f32x4 pv[2], gv[2], mv[2], vv[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int64_t i = base + q * (CHUNK / 2);
             if (i >= n) continue;
-            pv[q] = load4(p, i, n, vec);
-            gv[q] = load4(g, i, n, vec);
+            pv[q] = load4(p, i, n);
+            gv[q] = load4(g, i, n);
             mv[q] = *(const f32x4*)(em + off + i);  // the pad behind a tensor's end may be read, never written
             vv[q] = *(const f32x4*)(ev + off + i);
         }
@@ -221,9 +205,9 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwTable tab, float* __r
                 vv[q][e] = v;
                 pv[q][e] = apply(pv[q][e], m, __builtin_sqrtf(v), h.decay, step_size, inv_root, h.epsf);
             }
-            store4(p, i, n, vec, pv[q]);
-            store4(em + off, i, n, true, mv[q]);
-            store4(ev + off, i, n, true, vv[q]);
+            store4(p, i, n, pv[q]);
+            store4(em + off, i, n, mv[q]);
+            store4(ev + off, i, n, vv[q]);
         }
     }
 }
@@ -253,19 +237,27 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamwTable tab, uint8_t* __
         T* p = (T*)tab.p[k];
         const T* g = (const T*)tab.g[k];
         const int64_t n = tab.n[k], off = (int64_t)tab.block[k] * 128;
-        const bool vec = (((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) == 0;
         // 16 lanes hold one block of 128; a block that begins past the tensor's end does not exist
         const int64_t i = (int64_t)(ch - tab.first[k]) * CHUNK + threadIdx.x * 8;
         if ((i & ~(int64_t)127) >= n) continue;
         const int64_t blk = (off + i) >> 7;
-        f32x4 pv[2], gv[2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            pv[q] = load4(p, i + 4 * q, n, vec);
-            gv[q] = load4(g, i + 4 * q, n, vec);
-        }
         const u32x2 mc = *(const u32x2*)(em + off + i), uc = *(const u32x2*)(eu + off + i);
-        const float ms = scale_of(sm[blk]), us = scale_of(su[blk]);
+        const uint8_t msb = sm[blk], usb = su[blk];
+        f32x4 pv[2], gv[2];
+        if (i + 8 <= n) {  // one branch for all four quads
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                pv[q] = load4(p, i + 4 * q, i + 8);
+                gv[q] = load4(g, i + 4 * q, i + 8);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                pv[q] = load4(p, i + 4 * q, n);
+                gv[q] = load4(g, i + 4 * q, n);
+            }
+        }
+        const float ms = scale_of(msb), us = scale_of(usb);
         float m[8], u[8];
         float mmax = 0.f, umax = 0.f;
         bool mok = true, uok = true;
@@ -313,7 +305,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamwTable tab, uint8_t* __
             }
         }
 #pragma unroll
-        for (int q = 0; q < 2; ++q) store4(p, i + 4 * q, n, vec, pv[q]);
+        for (int q = 0; q < 2; ++q) store4(p, i + 4 * q, n, pv[q]);
         *(u32x2*)(em + off + i) = mo;
         *(u32x2*)(eu + off + i) = uo;
         if ((threadIdx.x & 15) == 0) {

@@ -394,3 +394,25 @@ def test_inference_parameters_are_refused_unchanged(cuda):
     with pytest.raises(RuntimeError, match='nference'):
         optim.adamw_step([p], [g], opt.exp_avg, opt.exp_avg_sq, opt.steps)
     assert bool((p == 1).all()) and int(opt.steps) == 0
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_tensors_at_any_address(cuda, bits, dtype):
+    """Parameters and gradients that begin one to three elements into their storage give the same bytes as aligned ones."""
+    from siren_amd import optim
+    sizes, out = [700, 4099, 130, 5, 3, 1], []
+    values, slopes = make(sizes, dtype, 3, 0.05), make(sizes, dtype, 4, 0.1)
+    for shift in range(4):
+        def place(ts):
+            held = [torch.empty(t.numel() + 8, dtype=dtype, device=cuda).fill_(7.) for t in ts]
+            for h, t in zip(held, ts):
+                h[shift:shift + t.numel()] = t.to(cuda)
+            return held, [h[shift:shift + t.numel()] for h, t in zip(held, ts)]
+        (hp, ps), (_, gs) = place(values), place(slopes)
+        opt = optim.FusedAdamW(ps, max_norm=0.5, state_bits=bits)
+        optim.adamw_step(ps, gs, opt.exp_avg, opt.exp_avg_sq, opt.steps, max_norm=0.5, scales=opt.scales)
+        for h, p in zip(hp, ps):
+            assert bool((h[:shift] == 7).all()) and bool((h[shift + p.numel():] == 7).all())
+        out.append(torch.cat([p.float() for p in ps] + [opt.exp_avg.float(), opt.exp_avg_sq.float()]))
+    assert all(torch.equal(o, out[0]) for o in out)

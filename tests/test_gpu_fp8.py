@@ -501,3 +501,27 @@ def test_graph_is_used_as_any_other(cuda, m, act):
     assert all(torch.equal(p, g) for p, g in zip(torch.autograd.grad(y, (x, w, b), dy), want))
     y = checkpoint(lambda *a: fp8.linear(*a, act), x, w, b, use_reentrant=False)
     assert all(torch.equal(p, g) for p, g in zip(torch.autograd.grad(y, (x, w, b), dy), want))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,cols,ld', [(200, 3, 3), (131, 6, 7), (129, 131, 131), (40, 66, 1 << 25), (3, 2, (1 << 25) + 1)])
+def test_quantize_at_any_address(cuda, dtype, rows, cols, ld):
+    """Rows that begin anywhere, narrow ones, and ones too far apart for 32-bit offsets: both layouts, and what a sine layer's
+    backward multiplies and sums on the way, as of a plain copy."""
+    from siren_amd import fp8
+    if dtype is torch.float32 and ld > 1000:
+        rows = min(rows, 20)  # a few GB
+    base = torch.zeros((rows - 1) * ld + cols + 3, dtype=dtype, device=cuda)
+    for shift in range(3):
+        x = base[shift:].as_strided((rows, cols), (ld, 1))
+        x.copy_(torch.randn(rows, cols, device=cuda))
+        for block in ('row', 'tile'):
+            for a, b in zip(fp8.quantize(x, block, transposed=True), fp8.quantize(x.clone(), block, transposed=True)):
+                assert torch.equal(a.data.view(torch.uint8), b.data.view(torch.uint8)) and torch.equal(a.scale, b.scale)
+            want = held(np64(x), tiles=block == 'tile')[0]
+            assert np.array_equal(np64(fp8.dequantize(fp8.quantize(x, block))), want)
+        w = torch.randn(cols, 9, device=cuda, requires_grad=True)
+        b = torch.randn(cols, device=cuda, requires_grad=True)
+        h = torch.randn(rows, 9, device=cuda).to(dtype).requires_grad_(True)
+        grads = [torch.autograd.grad(fp8.linear(h, w, b, 'sine'), (h, w, b), dy) for dy in (x, x.clone())]
+        assert all(torch.equal(p, q) for p, q in zip(*grads))

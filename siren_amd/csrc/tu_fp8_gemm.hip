@@ -17,6 +17,9 @@
 // An LDS row is 64 bytes of one operand row; its 16-byte pieces are permuted by (row >> 2) & 3 on the way in, so that the 16
 // lanes that read one piece of 16 rows hit distinct banks. The sums do not care in which order k is taken as long as both
 // operands agree, so a lane's 16 contiguous bytes serve two instructions of 8.
+#include <algorithm>
+#include <cmath>
+
 #include "fp8.h"
 #include "fp8_device.h"
 #include "siren_common.h"
@@ -480,17 +483,38 @@ bool less_waste(int64_t m) { return 10 * ((m + 255) / 256 * 256) > 11 * ((m + 12
 // 262144 x 1024 x 1024: 590 us with 256 rows, 607 with 128; 16384 x 4096 x 4096: 453 and 491; 50001 x 832 x 320: 48 and 37
 bool tall(int64_t m, int64_t n, int64_t k) { return k >= 1024 && tiles_of(m, n, 256) >= 512 && !less_waste(m); }
 
-// A product whose tiles do not fill the card splits its k axis: 1024 x 1024 over 262144 takes 458 us with 256 rows a tile, 525
-// with 128
-bool split_tall(int64_t m) { return m > 128 && !less_waste(m); }
-// enough workgroups to fill 256 CUs twice, at least 4 blocks each
-int splits_of(int64_t m, int64_t n, int64_t k) {
-    const int64_t tiles = tiles_of(m, n, split_tall(m) ? 256 : 128), steps = fp8_blocks(k);
-    if (tiles >= 256 || steps < 8) return 1;
-    int64_t s = (512 + tiles - 1) / tiles;
-    if (s > steps / 4) s = steps / 4;
-    const int64_t per = (steps + s - 1) / s;
-    return (int)((steps + per - 1) / per);
+// A product whose tiles do not fill the card splits its k axis, where that pays for the partial results' way through memory
+// and a second launch. By what was measured, in us: a block of k takes a workgroup of 128 rows 1.1, and 0.84 for each of those
+// that share its CU; the join 5, and each split's m n floats 1.6e-6 m n written and read. Two workgroups a CU at most (more
+// gained nothing). Split and whole: 200 x 200 x 1024 11 and 13, x 2048 12 and 22; 33 x 200 x 700 10.7 and 9.7, 2000 x 1000 x
+// 1024 24 and 14, x 2048 33 and 22. 1000 x 1000 x 4000 in 4, 16 and 1: 25, 32 and 29 us.
+struct Plan {
+    int splits;
+    bool tall;  // 256 rows a tile: sums of 64 blocks a workgroup and more (1024 x 1024 x 262144: 458 us and 525)
+};
+Plan plan_of(int64_t m, int64_t n, int64_t k) {
+    const int64_t tiles = tiles_of(m, n, 128), tall_tiles = tiles_of(m, n, 256), steps = fp8_blocks(k);
+    if (tiles >= 256 || steps < 4) return {1, tall(m, n, k)};
+    int64_t splits = 1;
+    bool rows256 = false;
+    if (m > 128 && !less_waste(m) && steps * tall_tiles >= 64 * 512) {
+        splits = 512 / tall_tiles;
+        rows256 = true;
+    } else {
+        const double plane = 1.6e-6 * (double)m * (double)n;
+        auto cost = [&](int64_t s) {
+            const double shared = 0.84 * (double)((tiles * s + 255) / 256);
+            return (double)((steps + s - 1) / s) * (shared > 1.1 ? shared : 1.1) + (s > 1 ? 5.0 + (double)s * plane : 0.0);
+        };
+        // the best number if a CU never had two, the largest that keeps it so, and 1
+        int64_t best = (int64_t)std::sqrt(1.1 * (double)steps / plane);
+        for (int64_t s : {std::min(best, 512 / tiles), std::min(best, 256 / tiles)}) {
+            s = std::min(s, steps / 2);
+            if (s > 1 && cost(s) < cost(splits)) splits = s;
+        }
+    }
+    const int64_t per = (steps + splits - 1) / splits;
+    return {(int)((steps + per - 1) / per), rows256};
 }
 
 template <typename T, bool E5M2A, bool SPLIT>
@@ -545,7 +569,7 @@ void launch_fp8_few_rows(hipStream_t stream, const void* x, int type, int64_t ld
 }
 
 int64_t fp8_product_ws_bytes(int64_t m, int64_t n, int64_t k) {
-    const int s = splits_of(m, n, k);
+    const int s = plan_of(m, n, k).splits;
     return s > 1 ? (int64_t)s * m * n * 4 : 0;
 }
 
@@ -570,29 +594,29 @@ void launch_fp8_product(hipStream_t stream, const Fp8Product& p) {
     g.act = p.act;
     g.omega = p.omega;
     g.deriv = (__bf16*)p.deriv;
-    const int splits = splits_of(g.m, g.n, p.k);
+    const Plan plan = plan_of(g.m, g.n, p.k);
+    const int splits = plan.splits;
     g.steps_per_split = (g.steps + splits - 1) / splits;
     g.out = splits > 1 ? p.ws : p.out;
     if (splits > 1) {
         if (p.e5m2_a)
-            launch_gemm<float, true, true>(stream, g, splits, split_tall(g.m));
+            launch_gemm<float, true, true>(stream, g, splits, plan.tall);
         else
-            launch_gemm<float, false, true>(stream, g, splits, split_tall(g.m));
+            launch_gemm<float, false, true>(stream, g, splits, plan.tall);
         g.out = p.out;
         if (p.type == FP8_F32) launch_join<float>(stream, g, p.ws, splits);
         if (p.type == FP8_BF16) launch_join<__bf16>(stream, g, p.ws, splits);
         if (p.type == FP8_F16) launch_join<_Float16>(stream, g, p.ws, splits);
         return;
     }
-    const bool rows256 = tall(g.m, g.n, p.k);
     if (p.e5m2_a) {
-        if (p.type == FP8_F32) launch_gemm<float, true, false>(stream, g, 1, rows256);
-        if (p.type == FP8_BF16) launch_gemm<__bf16, true, false>(stream, g, 1, rows256);
-        if (p.type == FP8_F16) launch_gemm<_Float16, true, false>(stream, g, 1, rows256);
+        if (p.type == FP8_F32) launch_gemm<float, true, false>(stream, g, 1, plan.tall);
+        if (p.type == FP8_BF16) launch_gemm<__bf16, true, false>(stream, g, 1, plan.tall);
+        if (p.type == FP8_F16) launch_gemm<_Float16, true, false>(stream, g, 1, plan.tall);
     } else {
-        if (p.type == FP8_F32) launch_gemm<float, false, false>(stream, g, 1, rows256);
-        if (p.type == FP8_BF16) launch_gemm<__bf16, false, false>(stream, g, 1, rows256);
-        if (p.type == FP8_F16) launch_gemm<_Float16, false, false>(stream, g, 1, rows256);
+        if (p.type == FP8_F32) launch_gemm<float, false, false>(stream, g, 1, plan.tall);
+        if (p.type == FP8_BF16) launch_gemm<__bf16, false, false>(stream, g, 1, plan.tall);
+        if (p.type == FP8_F16) launch_gemm<_Float16, false, false>(stream, g, 1, plan.tall);
     }
 }
 

@@ -525,3 +525,17 @@ def test_quantize_at_any_address(cuda, dtype, rows, cols, ld):
         h = torch.randn(rows, 9, device=cuda).to(dtype).requires_grad_(True)
         grads = [torch.autograd.grad(fp8.linear(h, w, b, 'sine'), (h, w, b), dy) for dy in (x, x.clone())]
         assert all(torch.equal(p, q) for p, q in zip(*grads))
+
+
+@pytest.mark.parametrize('m,n,k', [(33, 200, 700), (200, 200, 1024), (65, 64, 30000), (700, 700, 5000), (2000, 1000, 4096),
+                                   (833, 321, 50001), (1024, 1024, 131072), (1000, 1023, 140000)])
+def test_long_sums_are_exact(cuda, m, n, k):
+    """Small whole numbers, which e4m3 holds and whose sums 32 bits hold: every way of splitting the sum gives them exactly."""
+    from siren_amd import fp8
+    g = torch.Generator(device=cuda).manual_seed(k)
+    a = torch.randint(-3, 4, (m, k), generator=g, device=cuda)
+    b = torch.randint(-3, 4, (n, k), generator=g, device=cuda)
+    a[:, ::128], b[:, ::128] = 4, 4  # no block's scale is below 1/64: all values stay whole
+    out = fp8.matmul(fp8.quantize(a.float()), fp8.quantize(b.float()))
+    want = sum(a[:, c:c + 16384].double() @ b[:, c:c + 16384].double().t().contiguous() for c in range(0, k, 16384))
+    assert torch.equal(out.double(), want)

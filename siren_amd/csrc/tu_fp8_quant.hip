@@ -8,6 +8,8 @@
 // the product that sums over the rows): one workgroup holds a 128 x 128 tile in registers and writes both, with the
 // column sums of a bias's gradient on the way, so the tensor is read once. 64 values a thread: 16 rows x 4 columns, so
 // a row's maximum is a reduction over half a wave, a column's one over LDS, and the transpose leaves as 16-byte pieces.
+// Bytes bound it: 262144 x 1024 fp32 into both layouts 301 us (1.6 GB, 5.3 TB/s), bf16 214 us (5.0 TB/s; a bf16 value costs
+// the same instructions for half the bytes); rows alone 224 us from fp32 (6.0 TB/s).
 #include "fp8.h"
 #include "fp8_device.h"
 #include "siren_common.h"

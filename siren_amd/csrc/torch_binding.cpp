@@ -65,6 +65,7 @@ void check_input(const Tensor& x, const char* what) {
     TORCH_CHECK(x.is_cuda(), "siren_amd.fp8 runs on ROCm devices (MI355X) only; got a ", x.device().type(), " tensor as ", what);
     TORCH_CHECK_TYPE(type_code(x.scalar_type()) >= 0, what, " must be fp32, bf16 or fp16; got ", x.scalar_type());
     TORCH_CHECK_TYPE(x.layout() == at::kStrided, what, " must be a dense tensor");
+    TORCH_CHECK(!x._fw_grad(0).defined(), "siren_amd.fp8 has no forward-mode derivatives; ", what, " carries a tangent");
 }
 
 int64_t blocks(int64_t n) { return (n + 127) / 128; }

@@ -123,7 +123,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     synchronises with the host, and a captured step advances by itself on every replay (lr and the rest are captured).
 
     params, grads: lists of tensors, fp32, bf16 or fp16, each gradient of its parameter's type and shape; a gradient may
-    be None (the tensor and its state stay as they are). Parameters are contiguous and do not overlap.
+    be None (the tensor and its state stay as they are). Parameters are contiguous; they, the gradients and the states do
+    not overlap.
     exp_avg, exp_avg_sq: flat states, each tensor's padded to a multiple of 128: fp32, or with scales (two uint8 tensors,
     one byte per 128 elements) torch.float8_e4m3fn: exp_avg holds m, exp_avg_sq holds sqrt(v), value * 2^(byte - 127). The
     8-bit states are rounded up or down at random, from (seed, step, element): the same call gives the same result.

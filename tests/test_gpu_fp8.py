@@ -539,3 +539,17 @@ def test_long_sums_are_exact(cuda, m, n, k):
     out = fp8.matmul(fp8.quantize(a.float()), fp8.quantize(b.float()))
     want = sum(a[:, c:c + 16384].double() @ b[:, c:c + 16384].double().t().contiguous() for c in range(0, k, 16384))
     assert torch.equal(out.double(), want)
+
+
+def test_forward_mode_is_refused(cuda):
+    import torch.autograd.forward_ad as fwd
+    from siren_amd import fp8
+    x, w, b = torch.randn(5, 130, device=cuda), torch.randn(70, 130, device=cuda), torch.randn(70, device=cuda)
+    w8 = fp8.quantize(w, 'tile')
+    with fwd.dual_level():
+        for call in (lambda: fp8.linear(fwd.make_dual(x, x), w, b), lambda: fp8.linear(x, fwd.make_dual(w, w), b),
+                     lambda: fp8.linear(x, w, fwd.make_dual(b, b)), lambda: fp8.linear(fwd.make_dual(x, x), w8),
+                     lambda: fp8.quantize(fwd.make_dual(x, x))):
+            with pytest.raises(RuntimeError, match='tangent'):
+                call()
+        fp8.linear(x, w, b)

@@ -53,23 +53,24 @@ struct GemmArgs {
 // Nontemporal: a result is read by a later kernel, after the operands that it would push out of L2 (262144 x 1024 x 1024
 // fp32 out: 620 -> 550 us). Rows of odd widths begin within lines that two stores share, which L2 has to join: 30000 x 1023
 // fp32 takes 58 us through L2, 96 nontemporal, 71 element by element.
+// dst is global memory, which the compiler has to be told: a pointer out of a struct of arguments is generic to it, and a flat
+// store counts as an access of LDS too, so that the epilogue's waits for LDS waited for memory
+// (65536 x 256 x 256 bf16: 17.0 us, 13.8 with both this and the pacing of stores below).
 template <typename T>
 __device__ __forceinline__ void put4(T* dst, f32x4 v, int valid, bool vec) {
-    if (!vec && valid >= 4) {
-        *(typename Quad<T>::Type*)dst = typename Quad<T>::Type{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-        return;
-    }
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(1))) T Element;
+    typedef __attribute__((address_space(1))) T4 Line;
+    typedef __attribute__((address_space(1))) typename Quad<T>::Type Anywhere;
+    const T4 h = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
     if (vec && valid >= 4) {
-        if constexpr (sizeof(T) == 4) {
-            __builtin_nontemporal_store(v, (f32x4*)dst);
-        } else {
-            typedef T T4 __attribute__((ext_vector_type(4)));
-            __builtin_nontemporal_store((T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}), (T4*)dst);
-        }
+        __builtin_nontemporal_store(h, (Line*)dst);
+    } else if (valid >= 4) {
+        *(Anywhere*)dst = h;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (k < valid) dst[k] = (T)v[k];
+            if (k < valid) ((Element*)dst)[k] = h[k];
     }
 }
 
@@ -299,6 +300,9 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
         if (col < g.n) {
             const Finish<T> to(g, col);
             for (int row = sub; row < RT * 32; row += 32) {  // four rows' reads before the first is stored
+                // Eight of a wave's stores under way and no more: a burst of all 32 stands before the loads of the workgroup
+                // that shares the CU (262144 x 1024 x 1024 fp32 526 us, paced 510; 50001 x 832 x 320 bf16 37.5 and 35.4)
+                asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
                 f32x4 v[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) v[u] = *(const f32x4*)(strip + (row + 8 * u) * ES + quad);

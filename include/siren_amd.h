@@ -436,6 +436,18 @@ int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t c
                            int32_t format, int32_t tiles, int32_t panels, void* q, void* s, void* qt, void* st,
                            float* colsum_ws, float* colsum, void* stream);
 
+/* The same of one tensor or two (count 1 or 2) that do not depend on each other, in one launch where their types are alike. */
+typedef struct siren_fp8_source {
+    const void* x;
+    int32_t dtype, format;
+    int64_t rows, cols, ld;
+    const void* mult;
+    int32_t tiles, panels;
+    void *q, *s, *qt, *st;
+    float *colsum_ws, *colsum;
+} siren_fp8_source;
+int32_t siren_fp8_quantize_sources(const siren_fp8_source* src, int32_t count, void* stream);
+
 /* out (m, n) = act(a b^T + bias) of a (m, k) and b (n, k) quantised along k (k < 2^24, n < 2^22), sums in 32 bits.
  * a may be e4m3 or e5m2, b is e4m3. act 0: none, 1: sin(omega z), with deriv (m, n) bf16, nullable, = omega cos(omega z).
  * bias (n) fp32, nullable. ws: siren_fp8_matmul_ws_bytes(m, n, k) bytes. */

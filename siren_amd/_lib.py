@@ -100,6 +100,7 @@ _SIGS = {
     'siren_hvp_backward_batched_ws_floats': [_CFG, _I64, _I64, ctypes.POINTER(_I64)],
     'siren_hvp_backward_batched': [_CFG, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     'siren_fp8_quantize': [_P, _I32, _I64, _I64, _I64, _P, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P],
+    'siren_fp8_quantize_sources': [_P, _I32, _P],
     'siren_fp8_matmul_ws_bytes': [_I64, _I64, _I64, ctypes.POINTER(_I64)],
     'siren_fp8_matmul': [_P, _P, _I64, _I32, _I32, _P, _P, _I64, _I32, _I64, _P, _I32, ctypes.c_float, _P, _I32, _P, _P,
                          _P],
@@ -154,7 +155,7 @@ def native():
             raise ImportError('siren_amd: the torch binding is missing or was built for another torch (%s) - build it with '
                               '`python -c "import __graft_entry__ as g; g.build()"`' % e) from e
         mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in
-                  ('siren_last_error', 'siren_fp8_quantize', 'siren_fp8_matmul_ws_bytes', 'siren_fp8_matmul',
+                  ('siren_last_error', 'siren_fp8_quantize_sources', 'siren_fp8_matmul_ws_bytes', 'siren_fp8_matmul',
                    'siren_fp8_linear_ws_bytes', 'siren_fp8_linear', 'siren_adamw_scratch_bytes', 'siren_adamw_step')})
         _native = mod
     return _native

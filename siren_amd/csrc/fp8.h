@@ -27,6 +27,7 @@ struct Fp8Quant {
     int type, e5m2, tiles, panels;  // panels, as in Fp8Operand: 1 of q, 2 of qt
 };
 void launch_fp8_quant(hipStream_t st, const Fp8Quant& a);
+void launch_fp8_quant2(hipStream_t st, const Fp8Quant& a, const Fp8Quant& b);  // in one launch where their types are alike
 // out[c] = sum over the row blocks of colsum (blocks, cols), in order
 void launch_fp8_colsum(hipStream_t st, const float* colsum, int64_t blocks, int64_t cols, float* out);
 

@@ -1698,32 +1698,58 @@ int check_fp8_source(const void* x, int32_t dtype, int64_t rows, int64_t cols, i
 }
 }  // namespace
 
+// the checks of one tensor; *none: there is nothing to do for it
+static int check_fp8_quantize(const siren_fp8_source& a, bool* none) {
+    if (int rc = check_fp8_type(a.dtype)) return rc;
+    const int64_t rows = a.rows, cols = a.cols;
+    if (rows < 0 || cols < 0 || (a.format != 0 && a.format != 1) || (a.panels & ~3) != 0)
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: need rows, cols >= 0, format 0 (e4m3) or 1 (e5m2) and panels in 0..3");
+    // in the order of their sizes in threads: the column sums' launch, a tile a workgroup, 32 rows of a block a workgroup
+    if ((a.colsum != nullptr && siren::fp8_blocks(cols) > kMaxGrid / 16) ||
+        siren::fp8_blocks(cols) > kMaxGrid / std::max<int64_t>(1, siren::fp8_blocks(rows) * (a.qt == nullptr ? 4 : 1)))
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: too many tiles for one launch");
+    if ((a.q == nullptr) != (a.s == nullptr) || (a.qt == nullptr) != (a.st == nullptr))
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: values and scales go together");
+    if (a.colsum != nullptr && a.colsum_ws == nullptr && rows > 128)
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: colsum needs colsum_ws");
+    *none = rows == 0 || cols == 0;
+    if (*none) return SIREN_OK;
+    if (int rc = check_fp8_source(a.x, a.dtype, rows, cols, a.ld)) return rc;
+    if (a.q == nullptr && a.qt == nullptr && a.colsum == nullptr)
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: nothing to write");
+    if (!aligned(a.q, 16) || !aligned(a.qt, 16) || !aligned(a.s, 4) || !aligned(a.st, 4) || !aligned(a.mult, 16))
+        return fail(SIREN_EINVAL, "siren_fp8_quantize: q, qt and mult must be 16-byte aligned, scales 4-byte aligned");
+    return SIREN_OK;
+}
+
+int32_t siren_fp8_quantize_sources(const siren_fp8_source* src, int32_t count, void* stream) {
+    if (src == nullptr || (count != 1 && count != 2)) return fail(SIREN_EINVAL, "siren_fp8_quantize: need one source or two");
+    siren::Fp8Quant work[2];
+    int n = 0;
+    for (int i = 0; i < count; ++i) {
+        const siren_fp8_source& a = src[i];
+        bool none = false;
+        if (int rc = check_fp8_quantize(a, &none)) return rc;
+        if (none) continue;
+        // one row block's column sums are the sums
+        work[n++] = siren::Fp8Quant{a.x, a.ld, a.rows, a.cols, a.mult, (uint8_t*)a.q, (uint8_t*)a.s, (uint8_t*)a.qt,
+                                    (uint8_t*)a.st, a.colsum == nullptr || a.rows <= 128 ? a.colsum : a.colsum_ws, a.dtype,
+                                    a.format, a.tiles != 0, a.panels};
+    }
+    if (n == 1) siren::launch_fp8_quant((hipStream_t)stream, work[0]);
+    if (n == 2) siren::launch_fp8_quant2((hipStream_t)stream, work[0], work[1]);
+    for (int i = 0; i < count; ++i)
+        if (src[i].colsum != nullptr && src[i].rows > 128 && src[i].cols > 0)
+            siren::launch_fp8_colsum((hipStream_t)stream, src[i].colsum_ws, siren::fp8_blocks(src[i].rows), src[i].cols,
+                                     src[i].colsum);
+    return n == 0 ? SIREN_OK : hip_status("siren_fp8_quantize");
+}
+
 int32_t siren_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, const void* mult,
                            int32_t format, int32_t tiles, int32_t panels, void* q, void* s, void* qt, void* st,
                            float* colsum_ws, float* colsum, void* stream) {
-    if (int rc = check_fp8_type(dtype)) return rc;
-    if (rows < 0 || cols < 0 || (format != 0 && format != 1) || (panels & ~3) != 0)
-        return fail(SIREN_EINVAL, "siren_fp8_quantize: need rows, cols >= 0, format 0 (e4m3) or 1 (e5m2) and panels in 0..3");
-    // in the order of their sizes in threads: the column sums' launch, a tile a workgroup, 32 rows of a block a workgroup
-    if ((colsum != nullptr && siren::fp8_blocks(cols) > kMaxGrid / 16) ||
-        siren::fp8_blocks(cols) > kMaxGrid / std::max<int64_t>(1, siren::fp8_blocks(rows) * (qt == nullptr ? 4 : 1)))
-        return fail(SIREN_EINVAL, "siren_fp8_quantize: too many tiles for one launch");
-    if ((q == nullptr) != (s == nullptr) || (qt == nullptr) != (st == nullptr))
-        return fail(SIREN_EINVAL, "siren_fp8_quantize: values and scales go together");
-    if (colsum != nullptr && colsum_ws == nullptr && rows > 128) return fail(SIREN_EINVAL, "siren_fp8_quantize: colsum needs colsum_ws");
-    if (rows == 0 || cols == 0) return SIREN_OK;
-    if (int rc = check_fp8_source(x, dtype, rows, cols, ld)) return rc;
-    if (q == nullptr && qt == nullptr && colsum == nullptr) return fail(SIREN_EINVAL, "siren_fp8_quantize: nothing to write");
-    if (!aligned(q, 16) || !aligned(qt, 16) || !aligned(s, 4) || !aligned(st, 4) || !aligned(mult, 16))
-        return fail(SIREN_EINVAL, "siren_fp8_quantize: q, qt and mult must be 16-byte aligned, scales 4-byte aligned");
-    // one row block's column sums are the sums
-    const bool one = rows <= 128;
-    siren::Fp8Quant a{x, ld, rows, cols, mult, (uint8_t*)q, (uint8_t*)s, (uint8_t*)qt, (uint8_t*)st,
-                      colsum == nullptr || one ? colsum : colsum_ws, dtype, format, tiles != 0, panels};
-    siren::launch_fp8_quant((hipStream_t)stream, a);
-    if (colsum != nullptr && !one)
-        siren::launch_fp8_colsum((hipStream_t)stream, colsum_ws, siren::fp8_blocks(rows), cols, colsum);
-    return hip_status("siren_fp8_quantize");
+    const siren_fp8_source a = {x, dtype, format, rows, cols, ld, mult, tiles, panels, q, s, qt, st, colsum_ws, colsum};
+    return siren_fp8_quantize_sources(&a, 1, stream);
 }
 
 int32_t siren_fp8_matmul_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes) {

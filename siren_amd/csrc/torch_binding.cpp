@@ -25,7 +25,7 @@ typedef std::optional<Tensor> MaybeTensor;
 
 struct Library {
     decltype(&siren_last_error) last_error;
-    decltype(&siren_fp8_quantize) quantize;
+    decltype(&siren_fp8_quantize_sources) quantize;
     decltype(&siren_fp8_matmul_ws_bytes) matmul_ws_bytes;
     decltype(&siren_fp8_matmul) matmul;
     decltype(&siren_fp8_linear_ws_bytes) linear_ws_bytes;
@@ -37,7 +37,7 @@ struct Library {
 void bind(const std::map<std::string, uintptr_t>& f) {
 #define SIREN_BIND(field, name) lib.field = reinterpret_cast<decltype(lib.field)>(f.at(name))
     SIREN_BIND(last_error, "siren_last_error");
-    SIREN_BIND(quantize, "siren_fp8_quantize");
+    SIREN_BIND(quantize, "siren_fp8_quantize_sources");
     SIREN_BIND(matmul_ws_bytes, "siren_fp8_matmul_ws_bytes");
     SIREN_BIND(matmul, "siren_fp8_matmul");
     SIREN_BIND(linear_ws_bytes, "siren_fp8_linear_ws_bytes");
@@ -72,16 +72,40 @@ int64_t blocks(int64_t n) { return (n + 127) / 128; }
 int64_t padded(int64_t n) { return blocks(n) * 128; }
 int64_t words(int64_t n) { return (blocks(n) + 3) / 4 * 4; }
 
-// A quantised (rows, cols) tensor: values in rows (rows, padded cols) or in panels (padded cols / 64, rows, 64). What the
-// layer makes for itself is one allocation, values before scales (hold); what the user holds is two tensors.
+// A quantised (rows, cols) tensor in memory that someone holds: values in rows (rows, padded cols) or in panels (padded
+// cols / 64, rows, 64), and its scales
 struct Blocks {
-    Tensor hold, data, scale;
+    char *values = nullptr, *scales = nullptr;
     int64_t rows = 0, cols = 0;
     int layout = 0, fmt = 0;
-    char* values() const { return (char*)(hold.defined() ? hold : data).data_ptr(); }
-    char* scales() const { return hold.defined() ? values() + rows * padded(cols) : (char*)scale.data_ptr(); }
-    const Tensor& any() const { return hold.defined() ? hold : data; }
+    int64_t value_bytes() const { return rows * padded(cols); }
+    int64_t scale_bytes() const { return ((layout & SIREN_FP8_TILES) ? blocks(rows) : rows) * words(cols); }
 };
+
+// What the layer makes for itself lies in one allocation, each tensor's values before its scales; those that are not wanted
+// (no rows) take nothing
+Tensor hold(const Tensor& like, std::initializer_list<Blocks*> all, Tensor memory = Tensor()) {
+    int64_t size = 0;
+    for (const Blocks* b : all) size += b->value_bytes() + (b->scale_bytes() + 15) / 16 * 16;
+    if (!memory.defined() && size > 0) memory = at::empty({size}, like.options().dtype(at::kByte));
+    char* at = size > 0 ? (char*)memory.data_ptr() : nullptr;
+    for (Blocks* b : all) {
+        if (b->rows == 0) continue;
+        b->values = at;
+        b->scales = at + b->value_bytes();
+        at = b->scales + (b->scale_bytes() + 15) / 16 * 16;
+    }
+    return memory;
+}
+
+Blocks plan(int64_t rows, int64_t cols, int layout, int fmt = 0) {
+    Blocks b;
+    b.rows = rows;
+    b.cols = cols;
+    b.layout = layout;
+    b.fmt = fmt;
+    return b;
+}
 
 // x as the kernels read it: columns one element apart, rows any distance that does not overlap
 Tensor rows_of(const Tensor& x, int64_t& ld) {
@@ -91,46 +115,44 @@ Tensor rows_of(const Tensor& x, int64_t& ld) {
     return y;
 }
 
-enum Want { PANELS = 1, TRANSPOSED_PANELS = 2, TILES = 4, TENSORS = 8 };
-
-// One pass over x (times mult): its rows, its transpose's rows, its column sums, as wanted
-void quantize_into(const Tensor& x0, int want, int fmt, const Tensor& mult, Blocks* q, Blocks* qt, Tensor* colsum) {
-    int64_t ld;
-    const Tensor x = rows_of(x0, ld);
-    const int64_t rows = x.size(0), cols = x.size(1);
-    const auto u8 = x.options().dtype(at::kByte);
-    const bool tiles = want & TILES;
-    auto make = [&](Blocks* b, int64_t r, int64_t c, bool panels) {
-        const int64_t scale_rows = tiles ? blocks(r) : r;
-        if (want & TENSORS) {
-            b->data = at::empty({r, padded(c)}, x.options().dtype(fmt ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn));
-            b->scale = at::empty({scale_rows, words(c)}, u8);
-        } else {
-            b->hold = at::empty({r * padded(c) + scale_rows * words(c)}, u8);
+// One pass over x (times mult): its rows (q), its transpose's rows (qt), its column sums, those that have memory
+struct Source {
+    Tensor x, ws;
+    siren_fp8_source arg = {};
+    Source(const Tensor& x0, const Blocks& q, const Blocks& qt, const Tensor& mult, Tensor* colsum) {
+        x = rows_of(x0, arg.ld);
+        const Blocks& any = q.values ? q : qt;
+        arg.x = x.data_ptr();
+        arg.dtype = type_code(x.scalar_type());
+        arg.rows = x.size(0);
+        arg.cols = x.size(1);
+        arg.mult = mult.defined() ? mult.data_ptr() : nullptr;
+        arg.format = any.fmt;
+        arg.tiles = (any.layout & SIREN_FP8_TILES) != 0;
+        arg.panels = ((q.layout & SIREN_FP8_PANELS) ? 1 : 0) | ((qt.layout & SIREN_FP8_PANELS) ? 2 : 0);
+        arg.q = q.values;
+        arg.s = q.scales;
+        arg.qt = qt.values;
+        arg.st = qt.scales;
+        if (colsum) {
+            const auto f32 = x.options().dtype(at::kFloat);
+            if (arg.rows > 128) ws = at::empty({blocks(arg.rows), arg.cols}, f32);
+            *colsum = at::empty({arg.cols}, f32);
+            arg.colsum_ws = ws.defined() ? ws.data_ptr<float>() : nullptr;
+            arg.colsum = colsum->data_ptr<float>();
         }
-        b->rows = r;
-        b->cols = c;
-        b->layout = (tiles ? SIREN_FP8_TILES : 0) | (panels ? SIREN_FP8_PANELS : 0);
-        b->fmt = fmt;
-    };
-    if (q) make(q, rows, cols, want & PANELS);
-    if (qt) make(qt, cols, rows, want & TRANSPOSED_PANELS);
-    Tensor ws;
-    if (colsum) {
-        const auto f32 = x.options().dtype(at::kFloat);
-        if (rows > 128) ws = at::empty({blocks(rows), cols}, f32);
-        *colsum = at::empty({cols}, f32);
     }
-    const int panels = (want & PANELS ? 1 : 0) | (want & TRANSPOSED_PANELS ? 2 : 0);
-    check(lib.quantize(x.data_ptr(), type_code(x.scalar_type()), rows, cols, ld, mult.defined() ? mult.data_ptr() : nullptr, fmt,
-                       tiles, panels, q ? q->values() : nullptr, q ? q->scales() : nullptr, qt ? qt->values() : nullptr,
-                       qt ? qt->scales() : nullptr, ws.defined() ? ws.data_ptr<float>() : nullptr,
-                       colsum ? colsum->data_ptr<float>() : nullptr, stream_of(x)),
-          "siren_fp8_quantize");
+};
+
+void quantize_into(const Source& a) { check(lib.quantize(&a.arg, 1, stream_of(a.x)), "siren_fp8_quantize"); }
+void quantize_into(const Source& a, const Source& b) {
+    const siren_fp8_source both[2] = {a.arg, b.arg};
+    check(lib.quantize(both, 2, stream_of(a.x)), "siren_fp8_quantize");
 }
 
-Tensor product(const Blocks& a, const Blocks& b, const Tensor& bias, int act, double omega, at::ScalarType type, Tensor* deriv) {
-    const auto opt = a.any().options().dtype(at::kByte);
+Tensor product(const Tensor& like, const Blocks& a, const Blocks& b, const Tensor& bias, int act, double omega, at::ScalarType type,
+               Tensor* deriv) {
+    const auto opt = like.options().dtype(at::kByte);
     Tensor out = at::empty({a.rows, b.rows}, opt.dtype(type));
     // the sine's derivative meets a gradient that is rounded to 3 bits of mantissa next: 8 bits of it are enough
     if (deriv) *deriv = at::empty({a.rows, b.rows}, opt.dtype(at::kBFloat16));
@@ -138,9 +160,9 @@ Tensor product(const Blocks& a, const Blocks& b, const Tensor& bias, int act, do
     check(lib.matmul_ws_bytes(a.rows, b.rows, a.cols, &need), "siren_fp8_matmul_ws_bytes");
     Tensor ws;
     if (need) ws = at::empty({need}, opt);
-    check(lib.matmul(a.values(), a.scales(), a.rows, a.layout, a.fmt, b.values(), b.scales(), b.rows, b.layout, a.cols,
+    check(lib.matmul(a.values, a.scales, a.rows, a.layout, a.fmt, b.values, b.scales, b.rows, b.layout, a.cols,
                      bias.defined() ? bias.data_ptr<float>() : nullptr, act, (float)omega, out.data_ptr(), type_code(type),
-                     deriv ? deriv->data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, stream_of(a.any())),
+                     deriv ? deriv->data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, stream_of(like)),
           "siren_fp8_matmul");
     return out;
 }
@@ -156,7 +178,7 @@ Tensor serve(const Tensor& x0, const Blocks& w, const Tensor& bias, int act, dou
     check(lib.linear_ws_bytes(m, w.rows, k, &need), "siren_fp8_linear_ws_bytes");
     Tensor ws;
     if (need) ws = at::empty({need}, x.options().dtype(at::kByte));
-    check(lib.linear(x.data_ptr(), type_code(x.scalar_type()), m, k, ld, w.values(), w.scales(), w.rows,
+    check(lib.linear(x.data_ptr(), type_code(x.scalar_type()), m, k, ld, w.values, w.scales, w.rows,
                      bias.defined() ? bias.data_ptr<float>() : nullptr, act, (float)omega, y.data_ptr(),
                      deriv ? deriv->data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, stream_of(x)),
           "siren_fp8_linear");
@@ -189,19 +211,19 @@ void check_capture(std::initializer_list<const Tensor*> leaves) {
 
 // The backward of y = act(x W^T + b): x was read once in the forward, dy is read once here, each quantised both along its
 // rows and along its columns in that pass; the weight's tiles serve both directions. A Node of its own rather than a
-// torch::autograd::Function, whose dictionary and bookkeeping cost 4 us of the 88 of a training step of 8 x 128 x 128 (all of
-// it host time, half the engine's own).
+// torch::autograd::Function, whose dictionary and bookkeeping cost 4 us of the 88 that a training step of 8 x 128 x 128
+// then took (all of it host time, half the engine's own; 76 since x and the weight are one launch and two allocations).
 struct LinearBackward : torch::autograd::Node {
-    int64_t m = 0, n = 0, k = 0, fmt = 0;
+    int64_t m = 0, n = 0, k = 0, fmt = 0, kept_bytes = 0;
     at::ScalarType tx = at::kFloat, tw = at::kFloat, tb = at::kFloat;
-    torch::autograd::SavedVariable qxt, qwt, deriv;  // saved as torch saves, so that its hooks (checkpointing) see them
+    Blocks qxt, qwt;                               // x and the weight by their columns, in kept's memory
+    torch::autograd::SavedVariable kept, deriv;  // saved as torch saves, so that its hooks (checkpointing) see them
 
     std::string name() const override { return "Fp8LinearBackward"; }
 
     void release_variables() override {
         const std::lock_guard<std::mutex> lock(mutex_);
-        qxt.reset_data();
-        qwt.reset_data();
+        kept.reset_data();
         deriv.reset_data();
     }
 
@@ -210,7 +232,7 @@ struct LinearBackward : torch::autograd::Node {
         const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1), nb = task_should_compute_output(2);
         Tensor dx, dw, db;
         const Tensor& dy = grads[0];
-        if (!dy.defined()) return {dx, dw, db};
+        if (!dy.defined() || !(nx || nw || nb)) return {dx, dw, db};
         const auto opt = dy.options();
         if (m == 0) {
             if (nx) dx = at::empty({0, k}, opt.dtype(tx));
@@ -222,13 +244,22 @@ struct LinearBackward : torch::autograd::Node {
         const bool create_graph = at::GradMode::is_enabled();
         {
             const at::NoGradGuard no_grad;
-            Blocks q, qt;
+            const Tensor g = dy.detach(), memory = kept.unpack(), factor = deriv.unpack();
+            Blocks xt = qxt, wt = qwt;
+            // a hook may have held them in between
+            for (const Tensor* t : {&memory, &factor})
+                TORCH_CHECK(!t->defined() || (t->device() == g.device() && t->is_contiguous() && (uintptr_t)t->data_ptr() % 16 == 0),
+                            "fp8.linear: a saved tensor came back on ", t->device(), ", or not as it was saved");
+            TORCH_CHECK((!memory.defined() || (memory.scalar_type() == at::kByte && memory.numel() == kept_bytes)) &&
+                            (!factor.defined() || (factor.scalar_type() == at::kBFloat16 && factor.numel() == m * n)),
+                        "fp8.linear: a saved tensor came back with another type or size");
+            if (memory.defined()) hold(g, {&xt, &wt}, memory);
+            Blocks q = plan(nx ? m : 0, n, SIREN_FP8_PANELS, (int)fmt), qt = plan(nw ? n : 0, m, SIREN_FP8_PANELS, (int)fmt);
+            const Tensor own = hold(g, {&q, &qt});
             Tensor sums;
-            quantize_into(dy.detach(), PANELS | TRANSPOSED_PANELS, (int)fmt, deriv.unpack(), nx ? &q : nullptr, nw ? &qt : nullptr,
-                          nb ? &sums : nullptr);
-            const Tensor none;
-            if (nx) dx = product(q, {qwt.unpack(), none, none, k, n, SIREN_FP8_TILES | SIREN_FP8_PANELS}, none, 0, 0., tx, nullptr);
-            if (nw) dw = product(qt, {qxt.unpack(), none, none, k, m, SIREN_FP8_PANELS}, none, 0, 0., tw, nullptr);
+            quantize_into(Source(g, q, qt, factor, nb ? &sums : nullptr));
+            if (nx) dx = product(g, q, wt, Tensor(), 0, 0., tx, nullptr);
+            if (nw) dw = product(g, qt, xt, Tensor(), 0, 0., tw, nullptr);
             if (nb) db = sums.to(tb);
         }
         if (create_graph) {
@@ -260,22 +291,26 @@ Tensor train(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t 
         } else {
             const c10::DeviceGuard guard(x.device());
             const Tensor b32 = bias32(bias);
-            Blocks qx, qxt, qw, qwt;
+            const int64_t m = node->m, n = node->n, k = node->k;
+            int64_t ws = 0;
+            check(lib.linear_ws_bytes(m, n, k, &ws), "siren_fp8_linear_ws_bytes");
+            const bool few = ws == 0;  // the product quantises its rows itself, and reads the weight in rows
+            Blocks qx = plan(few ? 0 : m, k, SIREN_FP8_PANELS), qw = plan(n, k, SIREN_FP8_TILES | (few ? 0 : SIREN_FP8_PANELS));
+            const Tensor own = hold(x, {&qx, &qw});
+            Blocks &qxt = node->qxt, &qwt = node->qwt;
+            qxt = plan(nw ? k : 0, m, SIREN_FP8_PANELS);
+            qwt = plan(nx ? k : 0, n, SIREN_FP8_TILES | SIREN_FP8_PANELS);
+            const Tensor kept = hold(x, {&qxt, &qwt});
+            const Source from_w(weight, qw, qwt, Tensor(), nullptr);
+            if (few && !nw)
+                quantize_into(from_w);
+            else
+                quantize_into(Source(x, qx, qxt, Tensor(), nullptr), from_w);
             Tensor d;
             Tensor* deriv = act ? &d : nullptr;
-            int64_t ws = 0;
-            check(lib.linear_ws_bytes(node->m, node->n, node->k, &ws), "siren_fp8_linear_ws_bytes");
-            if (ws == 0) {  // few rows: the product quantises them itself, and reads the weight in rows
-                quantize_into(weight, TILES | TRANSPOSED_PANELS, 0, Tensor(), &qw, nx ? &qwt : nullptr, nullptr);
-                y = serve(x, qw, b32, (int)act, omega, deriv);
-                if (nw) quantize_into(x, TRANSPOSED_PANELS, 0, Tensor(), nullptr, &qxt, nullptr);
-            } else {
-                quantize_into(x, PANELS | TRANSPOSED_PANELS, 0, Tensor(), &qx, nw ? &qxt : nullptr, nullptr);
-                quantize_into(weight, TILES | PANELS | TRANSPOSED_PANELS, 0, Tensor(), &qw, nx ? &qwt : nullptr, nullptr);
-                y = product(qx, qw, b32, (int)act, omega, x.scalar_type(), deriv);
-            }
-            node->qxt = torch::autograd::SavedVariable(qxt.hold, false);
-            node->qwt = torch::autograd::SavedVariable(qwt.hold, false);
+            y = few ? serve(x, qw, b32, (int)act, omega, deriv) : product(x, qx, qw, b32, (int)act, omega, x.scalar_type(), deriv);
+            node->kept = torch::autograd::SavedVariable(kept, false);
+            node->kept_bytes = kept.defined() ? kept.numel() : 0;
             node->deriv = torch::autograd::SavedVariable(d, false);
         }
     }
@@ -319,26 +354,45 @@ Blocks packed_operand(const Tensor& data, const Tensor& scale, int64_t cols, con
                       "Blocks must be contiguous, their data 16-byte and their scales 4-byte aligned");
     TORCH_CHECK_VALUE(data.device() == dev && scale.device() == dev, "Blocks on ", data.device(), " but the other operand on ", dev);
     // one row is both: its tile is its row block
-    return {Tensor(), data, scale, data.size(0), cols, tiles_only || scale.size(0) != data.size(0) ? SIREN_FP8_TILES : 0,
-            format_code(data.scalar_type())};
+    Blocks b = plan(data.size(0), cols, tiles_only || scale.size(0) != data.size(0) ? SIREN_FP8_TILES : 0,
+                    format_code(data.scalar_type()));
+    b.values = (char*)data.data_ptr();
+    b.scales = (char*)scale.data_ptr();
+    return b;
+}
+
+// what the user holds: two tensors
+Blocks tensors(const Tensor& like, int64_t rows, int64_t cols, bool tiles, int64_t fmt, Tensor& data, Tensor& scale) {
+    Blocks b = plan(rows, cols, tiles ? SIREN_FP8_TILES : 0, (int)fmt);
+    data = at::empty({rows, padded(cols)}, like.options().dtype(fmt ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn));
+    scale = at::empty({tiles ? blocks(rows) : rows, words(cols)}, like.options().dtype(at::kByte));
+    b.values = (char*)data.data_ptr();
+    b.scales = (char*)scale.data_ptr();
+    return b;
+}
+
+void check_matrix(const Tensor& x) {
+    check_input(x, "x");
+    TORCH_CHECK_VALUE(x.dim() == 2, "x must be (rows, cols); got ", x.sizes());
 }
 
 std::pair<Tensor, Tensor> quantize(const Tensor& x, bool tiles, int64_t fmt) {
-    check_input(x, "x");
-    TORCH_CHECK_VALUE(x.dim() == 2, "x must be (rows, cols); got ", x.sizes());
+    check_matrix(x);
     const c10::DeviceGuard guard(x.device());
-    Blocks q;
-    quantize_into(x.detach(), TENSORS | (tiles ? TILES : 0), (int)fmt, Tensor(), &q, nullptr, nullptr);
-    return {q.data, q.scale};
+    Tensor data, scale;
+    const Blocks q = tensors(x, x.size(0), x.size(1), tiles, fmt, data, scale);
+    quantize_into(Source(x.detach(), q, Blocks(), Tensor(), nullptr));
+    return {data, scale};
 }
 
 std::vector<Tensor> quantize_both(const Tensor& x, bool tiles, int64_t fmt) {
-    check_input(x, "x");
-    TORCH_CHECK_VALUE(x.dim() == 2, "x must be (rows, cols); got ", x.sizes());
+    check_matrix(x);
     const c10::DeviceGuard guard(x.device());
-    Blocks q, qt;
-    quantize_into(x.detach(), TENSORS | (tiles ? TILES : 0), (int)fmt, Tensor(), &q, &qt, nullptr);
-    return {q.data, q.scale, qt.data, qt.scale};
+    Tensor data, scale, tdata, tscale;
+    const Blocks q = tensors(x, x.size(0), x.size(1), tiles, fmt, data, scale);
+    const Blocks qt = tensors(x, x.size(1), x.size(0), tiles, fmt, tdata, tscale);
+    quantize_into(Source(x.detach(), q, qt, Tensor(), nullptr));
+    return {data, scale, tdata, tscale};
 }
 
 std::pair<Tensor, MaybeTensor> matmul(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, int64_t cols,
@@ -355,7 +409,7 @@ std::pair<Tensor, MaybeTensor> matmul(const Tensor& a, const Tensor& sa, const T
     }
     const c10::DeviceGuard guard(a.device());
     Tensor d;
-    Tensor y = product(qa, qb, b32, (int)act, omega, type, derivative ? &d : nullptr);
+    Tensor y = product(a, qa, qb, b32, (int)act, omega, type, derivative ? &d : nullptr);
     return {y, derivative ? MaybeTensor(d) : std::nullopt};
 }
 
@@ -386,8 +440,9 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& maybe_bi
         return like_input(x, train(x2, weight, bias, act, omega, fmt));
     }
     const c10::DeviceGuard guard(x.device());
-    Blocks w;
-    quantize_into(weight.detach(), TILES, 0, Tensor(), &w, nullptr, nullptr);
+    Blocks w = plan(weight.size(0), weight.size(1), SIREN_FP8_TILES);
+    const Tensor own = hold(weight, {&w});
+    quantize_into(Source(weight.detach(), w, Blocks(), Tensor(), nullptr));
     return like_input(x, serve(x2.detach(), w, bias32(bias), (int)act, omega, nullptr));
 }
 

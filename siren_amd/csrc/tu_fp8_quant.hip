@@ -21,18 +21,37 @@ namespace {
 constexpr int QT = 128;           // tile edge
 constexpr int QSTRIDE = QT + 16;  // LDS row of the transposed bytes: 16-byte pieces on distinct banks
 
+struct QuantArgs {
+    const void* x;
+    int64_t ld, rows, cols;
+    const __bf16* mult;
+    uint8_t *q, *s, *qt, *st;
+    float* colsum;
+    int tiles, near, col_blocks, panels;
+};
+
+// One tensor, or two in one launch (a layer's x and weight: small ones are all launch): workgroups from `first` on take b's
+// tiles.
 template <typename T, bool E5M2, bool MULT>
-__global__ __launch_bounds__(256, 4) void quant_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
-                                                    const __bf16* __restrict__ mult, uint8_t* __restrict__ q,
-                                                    uint8_t* __restrict__ s, uint8_t* __restrict__ qt,
-                                                    uint8_t* __restrict__ st, float* __restrict__ colsum, int tiles,
-                                                    int near, int col_blocks, int panels) {
+__global__ __launch_bounds__(256, 4) void quant_kernel(QuantArgs a, QuantArgs b, unsigned first) {
+    const bool second = blockIdx.x >= first;
+    const QuantArgs& arg = second ? b : a;
+    const unsigned tile = second ? blockIdx.x - first : blockIdx.x;
+    const T* __restrict__ x = (const T*)arg.x;
+    const int64_t ld = arg.ld, rows = arg.rows, cols = arg.cols;
+    const __bf16* __restrict__ mult = arg.mult;
+    uint8_t* __restrict__ q = arg.q;
+    uint8_t* __restrict__ s = arg.s;
+    uint8_t* __restrict__ qt = arg.qt;
+    uint8_t* __restrict__ st = arg.st;
+    float* __restrict__ colsum = arg.colsum;
+    const int tiles = arg.tiles, near = arg.near, col_blocks = arg.col_blocks, panels = arg.panels;
     __shared__ __align__(16) uint8_t tr[QT * QSTRIDE];
     __shared__ float part[8][QT];
     __shared__ float wmax[4];
     const int t = threadIdx.x, c4 = t & 31, rg = t >> 5;
-    const int64_t rb = blockIdx.x / col_blocks;
-    const int cb = (int)(blockIdx.x % col_blocks);
+    const int64_t rb = tile / (unsigned)col_blocks;
+    const int cb = (int)(tile % (unsigned)col_blocks);
     const int64_t r0 = rb * QT + rg * 16;
     const int64_t c0 = (int64_t)cb * QT + c4 * 4;
     const int64_t row_blocks = (rows + QT - 1) / QT;
@@ -314,28 +333,25 @@ __global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ 
 
 }  // namespace
 
-void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
-    const int64_t col_blocks = fp8_blocks(a.cols), grid = fp8_blocks(a.rows) * col_blocks;
+namespace {
+
+bool rows_only(const Fp8Quant& a) { return a.qt == nullptr && a.colsum == nullptr && a.mult == nullptr && !a.tiles; }
+
+QuantArgs args_of(const Fp8Quant& a) {
     const int near = a.rows == 1 || a.ld < 1 << 25;  // 31 rows are less than 2^32 bytes apart
-    if (a.qt == nullptr && a.colsum == nullptr && a.mult == nullptr && !a.tiles) {
-        const int64_t groups = (a.rows + ROWS_PER_GROUP - 1) / ROWS_PER_GROUP * col_blocks;
-#define SIREN_QUANT_ROWS(T, E)                                                                                           \
-    hipLaunchKernelGGL((quant_rows_kernel<T, E>), dim3((unsigned)groups), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
-                       a.cols, a.q, a.s, (int)col_blocks, a.panels)
-        if (a.type == FP8_F32 && a.e5m2) SIREN_QUANT_ROWS(float, true);
-        if (a.type == FP8_BF16 && a.e5m2) SIREN_QUANT_ROWS(__bf16, true);
-        if (a.type == FP8_F16 && a.e5m2) SIREN_QUANT_ROWS(_Float16, true);
-        if (a.type == FP8_F32 && !a.e5m2) SIREN_QUANT_ROWS(float, false);
-        if (a.type == FP8_BF16 && !a.e5m2) SIREN_QUANT_ROWS(__bf16, false);
-        if (a.type == FP8_F16 && !a.e5m2) SIREN_QUANT_ROWS(_Float16, false);
-#undef SIREN_QUANT_ROWS
-        return;
-    }
-#define SIREN_QUANT(T, E, M)                                                                                            \
-    hipLaunchKernelGGL((quant_kernel<T, E, M>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, a.cols, \
-                       (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, near, (int)col_blocks, a.panels)
-#define SIREN_QUANT_TYPES(E, M)                     \
-    do {                                            \
+    return QuantArgs{a.x, a.ld, a.rows, a.cols, (const __bf16*)a.mult, a.q, a.s, a.qt, a.st, a.colsum, a.tiles, near,
+                     (int)fp8_blocks(a.cols), a.panels};
+}
+
+unsigned tiles_in(const Fp8Quant& a) { return (unsigned)(fp8_blocks(a.rows) * fp8_blocks(a.cols)); }
+
+void launch_tiles(hipStream_t stream, const Fp8Quant& a, const Fp8Quant* b) {
+    const QuantArgs first = args_of(a), second = b != nullptr ? args_of(*b) : first;
+    const unsigned n = tiles_in(a);
+    const dim3 grid(n + (b != nullptr ? tiles_in(*b) : 0u));
+#define SIREN_QUANT(T, E, M) hipLaunchKernelGGL((quant_kernel<T, E, M>), grid, dim3(256), 0, stream, first, second, n)
+#define SIREN_QUANT_TYPES(E, M)                              \
+    do {                                                     \
         if (a.type == FP8_F32) SIREN_QUANT(float, E, M);     \
         if (a.type == FP8_BF16) SIREN_QUANT(__bf16, E, M);   \
         if (a.type == FP8_F16) SIREN_QUANT(_Float16, E, M);  \
@@ -350,6 +366,32 @@ void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
         SIREN_QUANT_TYPES(false, false);
 #undef SIREN_QUANT_TYPES
 #undef SIREN_QUANT
+}
+
+}  // namespace
+
+void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
+    if (!rows_only(a)) return launch_tiles(stream, a, nullptr);
+    const int col_blocks = (int)fp8_blocks(a.cols);
+    const int64_t groups = (a.rows + ROWS_PER_GROUP - 1) / ROWS_PER_GROUP * col_blocks;
+#define SIREN_QUANT_ROWS(T, E)                                                                                           \
+    hipLaunchKernelGGL((quant_rows_kernel<T, E>), dim3((unsigned)groups), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
+                       a.cols, a.q, a.s, col_blocks, a.panels)
+    if (a.type == FP8_F32 && a.e5m2) SIREN_QUANT_ROWS(float, true);
+    if (a.type == FP8_BF16 && a.e5m2) SIREN_QUANT_ROWS(__bf16, true);
+    if (a.type == FP8_F16 && a.e5m2) SIREN_QUANT_ROWS(_Float16, true);
+    if (a.type == FP8_F32 && !a.e5m2) SIREN_QUANT_ROWS(float, false);
+    if (a.type == FP8_BF16 && !a.e5m2) SIREN_QUANT_ROWS(__bf16, false);
+    if (a.type == FP8_F16 && !a.e5m2) SIREN_QUANT_ROWS(_Float16, false);
+#undef SIREN_QUANT_ROWS
+}
+
+void launch_fp8_quant2(hipStream_t stream, const Fp8Quant& a, const Fp8Quant& b) {
+    const bool alike = a.type == b.type && a.e5m2 == b.e5m2 && (a.mult != nullptr) == (b.mult != nullptr);
+    if (alike && !rows_only(a) && !rows_only(b) && (int64_t)tiles_in(a) + tiles_in(b) <= 0xFFFFFF)
+        return launch_tiles(stream, a, &b);
+    launch_fp8_quant(stream, a);
+    launch_fp8_quant(stream, b);
 }
 
 void launch_fp8_colsum(hipStream_t stream, const float* colsum, int64_t blocks, int64_t cols, float* out) {

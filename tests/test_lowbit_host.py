@@ -32,6 +32,30 @@ def test_quantize_validates(lib):
         assert lib.siren_last_error()
 
 
+def test_quantize_sources_validate(lib):
+    def source(**kw):
+        f = dict(x=64, dtype=0, format=0, rows=4, cols=8, ld=8, mult=None, tiles=0, panels=0, q=64, s=64, qt=None, st=None,
+                 colsum_ws=None, colsum=None)
+        f.update(kw)
+        return tuple(f[name] for name, _ in Source._fields_)
+
+    class Source(ctypes.Structure):
+        _fields_ = [('x', P), ('dtype', ctypes.c_int32), ('format', ctypes.c_int32), ('rows', ctypes.c_int64),
+                    ('cols', ctypes.c_int64), ('ld', ctypes.c_int64), ('mult', P), ('tiles', ctypes.c_int32),
+                    ('panels', ctypes.c_int32)] + [(n, P) for n in ('q', 's', 'qt', 'st', 'colsum_ws', 'colsum')]
+
+    def call(*sources, count=None):
+        held = (Source * len(sources))(*sources)
+        return lib.siren_fp8_quantize_sources(ctypes.byref(held), len(sources) if count is None else count, None)
+    assert call(source(rows=0)) == OK and call(source(rows=0), source(cols=0)) == OK
+    assert lib.siren_fp8_quantize_sources(None, 1, None) == EINVAL
+    for count in (0, 3, -1):
+        assert call(source(rows=0), source(rows=0), count=count) == EINVAL
+    # a wrong second one is refused before the first is begun
+    for bad in (dict(dtype=3), dict(s=None), dict(ld=7), dict(q=None, s=None), dict(x=None), dict(panels=4)):
+        assert call(source(), source(**bad)) == EINVAL and call(source(**bad), source()) == EINVAL, bad
+
+
 def test_products_validate(lib):
     def call(a=P(64), sa=P(64), m=4, b=P(64), sb=P(64), n=4, k=8, bias=None, act=0, omega=30., out=P(64), dtype=0, deriv=None,
              ws=None, fmt=0):

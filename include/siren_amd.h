@@ -458,7 +458,7 @@ int32_t siren_fp8_matmul(const void* a, const void* sa, int64_t m, int32_t a_lay
 
 /* y (m, n) = act(x w^T + bias), the layer of siren_fp8_quantize (rows of x, e4m3) and siren_fp8_matmul in one call:
  * x (m, k) of row stride ld, w (n, k) in 8 bits, tiles, in rows, y in x's dtype, deriv as
- * above. ws: siren_fp8_linear_ws_bytes (0 for up to 32 rows, which are one launch). */
+ * above. ws: siren_fp8_linear_ws_bytes (0 where few rows are one launch). */
 int32_t siren_fp8_linear_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes);
 int32_t siren_fp8_linear(const void* x, int32_t dtype, int64_t m, int64_t k, int64_t ld, const void* w, const void* sw,
                          int64_t n, const float* bias, int32_t act, float omega, void* y, void* deriv, void* ws, void* stream);

@@ -53,7 +53,7 @@ struct Fp8Product {
     void* ws;
 };
 // y (m, n) = act(x w^T + bias) for a few rows m in one launch, x quantised on the way (w: rows, tiles)
-bool fp8_few_rows(int64_t m);
+bool fp8_few_rows(int64_t m, int64_t n, int64_t k);
 void launch_fp8_few_rows(hipStream_t st, const void* x, int type, int64_t ld, int64_t m, int64_t k, const uint8_t* w,
                          const uint8_t* sw, int64_t n, const float* bias, int act, float omega, void* y, void* deriv);
 int64_t fp8_product_ws_bytes(int64_t m, int64_t n, int64_t k);

@@ -1782,7 +1782,7 @@ int32_t siren_fp8_matmul(const void* a, const void* sa, int64_t m, int32_t a_lay
 int32_t siren_fp8_linear_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes) {
     if (bytes == nullptr) return fail(SIREN_EINVAL, "bytes is NULL");
     if (int rc = check_fp8_product(m, n, k)) return rc;
-    *bytes = m == 0 || n == 0 || siren::fp8_few_rows(m)
+    *bytes = m == 0 || n == 0 || siren::fp8_few_rows(m, n, k)
                  ? 0
                  : (m * siren::fp8_padded(k) + m * siren::fp8_scale_cols(k) + 15) / 16 * 16 +
                                     siren::fp8_product_ws_bytes(m, n, k);
@@ -1796,7 +1796,7 @@ int32_t siren_fp8_linear(const void* x, int32_t dtype, int64_t m, int64_t k, int
     if (int rc = check_fp8_act(act, omega, deriv)) return rc;
     if (m == 0 || n == 0) return SIREN_OK;
     if (int rc = check_fp8_source(x, dtype, m, k, ld)) return rc;
-    const bool few = siren::fp8_few_rows(m);
+    const bool few = siren::fp8_few_rows(m, n, k);
     if (int rc = check_fp8_operands(few ? w : ws, few ? sw : ws, w, sw, bias, y, deriv)) return rc;
     if (few) {
         siren::launch_fp8_few_rows((hipStream_t)stream, x, dtype, ld, m, k, (const uint8_t*)w, (const uint8_t*)sw, n, bias,

@@ -51,19 +51,20 @@ struct GemmArgs {
 };
 
 // Nontemporal: a result is read by a later kernel, after the operands that it would push out of L2 (262144 x 1024 x 1024
-// fp32 out: 620 -> 550 us). Rows of odd widths begin within lines that two stores share, which L2 has to join: 30000 x 1023
-// fp32 takes 58 us through L2, 96 nontemporal, 71 element by element.
+// fp32 out: 620 -> 550 us). Rows that begin anywhere but at 64 bytes leave lines that two stores share, which L2 has to join:
+// 30000 x 1023 fp32 takes 58 us through L2, 96 nontemporal, 71 element by element; 14768 x 13240 bf16 174 and 338; with rows
+// of 1008 fp32 (a multiple of 64 bytes, not of 128) it is 199 through L2 and 131.
 // dst is global memory, which the compiler has to be told: a pointer out of a struct of arguments is generic to it, and a flat
 // store counts as an access of LDS too, so that the epilogue's waits for LDS waited for memory
 // (65536 x 256 x 256 bf16: 17.0 us, 13.8 with both this and the pacing of stores below).
 template <typename T>
-__device__ __forceinline__ void put4(T* dst, f32x4 v, int valid, bool vec) {
+__device__ __forceinline__ void put4(T* dst, f32x4 v, int valid, bool once) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(1))) T Element;
     typedef __attribute__((address_space(1))) T4 Line;
     typedef __attribute__((address_space(1))) typename Quad<T>::Type Anywhere;
     const T4 h = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-    if (vec && valid >= 4) {
+    if (once && valid >= 4) {
         __builtin_nontemporal_store(h, (Line*)dst);
     } else if (valid >= 4) {
         *(Anywhere*)dst = h;
@@ -105,11 +106,12 @@ template <typename T>
 struct Finish {
     int64_t col;
     int valid;
-    bool vec;
+    bool once, once16;  // rows of T, of 16 bits, begin at 64 bytes
     f32x4 bias;
     __device__ __forceinline__ Finish(const GemmArgs& g, int64_t c) : col(c) {
         valid = g.n - col < 4 ? (int)(g.n - col) : 4;
-        vec = (g.n & 3) == 0;
+        once = (g.n * (int)sizeof(T) & 63) == 0;
+        once16 = (g.n * 2 & 63) == 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) bias[k] = g.bias != nullptr && k < valid ? g.bias[col + k] : 0.f;
     }
@@ -121,12 +123,12 @@ struct Finish {
                 f32x4 d;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) d[k] = g.omega * __builtin_amdgcn_cosf(u[k]);
-                put4(g.deriv + row * g.n + col, d, valid, vec);
+                put4(g.deriv + row * g.n + col, d, valid, once16);
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_sinf(u[k]);
         }
-        put4((T*)g.out + row * g.n + col, v, valid, vec);
+        put4((T*)g.out + row * g.n + col, v, valid, once);
     }
 };
 
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
                     const int64_t m = wave_m + row + 8 * u;
                     if (m < g.m) {
                         if constexpr (SPLIT)
-                            put4((float*)g.out + (split * g.m + m) * g.n + col, v[u], to.valid, to.vec);
+                            put4((float*)g.out + (split * g.m + m) * g.n + col, v[u], to.valid, to.once);
                         else
                             to.store(g, m, v[u]);
                     }
@@ -327,22 +329,27 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
 // bits into LDS while they travel (half a wave a block), then the wave's rows of the weight times the rows of x, 16 at a
 // time. Rows of x that do not exist are whatever LDS holds: an output depends on its own row only. 65536 columns of 256:
 // 6 us for one row (16.8 MB: 2.8 TB/s), 9 for 32 (8.4 MB of results more).
-constexpr int FEW_ROWS = 32, FEW_K = 512, FEW_LD = FEW_K + 16;  // LDS rows 16 bytes apart from a bank period
+constexpr int FEW_ROWS = 32, FEW_K = 512;
 struct FewArgs {
     const void* x;
     int64_t ld, m, k;
     const uint8_t *w, *sw;
     GemmArgs out;  // n, bias, act, omega, out
 };
-template <typename T, int MT, int NT>
+//
+// KW = 4: the waves share 16 columns and split k, 2048 of it at a time, and add their sums in order through LDS: a quarter
+// of the steps where the columns alone do not fill the card (1 row, 4096 -> 1024: 16.8 us, 8.8).
+template <typename T, int MT, int NT, int KW>
 __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs f) {
-    constexpr int CHUNK = FEW_K / 128;
-    __shared__ __align__(16) uint8_t xq[MT * 16 * FEW_LD];
-    __shared__ uint8_t xs[MT * 16 * CHUNK];
+    constexpr int CHUNK = FEW_K / 128, ALL = CHUNK * KW;  // blocks of a wave, of the workgroup
+    constexpr int LD = ALL * 128 + 16;                    // LDS rows 16 bytes apart from a bank period
+    __shared__ __align__(16) uint8_t xq[MT * 16 * LD];
+    __shared__ uint8_t xs[MT * 16 * ALL];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, q = lane >> 4;
     const GemmArgs& g = f.out;
-    const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * (NT * 16);
+    const int64_t n0 = (KW == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x) * (NT * 16);
+    const int own = KW == 1 ? 0 : wave * CHUNK;  // the wave's first block among the workgroup's
     const int64_t kp = (f.k + 127) / 128 * 128;
     const int blocks = (int)(kp / 128);
     const uint8_t *w[NT], *sw[NT];
@@ -353,23 +360,24 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs f) {
         sw[j] = f.sw + (row >> 7) * ((blocks + 3) / 4 * 4);
     }
     f32x4 acc[MT][NT] = {};
-    for (int b0 = 0; b0 < blocks; b0 += CHUNK) {
-        const int here = blocks - b0 < CHUNK ? blocks - b0 : CHUNK;
+    for (int b0 = 0; b0 < blocks; b0 += ALL) {
+        const int here = blocks - b0 < ALL ? blocks - b0 : ALL;             // blocks of the workgroup
+        const int mine = here - own < CHUNK ? here - own : CHUNK;           // of the wave; none or fewer: nothing
         u32x4 wv[NT][CHUNK][2];
         uint32_t scales[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            scales[j] = *(const uint32_t*)(sw[j] + b0);
+            scales[j] = mine > 0 ? *(const uint32_t*)(sw[j] + b0 + own) : 0u;
 #pragma unroll
             for (int b = 0; b < CHUNK; ++b)
-                if (b < here) {
-                    wv[j][b][0] = *(const u32x4*)(w[j] + (b0 + b) * 128);
-                    wv[j][b][1] = *(const u32x4*)(w[j] + (b0 + b) * 128 + 64);
+                if (b < mine) {
+                    wv[j][b][0] = *(const u32x4*)(w[j] + (b0 + own + b) * 128);
+                    wv[j][b][1] = *(const u32x4*)(w[j] + (b0 + own + b) * 128 + 64);
                 }
         }
         if (b0 > 0) __syncthreads();  // x of the chunk before has been read
         // units of one block of one row, BATCH of a half wave's loaded before the first is rounded
-        constexpr int BATCH = MT == 1 ? 2 : 8;
+        constexpr int BATCH = MT == 1 && KW == 1 ? 2 : 8;
         const int c4 = threadIdx.x & 31, half = threadIdx.x >> 5, all = (int)f.m * here;
         for (int u0 = half; u0 < all; u0 += 8 * BATCH) {
             float v[BATCH][4];
@@ -384,24 +392,24 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs f) {
                 const int u = u0 + 8 * i, row = u / here, b = u - row * here;
                 const int byte = exponent_byte<false>(half_wave_amax(v[i][0], v[i][1], v[i][2], v[i][3]));
                 if (u < all) {
-                    *(uint32_t*)(xq + row * FEW_LD + b * 128 + c4 * 4) =
+                    *(uint32_t*)(xq + row * LD + b * 128 + c4 * 4) =
                         pack4<false>(v[i][0], v[i][1], v[i][2], v[i][3], scale_of(byte));
-                    if (c4 == 0) xs[row * CHUNK + b] = (uint8_t)byte;
+                    if (c4 == 0) xs[row * ALL + b] = (uint8_t)byte;
                 }
             }
         }
         __syncthreads();
 #pragma unroll
         for (int b = 0; b < CHUNK; ++b) {
-            if (b < here) {
+            if (b < mine) {
                 bf16x8 xf[MT][4];
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     const int row = t * 16 + r;
-                    const float fx = scale_of(xs[row * CHUNK + b]);
+                    const float fx = scale_of(xs[row * ALL + own + b]);
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
-                        const u32x4 c = *(const u32x4*)(xq + row * FEW_LD + b * 128 + p * 64 + q * 16);
+                        const u32x4 c = *(const u32x4*)(xq + row * LD + (own + b) * 128 + p * 64 + q * 16);
                         xf[t][2 * p] = widen8<false>(c[0], c[1], fx);
                         xf[t][2 * p + 1] = widen8<false>(c[2], c[3], fx);
                     }
@@ -420,6 +428,19 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs f) {
                 }
             }
         }
+    }
+    if constexpr (KW > 1) {
+        static_assert(NT == 1 && MT * 16 * LD >= KW * MT * 1024, "a wave's sums fit its share of x");
+        __syncthreads();  // x has been read
+        f32x4* red = (f32x4*)xq;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) red[(wave * MT + t) * 64 + lane] = acc[t][0];
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int k = 1; k < KW; ++k) acc[t][0] += red[(k * MT + t) * 64 + lane];
     }
     // the weight's rows are the instruction's rows: lane (r, q) holds y[r][n0 + 16 j + 4 q ..]
 #pragma unroll
@@ -544,7 +565,16 @@ void launch_gemm(hipStream_t stream, GemmArgs& g, int splits, bool rows256) {
 
 }  // namespace
 
-bool fp8_few_rows(int64_t m) { return m <= FEW_ROWS; }
+// One launch, or rounding, product and join. Each workgroup of the one rounds all of x, four rows of 2048 k in a round trip of
+// 3.3 us; the three take 14 us whatever the size. Columns 1024, one launch and three: 1 row of 4096 8.8 and 14.8 us, of 16384
+// 29 and 15.6; 9 rows of 2048 9.9 and 15.0, of 4096 17.4 and 14.8; 16 rows of 2048 11.7 and 14.6; 32 rows of 512 7.9 and 11.9,
+// of 1024 13.6 and 14.5, of 2048 25.7 and 14.9, 30 rows of 999 in bf16 21 and 15. Where the columns fill the card it reads the
+// weight's bytes as fast: 30000 x 16384 with 4 rows 110 and 130 us.
+bool fp8_few_rows(int64_t m, int64_t n, int64_t k) {
+    const bool wide = n >= 64 * 256;
+    if (m > 16) return m <= FEW_ROWS && k <= FEW_K;
+    return (m + 3) / 4 * ((k + 2047) / 2048) <= 4 || (wide && m <= 4);
+}
 
 void launch_fp8_few_rows(hipStream_t stream, const void* x, int type, int64_t ld, int64_t m, int64_t k, const uint8_t* w,
                          const uint8_t* sw, int64_t n, const float* bias, int act, float omega, void* y, void* deriv) {
@@ -562,19 +592,23 @@ void launch_fp8_few_rows(hipStream_t stream, const void* x, int type, int64_t ld
     f.out.omega = omega;
     f.out.out = y;
     f.out.deriv = (__bf16*)deriv;
-    // 32 columns a wave where that still is a workgroup a CU: half the rounding of x
-    const bool two = n >= 128 * 256;
-    const dim3 grid((unsigned)((n + (two ? 127 : 63)) / (two ? 128 : 64)));
+    // 32 columns a wave where that still is a workgroup a CU: half the rounding of x. A long k whose columns fill fewer CUs is
+    // split among a workgroup's waves
+    const bool two = n >= 128 * 256, split = m <= 16 && k > FEW_K && n < 64 * 256;
+    const int columns = split ? 16 : two ? 128 : 64;
+    const dim3 grid((unsigned)((n + columns - 1) / columns));
 #define SIREN_FEW(T)                                                                                \
     do {                                                                                            \
-        if (m <= 16 && two)                                                                         \
-            hipLaunchKernelGGL((few_rows_kernel<T, 1, 2>), grid, dim3(256), 0, stream, f);          \
+        if (split)                                                                                  \
+            hipLaunchKernelGGL((few_rows_kernel<T, 1, 1, 4>), grid, dim3(256), 0, stream, f);       \
+        else if (m <= 16 && two)                                                                    \
+            hipLaunchKernelGGL((few_rows_kernel<T, 1, 2, 1>), grid, dim3(256), 0, stream, f);       \
         else if (m <= 16)                                                                           \
-            hipLaunchKernelGGL((few_rows_kernel<T, 1, 1>), grid, dim3(256), 0, stream, f);          \
+            hipLaunchKernelGGL((few_rows_kernel<T, 1, 1, 1>), grid, dim3(256), 0, stream, f);       \
         else if (two)                                                                               \
-            hipLaunchKernelGGL((few_rows_kernel<T, 2, 2>), grid, dim3(256), 0, stream, f);          \
+            hipLaunchKernelGGL((few_rows_kernel<T, 2, 2, 1>), grid, dim3(256), 0, stream, f);       \
         else                                                                                        \
-            hipLaunchKernelGGL((few_rows_kernel<T, 2, 1>), grid, dim3(256), 0, stream, f);          \
+            hipLaunchKernelGGL((few_rows_kernel<T, 2, 1, 1>), grid, dim3(256), 0, stream, f);       \
     } while (0)
     if (type == FP8_F32) SIREN_FEW(float);
     if (type == FP8_BF16) SIREN_FEW(__bf16);

@@ -587,3 +587,22 @@ def test_gradients_of_some_leaves(cuda, m, dtype, needs):
         fp8.linear(*some, act).backward(dy)
         for t, g, n in zip(some, want, needs):
             assert torch.equal(t.grad, g) if n else t.grad is None
+
+
+@pytest.mark.parametrize('m', [1, 4, 5, 9, 16, 17, 32, 33])
+@pytest.mark.parametrize('k,n', [(513, 40), (1024, 300), (1025, 16384), (2048, 16385), (2049, 17), (4100, 70), (8192, 33), (8193, 129)])
+def test_few_rows_of_long_sums(cuda, m, k, n):
+    """Small whole numbers again: however few rows share out a long sum, it is exact; and a sine of it as a plain product's."""
+    from siren_amd import fp8
+    g = torch.Generator(device=cuda).manual_seed(m * k + n)
+    x = torch.randint(-3, 4, (m, k), generator=g, device=cuda).float()
+    w = torch.randint(-3, 4, (n, k), generator=g, device=cuda).float()
+    x[:, ::128], w[:, ::128] = 4., 4.
+    b = torch.randint(-9, 9, (n,), generator=g, device=cuda).float()
+    w8 = fp8.quantize(w, 'tile')
+    want = x.double() @ w.double().t().contiguous() + b
+    assert torch.equal(fp8.linear(x, w8, b).double(), want)
+    y = fp8.linear(x.bfloat16(), w8, b)
+    assert y.dtype is torch.bfloat16 and torch.equal(y, want.float().bfloat16())
+    plain = fp8.matmul(fp8.quantize(x), w8, b, 'sine', omega=0.01)
+    assert torch.equal(fp8.linear(x, w8, b, 'sine', omega=0.01), plain)

@@ -180,8 +180,9 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
     constexpr int STAGE = (TM + TN) * HK;       // bytes of one half block
     constexpr int LOADS = (TM + TN) / 16 / 4;   // 1 KiB pieces of it a wave loads
     constexpr int STAGES = RT == 2 ? 2 : 3;
-    constexpr int ES = 36;                      // floats of an LDS row of the epilogue
-    constexpr int STRIP = RT * 32 * ES;         // floats of a wave's
+    constexpr int ES = 68;                      // floats of an LDS row of the epilogue
+    constexpr int PASS = RT / 2;                // tiles of 32 rows a wave stores at a time
+    constexpr int STRIP = PASS * 32 * ES;       // floats of a wave's strip
     __shared__ __align__(16) uint8_t lds[STAGES * STAGE > STRIP * 16 ? STAGES * STAGE : STRIP * 16];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave & 1, wn = wave >> 1;
@@ -282,35 +283,41 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmArgs g) {
     }
 
     // B rows are the instruction's rows: registers 4 k .. 4 k + 3 of a 32 x 32 tile are out[lane % 32][8 k + 4 (lane / 32) ..].
-    // They pass through LDS (the wave's quarter of the stages, which no one reads any more), 32 columns at a time, so that
-    // 8 lanes store 128 bytes of one row: stored as they lie, 32 bytes a row, they cost HBM twice the requests. The loop
-    // over the rows also keeps the epilogue short; unrolled over the accumulators it outgrew the instruction cache.
+    // They pass through LDS (the wave's quarter of the stages, which no one reads any more), half of the wave's rows at a time,
+    // so that 16 lanes store the wave's 64 columns of one row: stored as they lie, 32 bytes a row, they cost HBM twice the
+    // requests, and with 32 columns at a time rows of odd widths left twice the shared lines (174691 x 344 x 1282 fp32: 411 us,
+    // now 319). The loop over the rows also keeps the epilogue short; unrolled over the accumulators it outgrew the
+    // instruction cache.
     float* strip = (float*)lds + wave * STRIP;
     __syncthreads();
     const int64_t wave_m = m0 + wm * RT * 32;
-    const int sub = lane >> 3, quad = (lane & 7) * 4;
+    const int sub = lane >> 4, quad = (lane & 15) * 4;
+    const int64_t col = n0 + wn * 64 + quad;
+    const Finish<T> to(g, col);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int p = 0; p < 2; ++p) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < PASS; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                *(f32x4*)(strip + (i * 32 + (lane & 31)) * ES + 8 * k + 4 * (lane >> 5)) =
-                    f32x4{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f32x16& from = acc[p * PASS + i][j];
+                    *(f32x4*)(strip + (i * 32 + (lane & 31)) * ES + j * 32 + 8 * k + 4 * (lane >> 5)) =
+                        f32x4{from[4 * k], from[4 * k + 1], from[4 * k + 2], from[4 * k + 3]};
+                }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const int64_t col = n0 + (wn * 2 + j) * 32 + quad;
         if (col < g.n) {
-            const Finish<T> to(g, col);
-            for (int row = sub; row < RT * 32; row += 32) {  // four rows' reads before the first is stored
+            for (int row = sub; row < PASS * 32; row += 16) {  // four rows' reads before the first is stored
                 // Eight of a wave's stores under way and no more: a burst of all 32 stands before the loads of the workgroup
                 // that shares the CU (262144 x 1024 x 1024 fp32 526 us, paced 510; 50001 x 832 x 320 bf16 37.5 and 35.4)
                 asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
                 f32x4 v[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = *(const f32x4*)(strip + (row + 8 * u) * ES + quad);
+                for (int u = 0; u < 4; ++u) v[u] = *(const f32x4*)(strip + (row + 4 * u) * ES + quad);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const int64_t m = wave_m + row + 8 * u;
+                    const int64_t m = wave_m + p * PASS * 32 + row + 4 * u;
                     if (m < g.m) {
                         if constexpr (SPLIT)
                             put4((float*)g.out + (split * g.m + m) * g.n + col, v[u], to.valid, to.once);

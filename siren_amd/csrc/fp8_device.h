@@ -5,6 +5,7 @@
 
 namespace siren {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -92,14 +93,28 @@ __device__ __forceinline__ float half_wave_max(float m) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// the largest finite magnitude of a half wave's quads: where the plain maximum of any in the wave is not finite (fmaxf
-// drops a NaN beside a number), the quads are looked through again
-__device__ __forceinline__ float half_wave_amax(float a, float b, float c, float d) {
-    float m = half_wave_max(fmaxf(fmaxf(__builtin_fabsf(a), __builtin_fabsf(b)),
-                                  fmaxf(__builtin_fabsf(c), __builtin_fabsf(d))));
-    if (__builtin_expect(__any(!(m < INFINITY)), 0))
-        m = half_wave_max(fmaxf(fmaxf(finite_abs(a), finite_abs(b)), fmaxf(finite_abs(c), finite_abs(d))));
+// the largest finite magnitude of a block, one quad a lane of half a wave or two a lane of a quarter: where the plain maximum
+// of any in the wave is not finite (fmaxf drops a NaN beside a number), the quads are looked through again
+template <int QUADS>
+__device__ __forceinline__ float block_amax(const float (&v)[QUADS][4]) {
+    float m = 0.f;
+#pragma unroll
+    for (int d = 0; d < QUADS; ++d)
+        m = fmaxf(m, fmaxf(fmaxf(__builtin_fabsf(v[d][0]), __builtin_fabsf(v[d][1])),
+                           fmaxf(__builtin_fabsf(v[d][2]), __builtin_fabsf(v[d][3]))));
+    m = QUADS == 1 ? half_wave_max(m) : row16_max(m);
+    if (__builtin_expect(__any(!(m < INFINITY)), 0)) {
+        m = 0.f;
+#pragma unroll
+        for (int d = 0; d < QUADS; ++d)
+            m = fmaxf(m, fmaxf(fmaxf(finite_abs(v[d][0]), finite_abs(v[d][1])), fmaxf(finite_abs(v[d][2]), finite_abs(v[d][3]))));
+        m = QUADS == 1 ? half_wave_max(m) : row16_max(m);
+    }
     return m;
+}
+__device__ __forceinline__ float half_wave_amax(float a, float b, float c, float d) {
+    const float v[1][4] = {{a, b, c, d}};
+    return block_amax<1>(v);
 }
 
 }  // namespace siren

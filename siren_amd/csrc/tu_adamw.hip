@@ -27,8 +27,6 @@ namespace siren {
 
 namespace {
 
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
 constexpr int CHUNK = 2048;       // elements of one tensor that a workgroup takes at a time: 16 scale blocks
 constexpr int NORM_THREADS = 512;
 

@@ -9,7 +9,7 @@
 // column sums of a bias's gradient on the way, so the tensor is read once. 64 values a thread: 16 rows x 4 columns, so
 // a row's maximum is a reduction over half a wave, a column's one over LDS, and the transpose leaves as 16-byte pieces.
 // Bytes bound it: 262144 x 1024 fp32 into both layouts 301 us (1.6 GB, 5.3 TB/s), bf16 214 us (5.0 TB/s; a bf16 value costs
-// the same instructions for half the bytes); rows alone 224 us from fp32 (6.0 TB/s).
+// the same instructions for half the bytes); rows alone 225 us from fp32 (6.0 TB/s).
 #include "fp8.h"
 #include "fp8_device.h"
 #include "siren_common.h"
@@ -275,38 +275,60 @@ __global__ __launch_bounds__(256, 4) void quant_kernel(QuantArgs a, QuantArgs b,
     }
 }
 
-// Rows alone, nothing transposed (a layer that is only evaluated): half a wave takes one block of a row, a workgroup one
-// block of 32 rows, 4 a half wave, all loaded before any is reduced. A few rows are a matter of latency here (the tile
-// kernel above is thousands of instructions long, 8 us for one row), many one of bytes.
-constexpr int ROWS_PER_GROUP = 32;
+// Rows alone, nothing transposed (a layer that is only evaluated): 16 bytes a lane, so half a wave (a quarter, of 16-bit
+// values) takes one block of a row, and a workgroup one block of 32 (64) rows, 4 a unit, all loaded before any is reduced. A few
+// rows are a matter of latency here (the tile kernel above is thousands of instructions long, 8 us for one row), many one of
+// bytes: 16384 x 1024 bf16 11 us (4.5 TB/s), 262144 x 1024 fp32 226 us (5.9 TB/s).
+template <typename T>
+constexpr int ROW_LANES = sizeof(T) == 4 ? 32 : 16;
+template <typename T>
+constexpr int ROWS_PER_GROUP = 4 * 256 / ROW_LANES<T>;
 template <typename T, bool E5M2>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
                                                          uint8_t* __restrict__ q, uint8_t* __restrict__ s,
                                                          int col_blocks, int panels) {
-    const int c4 = threadIdx.x & 31, unit = threadIdx.x >> 5;
+    constexpr int LANES = ROW_LANES<T>, QUADS = 32 / LANES, UNITS = 256 / LANES;
+    const int lane = threadIdx.x & (LANES - 1), unit = threadIdx.x / LANES;
     const int64_t rb = blockIdx.x / col_blocks;
     const int cb = (int)(blockIdx.x % col_blocks);
-    const int64_t c0 = (int64_t)cb * QT + c4 * 4;
-    const int64_t left = cols - c0;
-    const int valid = left < 4 ? (left > 0 ? (int)left : 0) : 4;
+    const int col = lane * 4 * QUADS;  // in the block
+    const int64_t c0 = (int64_t)cb * QT + col;
     const int64_t s_ld = (col_blocks + 3) / 4 * 4;
-    float v[4][4];
+    float v[4][QUADS][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t r = rb * ROWS_PER_GROUP + i * 8 + unit;
-        load_quad(x + (r < rows ? r : rows - 1) * ld + c0, valid, v[i]);
+        const int64_t r = rb * ROWS_PER_GROUP<T> + i * UNITS + unit;
+        const T* src = x + (r < rows ? r : rows - 1) * ld + c0;
+        if (QUADS == 2 && c0 + 8 <= cols) {
+            typedef T Oct __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+            const Oct h = *(const Oct*)src;
+#pragma unroll
+            for (int k = 0; k < 4 * QUADS; ++k) v[i][k >> 2][k & 3] = (float)h[k];
+        } else {
+#pragma unroll
+            for (int d = 0; d < QUADS; ++d) {
+                const int64_t left = cols - c0 - 4 * d;
+                load_quad(src + 4 * d, left < 4 ? (left > 0 ? (int)left : 0) : 4, v[i][d]);
+            }
+        }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t r = rb * ROWS_PER_GROUP + i * 8 + unit;
-        const int byte = exponent_byte<E5M2>(half_wave_amax(v[i][0], v[i][1], v[i][2], v[i][3]));
+        const int64_t r = rb * ROWS_PER_GROUP<T> + i * UNITS + unit;
+        const int byte = exponent_byte<E5M2>(block_amax<QUADS>(v[i]));
         if (r < rows) {
-            uint8_t* dst = (panels & 1) ? q + ((cb * 2 + (c4 >> 4)) * rows + r) * 64 + (c4 & 15) * 4
-                                  : q + r * ((int64_t)col_blocks * QT) + c0;
-            *(uint32_t*)dst = pack4<E5M2>(v[i][0], v[i][1], v[i][2], v[i][3], scale_of(byte));
+            uint32_t* dst = (uint32_t*)((panels & 1) ? q + ((cb * 2 + (col >> 6)) * rows + r) * 64 + (col & 63)
+                                                     : q + r * ((int64_t)col_blocks * QT) + c0);
+            uint32_t w[QUADS];
+#pragma unroll
+            for (int d = 0; d < QUADS; ++d) w[d] = pack4<E5M2>(v[i][d][0], v[i][d][1], v[i][d][2], v[i][d][3], scale_of(byte));
+            if constexpr (QUADS == 2)
+                *(u32x2*)dst = u32x2{w[0], w[1]};
+            else
+                *dst = w[0];
             // the pad bytes of a row's last word stand for 1
-            if (c4 == 0) s[r * s_ld + cb] = (uint8_t)byte;
-            if (cb == col_blocks - 1 && c4 > 0 && cb + c4 < s_ld) s[r * s_ld + cb + c4] = 127;
+            if (lane == 0) s[r * s_ld + cb] = (uint8_t)byte;
+            if (cb == col_blocks - 1 && lane > 0 && cb + lane < s_ld) s[r * s_ld + cb + lane] = 127;
         }
     }
 }
@@ -373,7 +395,8 @@ void launch_tiles(hipStream_t stream, const Fp8Quant& a, const Fp8Quant* b) {
 void launch_fp8_quant(hipStream_t stream, const Fp8Quant& a) {
     if (!rows_only(a)) return launch_tiles(stream, a, nullptr);
     const int col_blocks = (int)fp8_blocks(a.cols);
-    const int64_t groups = (a.rows + ROWS_PER_GROUP - 1) / ROWS_PER_GROUP * col_blocks;
+    const int per = a.type == FP8_F32 ? ROWS_PER_GROUP<float> : ROWS_PER_GROUP<__bf16>;
+    const int64_t groups = (a.rows + per - 1) / per * col_blocks;
 #define SIREN_QUANT_ROWS(T, E)                                                                                           \
     hipLaunchKernelGGL((quant_rows_kernel<T, E>), dim3((unsigned)groups), dim3(256), 0, stream, (const T*)a.x, a.ld, a.rows, \
                        a.cols, a.q, a.s, col_blocks, a.panels)

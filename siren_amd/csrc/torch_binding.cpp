@@ -108,7 +108,8 @@ Blocks plan(int64_t rows, int64_t cols, int layout, int fmt = 0) {
 }
 
 // x as the kernels read it: columns one element apart, rows any distance that does not overlap
-Tensor rows_of(const Tensor& x, int64_t& ld) {
+Tensor rows_of(const Tensor& x0, int64_t& ld) {
+    const Tensor x = x0.is_neg() ? x0.resolve_neg() : x0;  // what a view negates is not so in memory
     const int64_t r = x.size(0), c = x.size(1);
     Tensor y = (c <= 1 || x.stride(1) == 1) && (r <= 1 || x.stride(0) >= c) ? x : x.contiguous();
     ld = r > 1 ? y.stride(0) : c;
@@ -185,7 +186,11 @@ Tensor serve(const Tensor& x0, const Blocks& w, const Tensor& bias, int act, dou
     return y;
 }
 
-Tensor bias32(const Tensor& bias) { return bias.defined() ? bias.detach().to(at::kFloat).contiguous() : bias; }
+Tensor bias32(const Tensor& bias) {
+    if (!bias.defined()) return bias;
+    const Tensor b = bias.detach();
+    return (b.is_neg() ? b.resolve_neg() : b).to(at::kFloat).contiguous();
+}
 
 // Gradients of gradients: the values pass, a backward through them says why there is none
 struct NotTwice : torch::autograd::Function<NotTwice> {
@@ -216,7 +221,7 @@ void check_capture(std::initializer_list<const Tensor*> leaves) {
 struct LinearBackward : torch::autograd::Node {
     int64_t m = 0, n = 0, k = 0, fmt = 0, kept_bytes = 0;
     at::ScalarType tx = at::kFloat, tw = at::kFloat, tb = at::kFloat;
-    Blocks qxt, qwt;                               // x and the weight by their columns, in kept's memory
+    Blocks qxt, qwt;                             // x and the weight by their columns, in kept's memory
     torch::autograd::SavedVariable kept, deriv;  // saved as torch saves, so that its hooks (checkpointing) see them
 
     std::string name() const override { return "Fp8LinearBackward"; }
@@ -467,7 +472,8 @@ MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Mayb
         types[i] = type_code(p.scalar_type());
         TORCH_CHECK(types[i] >= 0 && p.device() == dev, "adamw_step needs fp32, bf16 or fp16 parameters on one device; got ",
                     p.scalar_type(), " on ", p.device());
-        TORCH_CHECK_VALUE(p.is_contiguous(), "adamw_step needs contiguous parameters; parameter ", i, " has strides ", p.strides());
+        TORCH_CHECK_VALUE(p.is_contiguous() && !p.is_neg(), "adamw_step needs contiguous parameters; parameter ", i,
+                          " has strides ", p.strides(), p.is_neg() ? " and is a negated view" : "");
         ps[i] = p.data_ptr();
         gs[i] = nullptr;
         if (grads[i]) {
@@ -476,10 +482,10 @@ MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Mayb
                                   g.device() == dev,
                               "gradient ", i, " must be ", p.sizes(), " ", p.scalar_type(), " on ", dev, "; got ", g.sizes(), " ",
                               g.scalar_type(), " on ", g.device());
-            if (g.is_contiguous()) {
+            if (g.is_contiguous() && !g.is_neg()) {
                 gs[i] = g.data_ptr();
             } else {
-                keep.push_back(g.contiguous());
+                keep.push_back(g.resolve_neg().contiguous());
                 gs[i] = keep.back().data_ptr();
             }
         }

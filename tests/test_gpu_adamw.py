@@ -416,3 +416,15 @@ def test_tensors_at_any_address(cuda, bits, dtype):
             assert bool((h[:shift] == 7).all()) and bool((h[shift + p.numel():] == 7).all())
         out.append(torch.cat([p.float() for p in ps] + [opt.exp_avg.float(), opt.exp_avg_sq.float()]))
     assert all(torch.equal(o, out[0]) for o in out)
+
+
+def test_negated_views(cuda):
+    from siren_amd import optim
+    p, g = torch.randn(300, device=cuda), torch.randn(300, device=cuda)
+    a, b = p.clone(), p.clone()
+    for q, grad in ((a, torch._neg_view(g)), (b, -g)):
+        opt = optim.FusedAdamW([q])
+        optim.adamw_step([q], [grad], opt.exp_avg, opt.exp_avg_sq, opt.steps)
+    assert torch.equal(a, b) and not torch.equal(a, p)
+    with pytest.raises(ValueError, match='negated'):
+        optim.adamw_step([torch._neg_view(p)], [g], opt.exp_avg, opt.exp_avg_sq, opt.steps)

@@ -606,3 +606,20 @@ def test_few_rows_of_long_sums(cuda, m, k, n):
     assert y.dtype is torch.bfloat16 and torch.equal(y, want.float().bfloat16())
     plain = fp8.matmul(fp8.quantize(x), w8, b, 'sine', omega=0.01)
     assert torch.equal(fp8.linear(x, w8, b, 'sine', omega=0.01), plain)
+
+
+def test_negated_views(cuda):
+    """A view that torch negates on reading (of a conjugate's imaginary part) counts with its sign."""
+    from siren_amd import fp8
+    x, w, b = torch.randn(40, 130, device=cuda), torch.randn(70, 130, device=cuda), torch.randn(70, device=cuda)
+    neg = [torch._neg_view(t) for t in (x, w, b)]
+    assert all(t.is_neg() for t in neg)
+    for rows in (3, 40):
+        assert torch.equal(fp8.linear(neg[0][:rows], neg[1], neg[2]), fp8.linear(-x[:rows], -w, -b))
+        leaves = [t.detach().requires_grad_(True) for t in (neg[0][:rows], neg[1], neg[2])]
+        plain = [t.clone().requires_grad_(True) for t in (-x[:rows], -w, -b)]
+        dy = torch.randn(rows, 70, device=cuda)
+        got = torch.autograd.grad(fp8.linear(*leaves, 'sine'), leaves, torch._neg_view(dy))
+        want = torch.autograd.grad(fp8.linear(*plain, 'sine'), plain, -dy)
+        assert all(torch.equal(g, v) for g, v in zip(got, want))
+    assert torch.equal(fp8.dequantize(fp8.quantize(neg[0])), fp8.dequantize(fp8.quantize(-x)))

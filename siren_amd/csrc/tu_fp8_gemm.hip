@@ -45,7 +45,8 @@ struct GemmArgs {
     int tiles_m, tiles_n;
     const float* bias;
     int act;
-    float omega;
+    float omega, turn, turn_low;  // turns = omega / 2 pi, in 32 bits and what they leave
+    double turns;
     void* out;                   // split: fp32 partial products (splits, m, n)
     __bf16* deriv;
 };
@@ -75,27 +76,27 @@ __device__ __forceinline__ void put4(T* dst, f32x4 v, int valid, bool once) {
     }
 }
 
-constexpr float EXACT_PHASE = 1.0e5f;  // past this sincos_fast's reduction is not exact
+constexpr float MANY_TURNS = 4194304.f;  // 2^22: beyond, fp32 holds no whole number of turns and a fraction
 
-// Four phases in turns, for v_sin_f32 and v_cos_f32 (sincos_fast's reduction; to 4e-7 of the sine). One past EXACT_PHASE has
-// its turns taken in 64 bits (an fp32 phase over 1e9 is itself off by turns): in a branch that the wave takes if any lane has
-// one, where the others keep their result, so that no output depends on its neighbours. Chosen for each element, the 64-bit
-// steps were issued whether a lane needed them or not (262144 x 1024 x 1024 with the sine 692 us, now 670).
-__device__ __forceinline__ f32x4 turns4(const f32x4& t) {
+// The phases omega z of four z, in turns, for v_sin_f32 and v_cos_f32: z (omega / 2 pi) less its whole turns, by fused steps
+// with the factor in two parts, so that neither omega z nor the product is rounded on the way. Of phases past MANY_TURNS the
+// fraction is taken in 64 bits: in a branch that the wave takes if any lane has one, where the others keep their result, so that
+// no output depends on its neighbours. Chosen for each element, the 64-bit steps were issued whether a lane needed them or not
+// (262144 x 1024 x 1024 with the sine 692 us, 670 then; 16384 x 1024 x 1024 bf16 40.2 with the phase first, 38.9).
+__device__ __forceinline__ f32x4 turns4(const f32x4& z, const GemmArgs& g) {
     f32x4 u;
     float most = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const float q = __builtin_rintf(t[k] * 0.159154943091895336f);
-        const float r = __builtin_fmaf(-q, 6.28318548202514648f, t[k]);
-        u[k] = __builtin_fmaf(-q, -1.74845553146951e-7f, r) * 0.159154943091895336f;
-        most = fmaxf(most, __builtin_fabsf(t[k]));
+        const float q = __builtin_rintf(z[k] * g.turn);
+        u[k] = __builtin_fmaf(z[k], g.turn_low, __builtin_fmaf(z[k], g.turn, -q));
+        most = fmaxf(most, __builtin_fabsf(q));
     }
-    if (__builtin_expect(__any(most > EXACT_PHASE), 0)) {
+    if (__builtin_expect(__any(most > MANY_TURNS), 0)) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float w = (float)__builtin_amdgcn_fract((double)t[k] * 0.15915494309189533577);
-            u[k] = __builtin_fabsf(t[k]) > EXACT_PHASE ? w : u[k];
+            const float w = (float)__builtin_amdgcn_fract((double)z[k] * g.turns);
+            u[k] = __builtin_fabsf(z[k] * g.turn) > MANY_TURNS ? w : u[k];
         }
     }
     return u;
@@ -118,7 +119,7 @@ struct Finish {
     __device__ __forceinline__ void store(const GemmArgs& g, int64_t row, f32x4 v) const {
         v += bias;
         if (g.act == FP8_ACT_SINE) {
-            const f32x4 u = turns4(g.omega * v);
+            const f32x4 u = turns4(v, g);
             if (g.deriv != nullptr) {
                 f32x4 d;
 #pragma unroll
@@ -131,6 +132,13 @@ struct Finish {
         put4((T*)g.out + row * g.n + col, v, valid, once);
     }
 };
+
+void set_omega(GemmArgs& g, float omega) {
+    g.omega = omega;
+    g.turns = (double)omega * 0.15915494309189533577;
+    g.turn = (float)g.turns;
+    g.turn_low = (float)(g.turns - (double)g.turn);
+}
 
 // The products of one half block (64 k) of a wave's RT x 2 tiles of 32 x 32, bytes to bf16 and scaled on the way, in four
 // slices of 16 k: the next slice's widening (3 instructions a product at RT = 4) stands beside this one's products. (Placing
@@ -596,7 +604,7 @@ void launch_fp8_few_rows(hipStream_t stream, const void* x, int type, int64_t ld
     f.out.n = n;
     f.out.bias = bias;
     f.out.act = act;
-    f.out.omega = omega;
+    set_omega(f.out, omega);
     f.out.out = y;
     f.out.deriv = (__bf16*)deriv;
     // 32 columns a wave where that still is a workgroup a CU: half the rounding of x. A long k whose columns fill fewer CUs is
@@ -647,7 +655,7 @@ void launch_fp8_product(hipStream_t stream, const Fp8Product& p) {
     g.halves = (int)((p.k + HK - 1) / HK);
     g.bias = p.bias;
     g.act = p.act;
-    g.omega = p.omega;
+    set_omega(g, p.omega);
     g.deriv = (__bf16*)p.deriv;
     const Plan plan = plan_of(g.m, g.n, p.k);
     const int splits = plan.splits;

@@ -96,7 +96,7 @@ __device__ __forceinline__ f32x4 turns4(const f32x4& z, const GemmArgs& g) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float w = (float)__builtin_amdgcn_fract((double)z[k] * g.turns);
-            u[k] = __builtin_fabsf(z[k] * g.turn) > MANY_TURNS ? w : u[k];
+            u[k] = __builtin_fabsf(__builtin_rintf(z[k] * g.turn)) > MANY_TURNS ? w : u[k];  // as above: by its own turns
         }
     }
     return u;

@@ -623,3 +623,24 @@ def test_negated_views(cuda):
         want = torch.autograd.grad(fp8.linear(*plain, 'sine'), plain, -dy)
         assert all(torch.equal(g, v) for g, v in zip(got, want))
     assert torch.equal(fp8.dequantize(fp8.quantize(neg[0])), fp8.dequantize(fp8.quantize(-x)))
+
+
+def test_sine_at_any_phase(cuda):
+    """sin(omega z) of phases from none to 1e12, each exact in its own 32 bits, and no row's result by its neighbours'."""
+    from siren_amd import fp8
+    omega, n = 30., 64
+    w = torch.zeros(n, 128, device=cuda)
+    w8 = fp8.quantize(w, 'tile')
+    edge = 2. ** 22 * 2 * math.pi / omega
+    bias = torch.cat([torch.logspace(-6, 10.5, 40, dtype=torch.float64), edge * (1 + torch.linspace(-3e-7, 3e-7, 24).double())])
+    bias = bias.float().to(cuda)
+    x = torch.zeros(70, 128, device=cuda)
+    for m in (1, 20, 70):
+        y = fp8.linear(x[:m], w8, bias, 'sine', omega=omega)
+        want = np.sin(np64(bias) * omega)
+        # v_sin_f32's own error and the turns' last bit (2^-24 of a turn); past 2^22 turns, 2^-53 of the product in 64 bits
+        turns = np.abs(np64(bias)) * omega / (2 * math.pi)
+        tol = 1e-6 + 2 * math.pi * (turns * 2. ** -52)
+        assert (np.abs(np64(y) - want) <= tol).all()
+    alone = torch.cat([fp8.linear(x[:1], fp8.quantize(w[i:i + 1], 'tile'), bias[i:i + 1], 'sine', omega=omega) for i in range(n)], 1)
+    assert torch.equal(alone, fp8.linear(x[:1], w8, bias, 'sine', omega=omega))

@@ -448,7 +448,8 @@ typedef struct siren_fp8_source {
 } siren_fp8_source;
 int32_t siren_fp8_quantize_sources(const siren_fp8_source* src, int32_t count, void* stream);
 
-/* out (m, n) = act(a b^T + bias) of a (m, k) and b (n, k) quantised along k (k < 2^24, n < 2^22), sums in 32 bits.
+/* out (m, n) = act(a b^T + bias) of a (m, k) and b (n, k) quantised along k, sums in 32 bits. k <= 2^24 - 128 (rounded up to
+ * a multiple of 128 it stays below 2^24), n < 2^22.
  * a may be e4m3 or e5m2, b is e4m3. act 0: none, 1: sin(omega z), with deriv (m, n) bf16, nullable, = omega cos(omega z).
  * bias (n) fp32, nullable. ws: siren_fp8_matmul_ws_bytes(m, n, k) bytes. */
 int32_t siren_fp8_matmul_ws_bytes(int64_t m, int64_t n, int64_t k, int64_t* bytes);

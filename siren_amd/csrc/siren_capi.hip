@@ -1668,9 +1668,9 @@ int check_fp8_type(int32_t dtype) {
     return dtype >= siren::FP8_F32 && dtype <= siren::FP8_F16 ? SIREN_OK : fail(SIREN_EINVAL, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
 }
 int check_fp8_product(int64_t m, int64_t n, int64_t k) {
-    // the kernels address a tile's 256 rows by 32-bit offsets
-    if (m < 0 || n < 0 || k < 1 || siren::fp8_padded(k) > 0xFFFFFFFFll / 256 || n >= 1 << 22)
-        return fail(SIREN_EINVAL, "fp8 product: need m >= 0, 0 <= n < 2^22 and 1 <= k < 2^24");
+    // the kernels address a tile's 256 rows, of k rounded up to 128 bytes, by 32-bit offsets
+    if (m < 0 || n < 0 || k < 1 || k > (1 << 24) - 128 || n >= 1 << 22)
+        return fail(SIREN_EINVAL, "fp8 product: need m >= 0, 0 <= n < 2^22 and 1 <= k <= 2^24 - 128");
     if (siren::fp8_blocks(m) > kMaxGrid / std::max<int64_t>(1, siren::fp8_blocks(n)))
         return fail(SIREN_EINVAL, "fp8 product: too many tiles");
     return SIREN_OK;

@@ -276,6 +276,15 @@ struct LinearBackward : torch::autograd::Node {
     }
 };
 
+// The backward's products have limits of their own (a sum's length is the forward's rows or outputs, a result's columns its
+// inputs): a layer whose gradients the library would refuse is refused before its forward
+void check_backward(const Tensor& x, const Tensor& weight) {
+    const int64_t m = x.size(0), n = weight.size(0), k = weight.size(1);
+    int64_t bytes;
+    if (m > 0 && x.requires_grad()) check(lib.matmul_ws_bytes(m, k, n, &bytes), "fp8.linear: the gradient of x");
+    if (m > 0 && weight.requires_grad()) check(lib.matmul_ws_bytes(n, k, m, &bytes), "fp8.linear: the gradient of the weight");
+}
+
 // y = act(x W^T + b) with gradients
 Tensor train(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t act, double omega, int64_t fmt) {
     const bool nx = x.requires_grad(), nw = weight.requires_grad();
@@ -439,8 +448,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& maybe_bi
     TORCH_CHECK_VALUE(weight.device() == x.device(), "weight on ", weight.device(), " but x on ", x.device());
     const Tensor x2 = check_layer(x, bias, weight.size(0), weight.size(1), omega);
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()))) {
-        TORCH_CHECK_VALUE(!weight.requires_grad() || x2.size(0) < (1 << 24), "a weight's gradient sums over fewer than 2^24 rows; got ",
-                          x2.size(0));
+        check_backward(x2, weight);
         check_capture({&x, &weight, &bias});
         return like_input(x, train(x2, weight, bias, act, omega, fmt));
     }

@@ -644,3 +644,30 @@ def test_sine_at_any_phase(cuda):
         assert (np.abs(np64(y) - want) <= tol).all()
     alone = torch.cat([fp8.linear(x[:1], fp8.quantize(w[i:i + 1], 'tile'), bias[i:i + 1], 'sine', omega=omega) for i in range(n)], 1)
     assert torch.equal(alone, fp8.linear(x[:1], w8, bias, 'sine', omega=omega))
+
+
+def test_a_layer_whose_backward_would_not_fit_is_refused_at_once(cuda):
+    """dx and dW have the layer's inputs as their columns (fewer than 2^22), dW the rows as its sum (2^24 - 128 at most): the
+    forward of what a gradient would be refused for is refused, that of a layer without those gradients is not."""
+    from siren_amd import fp8
+    k = 1 << 22
+    x, w = torch.ones(1, k, device=cuda), torch.zeros(1, k, device=cuda)
+    w[0, :5] = 1.
+    assert fp8.linear(x, w).tolist() == [[5.]]
+    for a, b in ((x.clone().requires_grad_(True), w), (x, w.clone().requires_grad_(True))):
+        with pytest.raises(ValueError, match='gradient'):
+            fp8.linear(a, b)
+    b = torch.ones(1, device=cuda, requires_grad=True)
+    y = fp8.linear(x, w, b)  # a bias's gradient alone has no such product
+    assert torch.autograd.grad(y.sum(), b)[0].tolist() == [1.]
+    # one input less: a result of 2^22 - 1 columns, exact in ones
+    leaves = [x[:, 1:].clone().requires_grad_(True), w[:, 1:].clone().requires_grad_(True)]
+    dx, dw = torch.autograd.grad(fp8.linear(*leaves).sum(), leaves)
+    assert torch.equal(dx, leaves[1].detach()) and torch.equal(dw, leaves[0].detach())
+    rows, w = (1 << 24) - 128, torch.ones(1, 1, device=cuda, requires_grad=True)
+    x = torch.ones(rows + 1, 1, device=cuda)
+    with pytest.raises(ValueError, match='gradient of the weight'):
+        fp8.linear(x, w)
+    assert bool((fp8.linear(x, w.detach()) == 1).all())
+    y = fp8.linear(x[:rows], w)
+    assert torch.autograd.grad(y, w, torch.ones_like(y))[0].tolist() == [[float(rows)]]  # whole numbers below 2^24

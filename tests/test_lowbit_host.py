@@ -152,3 +152,14 @@ def test_modules_take_the_precision():
     assert [l[0].precision for l in FCBlock(2, 1, 1, 64, nonlinearity='relu').net] == ['fp32'] * 3
     with pytest.raises(ValueError):
         SingleBVPNet(precision='fp4', verbose=False)
+
+
+def test_longest_sums(lib):
+    """The longest sum is 2^24 - 128: a tile's 256 rows of k bytes, rounded up to 128, are addressed by 32-bit offsets. A
+    result has fewer than 2^22 columns. The refusal names the bound that it enforces."""
+    c = ctypes.c_int64(0)
+    for fn in (lib.siren_fp8_matmul_ws_bytes, lib.siren_fp8_linear_ws_bytes):
+        assert fn(4, 4, (1 << 24) - 128, ctypes.byref(c)) == OK and fn(4, (1 << 22) - 1, 8, ctypes.byref(c)) == OK
+        for bad in ((4, 4, (1 << 24) - 127), (4, 4, (1 << 24) - 1), (4, 1 << 22, 8)):
+            assert fn(*bad, ctypes.byref(c)) == EINVAL, bad
+            assert b'2^24 - 128' in lib.siren_last_error() and b'2^22' in lib.siren_last_error()

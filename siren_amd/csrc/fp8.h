@@ -9,7 +9,7 @@ namespace siren {
 enum Fp8Type : int { FP8_F32 = 0, FP8_BF16 = 1, FP8_F16 = 2 };  // types of unquantised tensors
 enum Fp8Act : int { FP8_ACT_NONE = 0, FP8_ACT_SINE = 1 };
 
-inline int64_t fp8_blocks(int64_t n) { return (n + 127) / 128; }
+inline int64_t fp8_blocks(int64_t n) { return n / 128 + (n % 128 != 0); }  // of any n >= 0: no sum to overflow
 inline int64_t fp8_padded(int64_t n) { return fp8_blocks(n) * 128; }            // bytes of a quantised row
 inline int64_t fp8_scale_cols(int64_t n) { return (fp8_blocks(n) + 3) / 4 * 4; }  // scale bytes of a row: whole words
 

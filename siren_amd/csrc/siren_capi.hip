@@ -1839,8 +1839,8 @@ int32_t siren_adamw_step(int64_t count, void* const* params, const void* const* 
         if (numels[i] > 0 && (params[i] == nullptr || !aligned(params[i], size) || !aligned(grads[i], size)))
             return fail(SIREN_EINVAL, "siren_adamw_step: a parameter is NULL or not aligned to its type");
         total += siren::fp8_blocks(numels[i]);
+        if (total > 0xFFFFFFFFll) return fail(SIREN_EINVAL, "siren_adamw_step: more than 2^32 blocks of state");
     }
-    if (total > 0xFFFFFFFFll) return fail(SIREN_EINVAL, "siren_adamw_step: more than 2^32 blocks of state");
     if (total > 0 && (exp_avg == nullptr || exp_avg_sq == nullptr || !aligned(exp_avg, 16) || !aligned(exp_avg_sq, 16) ||
                       (state_bits == 8 && (scale_avg == nullptr || scale_avg_sq == nullptr))))
         return fail(SIREN_EINVAL, "siren_adamw_step: states must be 16-byte aligned, 8-bit ones with their scales");

@@ -163,3 +163,20 @@ def test_longest_sums(lib):
         for bad in ((4, 4, (1 << 24) - 127), (4, 4, (1 << 24) - 1), (4, 1 << 22, 8)):
             assert fn(*bad, ctypes.byref(c)) == EINVAL, bad
             assert b'2^24 - 128' in lib.siren_last_error() and b'2^22' in lib.siren_last_error()
+
+
+@pytest.mark.parametrize('n', [(1 << 63) - 1, (1 << 63) - 60, (1 << 63) - 128, 1 << 62, 1 << 56])
+def test_sizes_at_the_end_of_64_bits(lib, n):
+    """No size wraps on its way to a check: each is refused."""
+    c = ctypes.c_int64(-7)
+    for fn in (lib.siren_fp8_matmul_ws_bytes, lib.siren_fp8_linear_ws_bytes):
+        for size in ((n, 4, 4), (4, n, 4), (4, 4, n), (n, n, n)):
+            assert fn(*size, ctypes.byref(c)) == EINVAL and c.value == -7, size
+    for rows, cols in ((n, 4), (4, n), (n, n)):
+        assert lib.siren_fp8_quantize(P(64), 0, rows, cols, cols, None, 0, 0, 0, P(64), P(64), None, None, None, None, None) == EINVAL
+        assert lib.siren_fp8_quantize(P(64), 0, rows, cols, cols, None, 0, 0, 0, P(64), P(64), P(64), P(64), P(64), P(64),
+                                      None) == EINVAL
+    many = 300  # their blocks' sum does not wrap either
+    ps, ns, ts = (P * many)(*[64] * many), (ctypes.c_int64 * many)(*[n] * many), (ctypes.c_int32 * many)()
+    assert lib.siren_adamw_step(many, ps, ps, ns, ts, 32, P(64), P(64), None, None, P(64), 1e-3, .9, .99, 1e-8, 0., 0., 0, P(64),
+                                None) == EINVAL

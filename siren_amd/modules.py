@@ -165,15 +165,19 @@ PRECISIONS = ('fp32', 'bf16x6', 'fp8')
 FP8_MIN_FEATURES = 64  # a layer with fewer inputs or outputs stays in fp32: coordinates need their bits, and bytes save nothing
 
 
-def _fp8_sine_apply(coords, weights_biases, outermost_linear):
-    """A sine network with its hidden products in 8 bits (fp8.linear with the sine in its epilogue), activations between
-    them in bf16 (8 bits of mantissa for values that the next layer rounds to 4). The first layer, and a last one with
-    fewer than FP8_MIN_FEATURES outputs, are plain fp32. Trains on values; its gradients are not differentiable again."""
+def _check_fp8_network(coords, weights_biases):
     if coords.device.type != 'cuda':
         raise RuntimeError('siren_amd runs on ROCm devices (MI355X) only; move the model and coords to "cuda". '
                            'The CPU restatement of the reference lives in oracle/ (test infrastructure).')
     if any(W.dim() != 2 for W, _ in weights_biases):
         raise _lib.SirenUnsupported("precision='fp8' takes unbatched weights")
+
+
+def _fp8_sine_apply(coords, weights_biases, outermost_linear):
+    """A sine network with its hidden products in 8 bits (fp8.linear with the sine in its epilogue), activations between
+    them in bf16 (8 bits of mantissa for values that the next layer rounds to 4). The first layer, and a last one with
+    fewer than FP8_MIN_FEATURES outputs, are plain fp32. Trains on values; its gradients are not differentiable again."""
+    _check_fp8_network(coords, weights_biases)
     a = coords
     for i, (W, b) in enumerate(weights_biases):
         last = i == len(weights_biases) - 1
@@ -184,6 +188,37 @@ def _fp8_sine_apply(coords, weights_biases, outermost_linear):
             z = nn.functional.linear(a.float(), W, b)
             a = torch.sin(30 * z) if sine else z
     return a.float()
+
+
+class _SineOfPhase(torch.autograd.Function):
+    """y and its derivative d with respect to z as the layer's kernel computes them, both bf16, as a function of z in fp32; the
+    gradient of y has y's type in the network."""
+
+    @staticmethod
+    def forward(ctx, z, y, d):
+        ctx.save_for_backward(d)
+        return y.float()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return g.to(torch.bfloat16).float() * ctx.saved_tensors[0].float().view(g.shape), None, None
+
+
+def _fp8_sine_layer_activations(a, W, b, sine):
+    """One layer of _fp8_sine_apply with its phase z, which the kernel does not store: (z, its sine or None), the network's
+    own values in fp32. For looking at a network: three products where the network takes one."""
+    if min(W.shape) < FP8_MIN_FEATURES:
+        z = nn.functional.linear(a.float(), W, b)
+        return z, torch.sin(30 * z) if sine else None
+    h = a.to(torch.bfloat16)
+    if not sine:
+        return fp8.linear(h, W, b).float(), None
+    z = fp8.linear(h.float(), W, b)
+    with torch.no_grad():
+        y = fp8.linear(h, W, b, 'sine')
+        d = fp8.matmul(fp8.quantize(h.reshape(-1, W.shape[1])), fp8.quantize(W, 'tile'), b, 'sine', derivative=True)[1]
+    return z, _SineOfPhase.apply(z, y, d)
 
 
 def _fused_apply(engine, jet, coords, weights_biases, precision='fp32'):
@@ -313,16 +348,24 @@ class FCBlock(MetaModule):
         return _fused_apply(self._engine(), self._jet, coords, wb, self.precision)
 
     def forward_with_activations(self, coords, params=None, retain_grad=False):
-        """Per-layer activations (modules.py:96-116): a visualisation API, evaluated layer by layer in torch."""
+        """Per-layer activations (modules.py:96-116): a visualisation API, evaluated layer by layer in torch. Those of
+        precision='fp8' are the values that the 8-bit network computes, and their gradients its own."""
         if params is None:
             params = OrderedDict(self.named_parameters())
         activations = OrderedDict()
         x = coords.clone().detach().requires_grad_(True)
         activations['input'] = x
+        fp8_sine = self.precision == 'fp8' and self.nonlinearity == 'sine'
+        if fp8_sine:
+            _check_fp8_network(x, [(params['net.%d.0.weight' % i], None) for i in range(len(self.net))])
         for i, layer in enumerate(self.net):
             sub = get_subdict(params, 'net.%d' % i)
+            if fp8_sine:
+                pair = _fp8_sine_layer_activations(x, sub['0.weight'], sub.get('0.bias'), len(layer) > 1)
             for j, sublayer in enumerate(layer):
-                if isinstance(sublayer, BatchLinear):
+                if fp8_sine:
+                    x = pair[j]
+                elif isinstance(sublayer, BatchLinear):
                     x = sublayer(x, params=get_subdict(sub, '%d' % j))
                 else:
                     x = sublayer(x)

@@ -208,3 +208,42 @@ def test_captured_training_step_of_a_network(cuda):
         for p, q in zip(eager[0].parameters(), captured[0].parameters()):
             assert torch.equal(p, q)
         torch.randn(1000, device=cuda).sum().item()
+
+
+@pytest.mark.parametrize('kind', ['sine', 'relu'])
+@pytest.mark.parametrize('outer', [True, False])
+@pytest.mark.parametrize('rows,out', [(9, 3), (300, 3), (300, 70)])
+def test_activations_are_the_networks_own(cuda, kind, outer, rows, out):
+    """forward_with_activations shows the network that forward runs: the same last value, the sine of each phase, and (past
+    the 32 rows of the few-rows kernel, whose sums run in another order) the same gradients."""
+    from siren_amd.modules import FCBlock
+    torch.manual_seed(4)
+    made = dict(in_features=2, out_features=out, num_hidden_layers=2, hidden_features=128, outermost_linear=outer, nonlinearity=kind)
+    net = FCBlock(precision='fp8', **made).to(cuda)
+    x = torch.rand(1, rows, 2, device=cuda) * 2 - 1
+    acts = net.forward_with_activations(x, retain_grad=True)
+    values = list(acts.values())
+    assert list(acts) == list(FCBlock(**made).to(cuda).forward_with_activations(x))
+    leaf = x.clone().requires_grad_(True)
+    y = net(leaf)
+    assert torch.equal(values[-1], y)
+    if kind == 'sine':
+        for z, a in zip(values[1::2], values[2::2]):
+            assert ((a - torch.sin(30 * z)).abs() <= 2. ** -8 * a.abs() + 1e-5).all()  # held in bf16
+    dy = torch.randn_like(y)
+    values[-1].backward(dy)
+    got = [values[0].grad] + [p.grad for p in net.parameters()]
+    assert all(v.grad is not None and torch.isfinite(v.grad).all() for v in values)
+    if rows > 32:
+        want = torch.autograd.grad(y, [leaf] + list(net.parameters()), dy)
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_activations_of_an_8_bit_network_refuse_what_it_refuses(cuda):
+    from siren_amd._lib import SirenUnsupported
+    from siren_amd.modules import FCBlock
+    net = FCBlock(2, 3, 1, 64, outermost_linear=True, nonlinearity='sine', precision='fp8').to(cuda)
+    with pytest.raises(SirenUnsupported):
+        net.forward_with_activations(torch.zeros(1, 4, 2, device=cuda), params={k: v[None] for k, v in net.named_parameters()})
+    with pytest.raises(RuntimeError, match='ROCm'):
+        net.cpu().forward_with_activations(torch.zeros(1, 4, 2))

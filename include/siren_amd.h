@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define SIREN_ABI_VERSION 8
+#define SIREN_ABI_VERSION 9
 
 enum {
     SIREN_OK = 0,
@@ -479,6 +479,13 @@ int32_t siren_adamw_step(int64_t count, void* const* params, const void* const* 
                          const int32_t* dtypes, int32_t state_bits, void* exp_avg, void* exp_avg_sq, void* scale_avg,
                          void* scale_avg_sq, int64_t* step, double lr, double beta1, double beta2, double eps,
                          double weight_decay, double max_norm, uint64_t seed, void* scratch, void* stream);
+/* The same where gradients may be missing in some steps. counts: DEVICE int64 (count), the steps that each tensor has taken; one
+ * is added where a tensor has elements and a gradient, and t of the two bias corrections is the sum (torch.optim.AdamW's own
+ * per-tensor steps). The random rounding goes by step. counts NULL: the call above, t is step's for all. */
+int32_t siren_adamw_step_each(int64_t count, void* const* params, const void* const* grads, const int64_t* numels,
+                              const int32_t* dtypes, int32_t state_bits, void* exp_avg, void* exp_avg_sq, void* scale_avg,
+                              void* scale_avg_sq, int64_t* step, int64_t* counts, double lr, double beta1, double beta2,
+                              double eps, double weight_decay, double max_norm, uint64_t seed, void* scratch, void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,7 +11,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('SIREN_AMD_LIB', os.path.join(_HERE, 'libsiren_amd.so'))
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 # Error codes (include/siren_amd.h)
 SIREN_OK, SIREN_EINVAL, SIREN_EUNSUPPORTED, SIREN_EHIP = 0, 1, 2, 3
@@ -109,6 +109,8 @@ _SIGS = {
     'siren_adamw_scratch_bytes': [_I64, ctypes.POINTER(_I64)],
     'siren_adamw_step': [_I64, _P, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _F64, _F64, _F64, _F64, _F64, _F64,
                          ctypes.c_uint64, _P, _P],
+    'siren_adamw_step_each': [_I64, _P, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _F64, _F64, _F64, _F64, _F64, _F64,
+                              ctypes.c_uint64, _P, _P],
 }
 EXPORTED = ('siren_abi_version', 'siren_last_error') + tuple(_SIGS)
 
@@ -156,7 +158,7 @@ def native():
                               '`python -c "import __graft_entry__ as g; g.build()"`' % e) from e
         mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in
                   ('siren_last_error', 'siren_fp8_quantize_sources', 'siren_fp8_matmul_ws_bytes', 'siren_fp8_matmul',
-                   'siren_fp8_linear_ws_bytes', 'siren_fp8_linear', 'siren_adamw_scratch_bytes', 'siren_adamw_step')})
+                   'siren_fp8_linear_ws_bytes', 'siren_fp8_linear', 'siren_adamw_scratch_bytes', 'siren_adamw_step_each')})
         _native = mod
     return _native
 

@@ -5,7 +5,7 @@
 
 namespace siren {
 
-constexpr int ADAMW_TENSORS = 112;      // tensors a launch: 32 bytes each of the 4 KiB of kernel arguments
+constexpr int ADAMW_TENSORS = 104;      // tensors a launch: 36 bytes each of the 4 KiB of kernel arguments
 constexpr int ADAMW_NORM_BLOCKS = 512;  // workgroups (and partial sums) of one norm launch: 2 a CU
 constexpr int ADAMW_BLOCKS = 4096;      // workgroups of one update launch
 
@@ -25,6 +25,7 @@ struct AdamwCall {
     void *m, *v;
     uint8_t *sm, *sv;
     int64_t* step;
+    int64_t* counts;  // nullable: each tensor's own number of steps
     AdamwHyper h;
     void* scratch;
 };

@@ -1822,13 +1822,22 @@ int32_t siren_adamw_step(int64_t count, void* const* params, const void* const* 
                          const int32_t* dtypes, int32_t state_bits, void* exp_avg, void* exp_avg_sq, void* scale_avg,
                          void* scale_avg_sq, int64_t* step, double lr, double beta1, double beta2, double eps,
                          double weight_decay, double max_norm, uint64_t seed, void* scratch, void* stream) {
+    return siren_adamw_step_each(count, params, grads, numels, dtypes, state_bits, exp_avg, exp_avg_sq, scale_avg, scale_avg_sq, step,
+                                 nullptr, lr, beta1, beta2, eps, weight_decay, max_norm, seed, scratch, stream);
+}
+
+int32_t siren_adamw_step_each(int64_t count, void* const* params, const void* const* grads, const int64_t* numels,
+                              const int32_t* dtypes, int32_t state_bits, void* exp_avg, void* exp_avg_sq, void* scale_avg,
+                              void* scale_avg_sq, int64_t* step, int64_t* counts, double lr, double beta1, double beta2,
+                              double eps, double weight_decay, double max_norm, uint64_t seed, void* scratch, void* stream) {
     if (count < 0 || (state_bits != 8 && state_bits != 32))
         return fail(SIREN_EINVAL, "siren_adamw_step: need count >= 0 and state_bits 8 or 32");
     if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !std::isfinite(lr) ||
         !std::isfinite(weight_decay) || !std::isfinite(eps))
         return fail(SIREN_EINVAL, "siren_adamw_step: need 0 <= beta < 1, eps >= 0 and finite lr, weight_decay");
-    if (step == nullptr || scratch == nullptr || !aligned(step, 8) || !aligned(scratch, 16))
-        return fail(SIREN_EINVAL, "siren_adamw_step: step and scratch must be aligned device memory");
+    if (step == nullptr || scratch == nullptr || !aligned(step, 8) || !aligned(scratch, 16) || !aligned(counts, 8))
+        return fail(SIREN_EINVAL, "siren_adamw_step: step, counts and scratch must be aligned device memory");
+    if (count > 0xFFFFFFFFll) return fail(SIREN_EINVAL, "siren_adamw_step: more than 2^32 tensors");
     if (count > 0 && (params == nullptr || grads == nullptr || numels == nullptr || dtypes == nullptr))
         return fail(SIREN_EINVAL, "siren_adamw_step: NULL pointer");
     int64_t total = 0;
@@ -1856,6 +1865,7 @@ int32_t siren_adamw_step(int64_t count, void* const* params, const void* const* 
     c.sm = (uint8_t*)scale_avg;
     c.sv = (uint8_t*)scale_avg_sq;
     c.step = step;
+    c.counts = counts;
     c.h = siren::AdamwHyper{lr, beta1, beta2, max_norm > 0.0 ? max_norm : 0.0, (float)(1.0 - beta1), (float)beta2,
                             (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay), seed};
     c.scratch = scratch;

@@ -31,7 +31,7 @@ struct Library {
     decltype(&siren_fp8_linear_ws_bytes) linear_ws_bytes;
     decltype(&siren_fp8_linear) linear;
     decltype(&siren_adamw_scratch_bytes) adamw_scratch_bytes;
-    decltype(&siren_adamw_step) adamw_step;
+    decltype(&siren_adamw_step_each) adamw_step;
 } lib;
 
 void bind(const std::map<std::string, uintptr_t>& f) {
@@ -43,7 +43,7 @@ void bind(const std::map<std::string, uintptr_t>& f) {
     SIREN_BIND(linear_ws_bytes, "siren_fp8_linear_ws_bytes");
     SIREN_BIND(linear, "siren_fp8_linear");
     SIREN_BIND(adamw_scratch_bytes, "siren_adamw_scratch_bytes");
-    SIREN_BIND(adamw_step, "siren_adamw_step");
+    SIREN_BIND(adamw_step, "siren_adamw_step_each");
 #undef SIREN_BIND
 }
 
@@ -461,7 +461,8 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& maybe_bi
 
 MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<MaybeTensor>& grads, const Tensor& m, const Tensor& v,
                        const Tensor& step, double lr, double b1, double b2, double eps, double weight_decay,
-                       std::optional<double> max_norm, uint64_t seed, const MaybeTensor& sm, const MaybeTensor& sv) {
+                       std::optional<double> max_norm, uint64_t seed, const MaybeTensor& sm, const MaybeTensor& sv,
+                       const MaybeTensor& counts) {
     const size_t n = params.size();
     TORCH_CHECK_VALUE(n >= 1 && grads.size() == n, "adamw_step needs as many gradients as parameters, one at least; got ",
                       grads.size(), " and ", n);
@@ -517,6 +518,9 @@ MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Mayb
             TORCH_CHECK_VALUE(s->scalar_type() == at::kByte && s->numel() == size / 128 && s->device() == dev && s->is_contiguous(),
                               "scales must be two tensors of ", size / 128, " contiguous uint8 on ", dev);
     TORCH_CHECK_VALUE(step.scalar_type() == at::kLong && step.numel() == 1 && step.device() == dev, "step must be one int64 on ", dev);
+    TORCH_CHECK_VALUE(!counts || (counts->scalar_type() == at::kLong && counts->numel() == (int64_t)n && counts->device() == dev &&
+                                  counts->is_contiguous()),
+                      "counts must be ", n, " contiguous int64 on ", dev);
     TORCH_CHECK_VALUE(!max_norm || *max_norm > 0., "max_norm must be positive or None; got ", max_norm.value_or(0.));
     int64_t need = 0;
     check(lib.adamw_scratch_bytes((int64_t)n, &need), "siren_adamw_scratch_bytes");
@@ -527,7 +531,8 @@ MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Mayb
     for (size_t i = 0; i < n; ++i)
         if (gs[i]) torch::autograd::impl::bump_version(params[i]);
     check(lib.adamw_step((int64_t)n, ps.data(), gs.data(), numels.data(), types.data(), sm ? 8 : 32, m.data_ptr(), v.data_ptr(),
-                         sm ? sm->data_ptr() : nullptr, sv ? sv->data_ptr() : nullptr, step.data_ptr<int64_t>(), lr, b1, b2, eps,
+                         sm ? sm->data_ptr() : nullptr, sv ? sv->data_ptr() : nullptr, step.data_ptr<int64_t>(),
+                         counts ? counts->data_ptr<int64_t>() : nullptr, lr, b1, b2, eps,
                          weight_decay, max_norm.value_or(0.), seed, scratch.data_ptr(), stream_of(step)),
           "siren_adamw_step");
     return max_norm ? MaybeTensor(scratch.select(0, 8)) : std::nullopt;

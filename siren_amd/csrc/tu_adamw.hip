@@ -29,11 +29,17 @@ namespace {
 
 constexpr int CHUNK = 2048;       // elements of one tensor that a workgroup takes at a time: 16 scale blocks
 constexpr int NORM_THREADS = 512;
+constexpr int KEY_THREAD = 128;   // where each tensor has its own bias: behind the threads that make those
+static_assert(ADAMW_TENSORS <= KEY_THREAD && KEY_THREAD < NORM_THREADS, "a thread a tensor");
 
-// what the update needs of the step's number, of the norm and of the seed, written by the first launch of a step
+// what the update needs of a number of steps t
+struct AdamwBias {
+    float step_size, inv_root;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+};
+// and of the step's own number and the seed, written by the first launch of a step
 struct AdamwScalars {
-    float step_size, root;  // lr / (1 - b1^t), sqrt(1 - b2^t)
-    uint64_t key;           // rng_key(seed, t)
+    AdamwBias bias;
+    uint64_t key;  // rng_key(seed, t)
 };
 
 struct AdamwTable {
@@ -42,6 +48,7 @@ struct AdamwTable {
     int64_t n[ADAMW_TENSORS];
     uint32_t block[ADAMW_TENSORS];  // the tensor's first 128-element block in the flat moments
     uint32_t first[ADAMW_TENSORS];  // its first chunk in this launch
+    uint32_t index[ADAMW_TENSORS];  // its place in the caller's list
     int count;
     uint32_t chunks;
 };
@@ -85,26 +92,55 @@ __device__ __forceinline__ void store4(T* dst, int64_t i, int64_t n, f32x4 v) {
     }
 }
 
-__device__ __forceinline__ void write_scalars(int64_t* step, AdamwScalars* out, const AdamwHyper& h) {
+__device__ __forceinline__ AdamwBias bias_of(int64_t t, const AdamwHyper& h) {
+    const float root = (float)sqrt(1.0 - pow(h.b2, (double)t));
+    return {(float)(h.lr / (1.0 - pow(h.b1, (double)t))), 1.f / root};
+}
+__device__ __forceinline__ int64_t write_key(int64_t* step, AdamwScalars* out, const AdamwHyper& h) {
     const int64_t t = *step + 1;
     *step = t;
-    out->step_size = (float)(h.lr / (1.0 - pow(h.b1, (double)t)));
-    out->root = (float)sqrt(1.0 - pow(h.b2, (double)t));
     out->key = rng_key(h.seed, (uint64_t)t);
+    return t;
+}
+__device__ __forceinline__ void write_scalars(int64_t* step, AdamwScalars* out, const AdamwHyper& h) {
+    out->bias = bias_of(write_key(step, out, h), h);
+}
+// A tensor whose gradient is missing now and then has taken fewer steps than the list: its moments have decayed less, and its
+// corrections go by its own count. One thread a tensor of the table, the step's key in another wave beside them: two powers in
+// 64 bits are 1 us of latency.
+__device__ __forceinline__ void write_biases(const AdamwTable& tab, int64_t* counts, AdamwBias* out, const AdamwHyper& h) {
+    if ((int)threadIdx.x >= tab.count) return;  // ADAMW_TENSORS threads at most
+    const int64_t t = counts[tab.index[threadIdx.x]] + 1;
+    counts[tab.index[threadIdx.x]] = t;
+    out[threadIdx.x] = bias_of(t, h);
 }
 
-// the first launch of a step that takes no norm
+// the first launch of a step that takes no norm, and with counts each table's
 __global__ void adamw_begin_kernel(int64_t* step, AdamwScalars* out, float* norm, AdamwHyper h) {
     write_scalars(step, out, h);
     *norm = 0.f;
+}
+__global__ void adamw_begin_each_kernel(AdamwTable tab, int64_t* step, AdamwScalars* out, float* norm, int64_t* counts,
+                                        AdamwBias* bias, AdamwHyper h) {
+    if (step != nullptr && threadIdx.x == KEY_THREAD) {
+        write_key(step, out, h);
+        *norm = 0.f;
+    }
+    write_biases(tab, counts, bias, h);
 }
 
 // partial[workgroup] = sum of g^2 over its chunks, in 64 bits: the factor c is then the same to its last bit whatever
 // the split, and with it every code. Squares of fp32 values are exact in 64 bits.
 template <typename T>
 __global__ __launch_bounds__(NORM_THREADS) void adamw_norm_kernel(AdamwTable tab, double* __restrict__ partial,
-                                                                  int64_t* step, AdamwScalars* out, AdamwHyper h) {
-    if (step != nullptr && blockIdx.x == 0 && threadIdx.x == 0) write_scalars(step, out, h);
+                                                                  int64_t* step, AdamwScalars* out, int64_t* counts,
+                                                                  AdamwBias* bias, AdamwHyper h) {
+    if (blockIdx.x == 0 && counts != nullptr) {
+        if (step != nullptr && threadIdx.x == KEY_THREAD) write_key(step, out, h);
+        write_biases(tab, counts, bias, h);
+    } else if (blockIdx.x == 0 && step != nullptr && threadIdx.x == 0) {
+        write_scalars(step, out, h);
+    }
     // four chunks' loads before the first is squared
     double acc = 0.0;
     for (uint32_t c0 = blockIdx.x; c0 < tab.chunks; c0 += 4 * gridDim.x) {
@@ -168,19 +204,20 @@ __device__ __forceinline__ float apply(float p, float m, float u, float decay, f
 
 // A workgroup's first chunk is asked for before the clip factor is made of the partial sums (one round trip less; the 8-bit
 // kernel's registers would lose a workgroup a CU for it).
-template <typename T>
+template <typename T, bool EACH>
 __global__ __launch_bounds__(256) void adamw32_kernel(AdamwTable tab, float* __restrict__ em, float* __restrict__ ev,
-                                                      const AdamwScalars* __restrict__ sc, AdamwHyper h,
+                                                      const AdamwBias* __restrict__ bias, AdamwHyper h,
                                                       const double* __restrict__ partial, int parts,
                                                       float* __restrict__ norm_out) {
     __shared__ double red[4];
     float c = 1.f;
-    const float step_size = sc->step_size, inv_root = 1.f / sc->root;
+    const AdamwBias all = *bias;
     for (uint32_t ch = blockIdx.x; ch < tab.chunks; ch += gridDim.x) {
         const int k = find_tensor(tab, ch);
         T* p = (T*)tab.p[k];
         const T* g = (const T*)tab.g[k];
         const int64_t n = tab.n[k], off = (int64_t)tab.block[k] * 128;
+        const AdamwBias own = EACH ? bias[k] : all;
         const int64_t base = (int64_t)(ch - tab.first[k]) * CHUNK + threadIdx.x * 4;
         f32x4 pv[2], gv[2], mv[2], vv[2];
 #pragma unroll
@@ -203,7 +240,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwTable tab, float* __r
                 moments(c * gv[q][e], m, v, h.omb1, h.b2f, h.omb2);
                 mv[q][e] = m;
                 vv[q][e] = v;
-                pv[q][e] = apply(pv[q][e], m, __builtin_sqrtf(v), h.decay, step_size, inv_root, h.epsf);
+                pv[q][e] = apply(pv[q][e], m, __builtin_sqrtf(v), h.decay, own.step_size, own.inv_root, h.epsf);
             }
             store4(p, i, n, pv[q]);
             store4(em + off, i, n, mv[q]);
@@ -222,20 +259,22 @@ __device__ __forceinline__ uint32_t random_code(float x, float inv, uint32_t r) 
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
-template <typename T>
+template <typename T, bool EACH>
 __global__ __launch_bounds__(256) void adamw8_kernel(AdamwTable tab, uint8_t* __restrict__ em, uint8_t* __restrict__ eu,
                                                      uint8_t* __restrict__ sm, uint8_t* __restrict__ su,
-                                                     const AdamwScalars* __restrict__ sc, AdamwHyper h,
+                                                     const AdamwScalars* __restrict__ sc,
+                                                     const AdamwBias* __restrict__ bias, AdamwHyper h,
                                                      const double* __restrict__ partial, int parts,
                                                      float* __restrict__ norm_out) {
     __shared__ double red[4];
     const float c = parts > 0 ? clip_factor(partial, parts, h.max_norm, norm_out, red) : 1.f;
-    const float step_size = sc->step_size, inv_root = 1.f / sc->root;
     const uint64_t key = sc->key;
+    const AdamwBias all = *bias;
     for (uint32_t ch = blockIdx.x; ch < tab.chunks; ch += gridDim.x) {
         const int k = find_tensor(tab, ch);
         T* p = (T*)tab.p[k];
         const T* g = (const T*)tab.g[k];
+        const AdamwBias own = EACH ? bias[k] : all;
         const int64_t n = tab.n[k], off = (int64_t)tab.block[k] * 128;
         // 16 lanes hold one block of 128; a block that begins past the tensor's end does not exist
         const int64_t i = (int64_t)(ch - tab.first[k]) * CHUNK + threadIdx.x * 8;
@@ -280,7 +319,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamwTable tab, uint8_t* __
                 uok = uok && finite(uj);
                 mmax = fmaxf(mmax, __builtin_fabsf(mj));
                 umax = fmaxf(umax, uj);
-                pv[j >> 2][j & 3] = apply(pv[j >> 2][j & 3], mj, uj, h.decay, step_size, inv_root, h.epsf);
+                pv[j >> 2][j & 3] = apply(pv[j >> 2][j & 3], mj, uj, h.decay, own.step_size, own.inv_root, h.epsf);
             }
         }
         // a block with an infinity or a NaN is held as a NaN (byte 255, codes 0); the maximum carries the fact
@@ -317,56 +356,78 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamwTable tab, uint8_t* __
 
 }  // namespace
 
+// one table per ADAMW_TENSORS tensors and at most one partly filled per type
+static int64_t adamw_tables(int64_t count) { return count / ADAMW_TENSORS + 3; }
 int64_t adamw_scratch_bytes(int64_t count) {
-    // one table per ADAMW_TENSORS tensors and at most one partly filled per type
-    const int64_t launches = count / ADAMW_TENSORS + 3;
-    return 64 + launches * ADAMW_NORM_BLOCKS * (int64_t)sizeof(double);
+    return 64 + adamw_tables(count) * ADAMW_NORM_BLOCKS * (int64_t)sizeof(double) +
+           (count * (int64_t)sizeof(AdamwBias) + 15) / 16 * 16;
 }
 
 void launch_adamw(hipStream_t st, const AdamwCall& a) {
-    // scratch: [scalars][norm, at 32][partial sums, at 64]
+    // scratch: [scalars][norm, at 32][partial sums, at 64][each listed tensor's bias, in the order of the tables]
     AdamwScalars* sc = (AdamwScalars*)a.scratch;
     float* norm = (float*)((char*)a.scratch + 32);
     double* partial = (double*)((char*)a.scratch + 64);
+    AdamwBias* biases = (AdamwBias*)(partial + adamw_tables(a.count) * ADAMW_NORM_BLOCKS);
+    const bool each = a.counts != nullptr;
     AdamwTable tab;
     int parts = 0;
-    // pass 0: the norm (clipping only), pass 1: the update. Each walks the tensors type by type, a table at a time.
-    for (int pass = a.h.max_norm > 0.0 ? 0 : 1; pass < 2; ++pass) {
-        bool begun = pass == 1 && parts > 0;
+    bool begun = false;
+    // pass 0: the norm (when clipping) and each tensor's bias (with counts), pass 1: the update. Each walks the tensors type by
+    // type, a table at a time.
+    for (int pass = a.h.max_norm > 0.0 || each ? 0 : 1; pass < 2; ++pass) {
         if (!begun && pass == 1) {
             hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(1), 0, st, a.step, sc, norm, a.h);
             begun = true;
         }
+        int64_t listed = 0;
         for (int type = 0; type < 3; ++type) {
             tab.count = 0;
             tab.chunks = 0;
             auto flush = [&]() {
                 if (tab.count == 0) return;
+                AdamwBias* bias = biases + listed;
+                listed += tab.count;
                 if (pass == 0) {
                     const unsigned grid = tab.chunks < (uint32_t)ADAMW_NORM_BLOCKS ? tab.chunks : ADAMW_NORM_BLOCKS;
                     int64_t* step = begun ? nullptr : a.step;
                     begun = true;
-#define SIREN_ADAMW_NORM(T) \
-    hipLaunchKernelGGL(adamw_norm_kernel<T>, dim3(grid), dim3(NORM_THREADS), 0, st, tab, partial + parts, step, sc, a.h)
-                    if (type == 0) SIREN_ADAMW_NORM(float);
-                    if (type == 1) SIREN_ADAMW_NORM(__bf16);
-                    if (type == 2) SIREN_ADAMW_NORM(_Float16);
+#define SIREN_ADAMW_NORM(T)                                                                                                  \
+    hipLaunchKernelGGL(adamw_norm_kernel<T>, dim3(grid), dim3(NORM_THREADS), 0, st, tab, partial + parts, step, sc, a.counts, \
+                       bias, a.h)
+                    if (!(a.h.max_norm > 0.0)) {
+                        hipLaunchKernelGGL(adamw_begin_each_kernel, dim3(1), dim3(KEY_THREAD + 1), 0, st, tab, step, sc, norm, a.counts, bias,
+                                           a.h);
+                    } else {
+                        if (type == 0) SIREN_ADAMW_NORM(float);
+                        if (type == 1) SIREN_ADAMW_NORM(__bf16);
+                        if (type == 2) SIREN_ADAMW_NORM(_Float16);
+                        parts += (int)grid;
+                    }
 #undef SIREN_ADAMW_NORM
-                    parts += (int)grid;
                 } else {
                     const unsigned grid = tab.chunks < (uint32_t)ADAMW_BLOCKS ? tab.chunks : ADAMW_BLOCKS;
-#define SIREN_ADAMW(T)                                                                                              \
-    do {                                                                                                            \
-        if (a.bits == 32)                                                                                           \
-            hipLaunchKernelGGL(adamw32_kernel<T>, dim3(grid), dim3(256), 0, st, tab, (float*)a.m, (float*)a.v, sc,   \
-                               a.h, partial, parts, norm);                                                          \
-        else                                                                                                        \
-            hipLaunchKernelGGL(adamw8_kernel<T>, dim3(grid), dim3(256), 0, st, tab, (uint8_t*)a.m, (uint8_t*)a.v,    \
-                               a.sm, a.sv, sc, a.h, partial, parts, norm);                                          \
+                    if (!each) bias = &sc->bias;
+#define SIREN_ADAMW(T, EACH)                                                                                                   \
+    do {                                                                                                                       \
+        if (a.bits == 32)                                                                                                      \
+            hipLaunchKernelGGL((adamw32_kernel<T, EACH>), dim3(grid), dim3(256), 0, st, tab, (float*)a.m, (float*)a.v, bias,   \
+                               a.h, partial, parts, norm);                                                                     \
+        else                                                                                                                   \
+            hipLaunchKernelGGL((adamw8_kernel<T, EACH>), dim3(grid), dim3(256), 0, st, tab, (uint8_t*)a.m, (uint8_t*)a.v,      \
+                               a.sm, a.sv, sc, bias, a.h, partial, parts, norm);                                               \
     } while (0)
-                    if (type == 0) SIREN_ADAMW(float);
-                    if (type == 1) SIREN_ADAMW(__bf16);
-                    if (type == 2) SIREN_ADAMW(_Float16);
+#define SIREN_ADAMW_TYPES(EACH)                 \
+    do {                                        \
+        if (type == 0) SIREN_ADAMW(float, EACH);    \
+        if (type == 1) SIREN_ADAMW(__bf16, EACH);   \
+        if (type == 2) SIREN_ADAMW(_Float16, EACH); \
+    } while (0)
+                    if (each)
+                        SIREN_ADAMW_TYPES(true);
+                    else
+                        SIREN_ADAMW_TYPES(false);
+#undef SIREN_ADAMW_TYPES
 #undef SIREN_ADAMW
                 }
                 tab.count = 0;
@@ -383,6 +444,7 @@ void launch_adamw(hipStream_t st, const AdamwCall& a) {
                     tab.n[tab.count] = n;
                     tab.block[tab.count] = (uint32_t)block;
                     tab.first[tab.count] = tab.chunks;
+                    tab.index[tab.count] = (uint32_t)k;
                     tab.chunks += (uint32_t)chunks;
                     ++tab.count;
                 }

@@ -117,7 +117,7 @@ def _state_size(params):
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
-               max_norm=None, seed=0, scales=None):
+               max_norm=None, seed=0, scales=None, counts=None):
     """One AdamW step (torch.optim.AdamW: decoupled weight decay, amsgrad and maximize off) over all tensors at once,
     after torch.nn.utils.clip_grad_norm_(max_norm) when max_norm is set. Everything is updated in place; nothing
     synchronises with the host, and a captured step advances by itself on every replay (lr and the rest are captured).
@@ -129,18 +129,21 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     one byte per 128 elements) torch.float8_e4m3fn: exp_avg holds m, exp_avg_sq holds sqrt(v), value * 2^(byte - 127). The
     8-bit states are rounded up or down at random, from (seed, step, element): the same call gives the same result.
     step: int64, one element, on the device: the steps done so far; 1 is added.
+    counts: int64, one element a parameter, on the device: the steps that each has taken; 1 is added where there is a gradient,
+    and the bias corrections go by it, as torch's do. Without counts they go by step, for a list whose gradients are all there
+    in every step.
 
     Returns the gradients' norm before clipping (a device tensor), or None without max_norm."""
     if not (0. <= betas[0] < 1. and 0. <= betas[1] < 1. and eps >= 0. and math.isfinite(lr) and math.isfinite(weight_decay)):
         raise ValueError('need 0 <= betas < 1, eps >= 0 and finite lr and weight_decay')
     sm, sv = (None, None) if scales is None else scales
     return _lib.native().adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas[0], betas[1], eps, weight_decay,
-                                    max_norm, seed & 0xFFFFFFFFFFFFFFFF, sm, sv)
+                                    max_norm, seed & 0xFFFFFFFFFFFFFFFF, sm, sv, counts)
 
 
 class FusedAdamW:
-    """AdamW over parameters where they lie (any mix of fp32, bf16, fp16; .grad may be replaced freely), two launches a
-    step. state_bits 8 keeps the moments in 8 bits (2 bytes a parameter instead of 8), rounded at random from seed."""
+    """AdamW over parameters where they lie (any mix of fp32, bf16, fp16; .grad may be replaced freely, and be missing: the
+    parameter and its moments then stay, and its bias corrections count its own steps), two launches a step. state_bits 8 keeps the moments in 8 bits (2 bytes a parameter instead of 8), rounded at random from seed."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32,
                  seed=0):
@@ -162,7 +165,8 @@ class FusedAdamW:
         # byte 1 is the scale of a block of zeros
         self.scales = None if state_bits == 32 else tuple(torch.ones(n // 128, dtype=torch.uint8, device=dev)
                                                           for _ in range(2))
-        self.steps = torch.zeros(1, dtype=torch.int64, device=dev)
+        self.steps = torch.zeros(1, dtype=torch.int64, device=dev)  # calls, and each parameter's own
+        self.counts = torch.zeros(len(self.params), dtype=torch.int64, device=dev)
         self._norm = None
 
     def zero_grad(self, set_to_none=True):
@@ -176,7 +180,8 @@ class FusedAdamW:
     def step(self):
         self._norm = adamw_step(self.params, [p.grad for p in self.params], self.exp_avg, self.exp_avg_sq, self.steps,
                                 lr=self.lr, betas=self.betas, eps=self.eps, weight_decay=self.weight_decay,
-                                max_norm=self.max_norm or None, seed=self.seed, scales=self.scales)
+                                max_norm=self.max_norm or None, seed=self.seed, scales=self.scales,
+                                counts=self.counts)
 
     def grad_norm(self):
         """The pre-clip global gradient norm of the last clipped step (device tensor; no host sync)."""
@@ -184,8 +189,8 @@ class FusedAdamW:
 
     def state_dict(self):
         """The state's own tensors (8-bit ones as they are held): clone what must outlive the next step."""
-        out = {'state_bits': self.state_bits, 'seed': self.seed, 'steps': self.steps, 'exp_avg': self.exp_avg,
-               'exp_avg_sq': self.exp_avg_sq}
+        out = {'state_bits': self.state_bits, 'seed': self.seed, 'steps': self.steps, 'counts': self.counts,
+               'exp_avg': self.exp_avg, 'exp_avg_sq': self.exp_avg_sq}
         if self.scales is not None:
             out['exp_avg_scale'], out['exp_avg_sq_scale'] = self.scales
         return out
@@ -198,4 +203,5 @@ class FusedAdamW:
         mine = self.state_dict()
         for k, t in mine.items():
             if isinstance(t, torch.Tensor):
-                t.copy_(state[k])
+                # a state of before each parameter's steps were counted: they were the calls
+                t.copy_(state['steps'].expand_as(t) if k == 'counts' and k not in state else state[k])

@@ -428,3 +428,112 @@ def test_negated_views(cuda):
     assert torch.equal(a, b) and not torch.equal(a, p)
     with pytest.raises(ValueError, match='negated'):
         optim.adamw_step([torch._neg_view(p)], [g], opt.exp_avg, opt.exp_avg_sq, opt.steps)
+
+
+def missing(i, t):
+    """Whether tensor i has no gradient in step t: one always has, one never, one begins late, others pause."""
+    return [False, True, t <= 7, t % 2 == 0, 3 <= t <= 9, t != 5][i % 6]
+
+
+@pytest.mark.parametrize('max_norm', [None, 1.])
+def test_missing_gradients_against_torch(cuda, max_norm):
+    """A parameter's bias corrections count its own steps, as torch.optim.AdamW's do: one whose first gradient comes late, ones
+    that pause, one that never has any. More tensors than a launch takes."""
+    from siren_amd.optim import FusedAdamW
+    g = torch.Generator().manual_seed(0)
+    sizes = [7, 130, 300, 5000, 33, 2] * 40
+    start = [torch.randn(s, generator=g).clamp(-4, 4) * 0.1 for s in sizes]
+    a, b = ([t.clone().to(cuda).requires_grad_(True) for t in start] for _ in range(2))
+    mine = FusedAdamW(a, lr=1e-3, weight_decay=0.05, max_norm=max_norm)
+    theirs = torch.optim.AdamW(b, lr=1e-3, weight_decay=0.05)
+    for t in range(1, 21):
+        for i, (p, q) in enumerate(zip(a, b)):
+            p.grad = None if missing(i, t) else torch.randn(p.shape, generator=g).to(cuda)
+            q.grad = None if p.grad is None else p.grad.clone()
+        if max_norm is not None:
+            torch.nn.utils.clip_grad_norm_(b, max_norm)
+        mine.step(), theirs.step()
+    assert mine.counts.tolist() == [sum(not missing(i, t) for t in range(1, 21)) for i in range(len(sizes))]
+    assert int(mine.steps) == 20
+    # 20 steps, each of at most (1 - b1) / sqrt(1 - b2) = 3.2 lr and within some 20 roundings, of parameters below 1
+    for p, q in zip(a, b):
+        assert (p - q).abs().max() <= 20 * (4e-3 * 20 * 2. ** -23 + 4 * 2. ** -24)
+
+
+@pytest.mark.parametrize('max_norm', [None, 1.])
+@pytest.mark.parametrize('bits', [32, 8])
+def test_missing_gradients_keep_what_is_theirs(cuda, bits, max_norm):
+    """Mixed types: without a gradient a parameter and its moments stay as they were; with one, moments, codes and step are the
+    definition's, the corrections by the parameter's own count. Captured and replayed it is the same."""
+    from siren_amd.optim import FusedAdamW
+    types = [torch.float32, torch.bfloat16, torch.float32, torch.float16, torch.float32, torch.bfloat16]
+    sizes = [300, 5, 4099, 129, 1, 640]
+
+    def build():
+        ps = [t.to(d).to(cuda).requires_grad_(True) for t, d in zip(make(sizes, torch.float32, 1, 0.05), types)]
+        return FusedAdamW(ps, lr=1e-3, weight_decay=0.1, max_norm=max_norm, state_bits=bits, seed=5)
+
+    opt, replayed = build(), build()
+    m = u = np.zeros(opt.exp_avg.numel(), np.float32)
+    count = [0] * 6
+    for t in range(1, 9):
+        grads = [x.to(d) for x, d in zip(make(sizes, torch.float32, 10 + t, 0.1), types)]
+        for o in (opt, replayed):
+            for i, (p, g) in enumerate(zip(o.params, grads)):
+                p.grad = None if missing(i, t) else g.to(cuda)
+        before = [p.detach().clone() for p in opt.params]
+        old = [s.clone() for s in (opt.exp_avg.view(torch.uint8), opt.exp_avg_sq.view(torch.uint8))]
+        opt.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            replayed.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(*([*o.params, o.exp_avg.view(torch.uint8), o.exp_avg_sq.view(torch.uint8), o.counts] for o in (opt, replayed))):
+            assert torch.equal(x, y), t
+        g = flat([x * 0 if missing(i, t) else x for i, x in enumerate(grads)])
+        c = 1. if max_norm is None else min(1., max_norm / (math.sqrt((g.astype(np.float64) ** 2).sum()) + 1e-6))
+        mn, un, cm, bm, cu, bu = oracle8(g, m, u, t, 5, c, 0.9, 0.999)
+        at = 0
+        for i, (p, q) in enumerate(zip(opt.params, before)):
+            span = slice(at, at + (p.numel() + 127) // 128 * 128)
+            at = span.stop
+            raw = [s.view(torch.uint8).view(-1, 4 if bits == 32 else 1)[span] for s in (opt.exp_avg, opt.exp_avg_sq)]
+            if missing(i, t):
+                assert torch.equal(p, q)
+                assert all(torch.equal(x, s.view(-1, 4 if bits == 32 else 1)[span]) for x, s in zip(raw, old))
+                continue
+            count[i] += 1
+            if bits == 8:
+                codes = [x.flatten().cpu().numpy() for x in raw]
+                assert np.array_equal(codes[0], cm[span]) and np.array_equal(codes[1], cu[span]), (t, i)
+            mt, ut = (mn[span], un[span]) if bits == 8 else (opt.exp_avg[span].cpu().numpy(), opt.exp_avg_sq[span].sqrt().cpu().numpy())
+            want, step = update(flat([q]), mt, ut, count[i], 1e-3, 0.9, 0.999, 1e-8, 0.1)
+            check_params(flat([p]), want, step, types[i], (t, i))
+        assert opt.counts.tolist() == count
+        if bits == 8:
+            m, u = (value(s.view(torch.uint8).cpu().numpy().astype(np.int64), b.cpu().numpy())
+                    for s, b in zip((opt.exp_avg, opt.exp_avg_sq), opt.scales))
+
+
+def test_counts_are_checked_saved_and_made_up(cuda):
+    from siren_amd.optim import FusedAdamW, adamw_step
+    ps = [torch.ones(300, device=cuda), torch.ones(5, device=cuda)]
+    opt = FusedAdamW(ps)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    ps[1].grad = None
+    opt.step()
+    assert opt.counts.tolist() == [2, 1]
+    saved = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in opt.state_dict().items()}
+    other = FusedAdamW([p.clone() for p in ps])
+    other.load_state_dict(saved)
+    assert other.counts.tolist() == [2, 1] and int(other.steps) == 2
+    del saved['counts']  # one from before they were counted
+    other.load_state_dict(saved)
+    assert other.counts.tolist() == [2, 2]
+    for bad in (opt.counts[:1], opt.counts.int(), opt.counts.cpu(), torch.zeros(2, 2, dtype=torch.int64, device=cuda)[:, 0]):
+        with pytest.raises(ValueError, match='counts'):
+            adamw_step(ps, [p.clone() for p in ps], opt.exp_avg, opt.exp_avg_sq, opt.steps, counts=bad)
+    assert int(opt.steps) == 2

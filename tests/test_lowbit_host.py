@@ -180,3 +180,15 @@ def test_sizes_at_the_end_of_64_bits(lib, n):
     ps, ns, ts = (P * many)(*[64] * many), (ctypes.c_int64 * many)(*[n] * many), (ctypes.c_int32 * many)()
     assert lib.siren_adamw_step(many, ps, ps, ns, ts, 32, P(64), P(64), None, None, P(64), 1e-3, .9, .99, 1e-8, 0., 0., 0, P(64),
                                 None) == EINVAL
+
+
+def test_adamw_with_counts_validates(lib):
+    def call(counts, step=P(64), count=1, scratch=P(64)):
+        return lib.siren_adamw_step_each(count, (P * 1)(64), (P * 1)(64), (ctypes.c_int64 * 1)(5), (ctypes.c_int32 * 1)(0), 32, P(64),
+                                         P(64), None, None, step, counts, 1e-3, .9, .99, 1e-8, 0., 0., 0, scratch, None)
+    for bad in (dict(counts=P(4)), dict(counts=P(65)), dict(counts=P(64), step=None), dict(counts=P(64), scratch=None),
+                dict(counts=P(64), count=-1), dict(counts=None, count=1 << 33)):
+        assert call(**bad) == EINVAL, bad
+    a, b = ctypes.c_int64(0), ctypes.c_int64(0)
+    assert lib.siren_adamw_scratch_bytes(1000, ctypes.byref(a)) == OK and lib.siren_adamw_scratch_bytes(2000, ctypes.byref(b)) == OK
+    assert b.value - a.value >= 8 * 1000 and a.value % 16 == 0  # room for each tensor's own corrections

@@ -174,7 +174,12 @@ class FusedAdamW:
             if set_to_none:
                 p.grad = None
             elif p.grad is not None:
-                p.grad.detach_().zero_()
+                # as torch's optimisers: a gradient that is a view (of a bucket) cannot be detached in place, and need not be
+                if p.grad.grad_fn is not None:
+                    p.grad.detach_()
+                else:
+                    p.grad.requires_grad_(False)
+                p.grad.zero_()
 
     @torch.no_grad()
     def step(self):

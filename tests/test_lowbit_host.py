@@ -192,3 +192,20 @@ def test_adamw_with_counts_validates(lib):
     a, b = ctypes.c_int64(0), ctypes.c_int64(0)
     assert lib.siren_adamw_scratch_bytes(1000, ctypes.byref(a)) == OK and lib.siren_adamw_scratch_bytes(2000, ctypes.byref(b)) == OK
     assert b.value - a.value >= 8 * 1000 and a.value % 16 == 0  # room for each tensor's own corrections
+
+
+def test_zero_grad_of_a_bucket():
+    """Gradients that are views of one buffer are cleared in place and stay its views."""
+    from types import SimpleNamespace
+    from siren_amd import optim
+    bucket = torch.ones(10)
+    p, q, r = torch.zeros(4, requires_grad=True), torch.zeros(6, requires_grad=True), torch.zeros(2, requires_grad=True)
+    p.grad, q.grad = bucket[:4], bucket[4:].view_as(q)
+    optim.FusedAdamW.zero_grad(SimpleNamespace(params=[p, q, r]), set_to_none=False)
+    assert not bucket.any() and p.grad.data_ptr() == bucket.data_ptr() and r.grad is None
+    x = torch.ones(4, requires_grad=True)  # one that is a graph's result is cut off from it
+    p.grad = x * 2
+    optim.FusedAdamW.zero_grad(SimpleNamespace(params=[p]), set_to_none=False)
+    assert p.grad.grad_fn is None and not p.grad.any()
+    optim.FusedAdamW.zero_grad(SimpleNamespace(params=[p, q]))
+    assert p.grad is None and q.grad is None

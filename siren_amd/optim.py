@@ -204,9 +204,14 @@ class FusedAdamW:
         if state['state_bits'] != self.state_bits or state['exp_avg'].numel() != self.exp_avg.numel():
             raise ValueError('a state of %d bits and %d values does not fit this optimiser\'s %d bits and %d values'
                              % (state['state_bits'], state['exp_avg'].numel(), self.state_bits, self.exp_avg.numel()))
-        self.seed = int(state['seed'])
-        mine = self.state_dict()
+        mine = {k: t for k, t in self.state_dict().items() if isinstance(t, torch.Tensor)}
+        # a state of before each parameter's steps were counted: they were the calls
+        theirs = {k: state['steps'].expand_as(t) if k == 'counts' and k not in state else state[k] for k, t in mine.items()}
+        seed = int(state['seed'])
+        for k, t in mine.items():  # all of it fits, or nothing is taken
+            if theirs[k].shape != t.shape or theirs[k].dtype != t.dtype:
+                raise ValueError('%s of the state is %s %s, this optimiser\'s %s %s'
+                                 % (k, tuple(theirs[k].shape), theirs[k].dtype, tuple(t.shape), t.dtype))
+        self.seed = seed
         for k, t in mine.items():
-            if isinstance(t, torch.Tensor):
-                # a state of before each parameter's steps were counted: they were the calls
-                t.copy_(state['steps'].expand_as(t) if k == 'counts' and k not in state else state[k])
+            t.copy_(theirs[k])

@@ -209,3 +209,38 @@ def test_zero_grad_of_a_bucket():
     assert p.grad.grad_fn is None and not p.grad.any()
     optim.FusedAdamW.zero_grad(SimpleNamespace(params=[p, q]))
     assert p.grad is None and q.grad is None
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_state_is_taken_whole_or_not(bits):
+    """load_state_dict of a state that lacks a tensor, or holds one of another size or type, changes nothing."""
+    from siren_amd import optim
+
+    def build(fill, n=256, count=2):
+        opt = object.__new__(optim.FusedAdamW)
+        opt.state_bits, opt.seed, dtype = bits, fill, torch.float32 if bits == 32 else torch.float8_e4m3fn
+        opt.exp_avg, opt.exp_avg_sq = (torch.full((n,), float(fill)).to(dtype) for _ in range(2))
+        opt.scales = None if bits == 32 else tuple(torch.full((n // 128,), fill, dtype=torch.uint8) for _ in range(2))
+        opt.steps, opt.counts = torch.full((1,), fill), torch.full((count,), fill)
+        return opt
+
+    def bytes_of(opt):
+        return [opt.seed] + [t.contiguous().view(torch.uint8).tolist() for t in opt.state_dict().values() if isinstance(t, torch.Tensor)]
+
+    mine, good = build(1), build(2).state_dict()
+    before = bytes_of(mine)
+    for key in good:
+        if key != 'counts':  # that one is made up
+            with pytest.raises(KeyError):
+                mine.load_state_dict({k: v for k, v in good.items() if k != key})
+            assert bytes_of(mine) == before, key
+        if isinstance(good[key], torch.Tensor):
+            for bad in (good[key].float()[:1].expand(3), good[key].to(torch.float64)):
+                with pytest.raises(ValueError):
+                    mine.load_state_dict({**good, key: bad})
+                assert bytes_of(mine) == before, key
+    with pytest.raises(ValueError):  # as many values, other tensors
+        mine.load_state_dict(build(2, count=3).state_dict())
+    assert bytes_of(mine) == before
+    mine.load_state_dict(good)
+    assert bytes_of(mine) == bytes_of(build(2))

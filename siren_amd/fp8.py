@@ -69,7 +69,7 @@ def dequantize(b):
     s = torch.where(byte > 0, byte << 23, 1 << 22).view(torch.float32)  # byte 0 is 2^-127, a subnormal number
     if b.tiled:
         s = s.repeat_interleave(BLOCK, 0)[:rows]
-    return (b.data.float().view(rows, kb, BLOCK) * s[:, :, None]).view(rows, -1)[:, :b.cols]
+    return (b.data.float().view(rows, kb, BLOCK) * s[:, :, None]).view(rows, kb * BLOCK)[:, :b.cols]
 
 
 def matmul(a, b, bias=None, activation=None, omega=30., dtype=torch.float32, derivative=False):

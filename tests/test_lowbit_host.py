@@ -244,3 +244,13 @@ def test_a_state_is_taken_whole_or_not(bits):
     assert bytes_of(mine) == before
     mine.load_state_dict(good)
     assert bytes_of(mine) == bytes_of(build(2))
+
+
+@pytest.mark.parametrize('rows,cols', [(0, 200), (0, 0), (3, 0)])
+@pytest.mark.parametrize('tile', [False, True])
+def test_dequantize_nothing(rows, cols, tile):
+    """What quantize returns for no rows or no columns is no values."""
+    from siren_amd import fp8
+    b = fp8.Blocks(torch.zeros(rows, (cols + 127) // 128 * 128).to(torch.float8_e4m3fn),
+                   torch.zeros((rows + 127) // 128 if tile else rows, (cols + 511) // 512 * 4, dtype=torch.uint8), cols)
+    assert fp8.dequantize(b).shape == (rows, cols)

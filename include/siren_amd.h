@@ -421,6 +421,9 @@ int32_t siren_laplace_backward_stored(const siren_cfg* cfg, const float* ws, con
  *   rows / 128 rounded up (one per 128 x 128)
  * In panels the values lie as (C / 64, rows, 64): 64 columns of all rows, then the next 64. The products read that
  * faster; it is what a program that quantises for one product asks for.
+ * The products take an operand's values as bf16 numbers. That is exact but at the ends of the range: of blocks whose magnitudes
+ * stay under 2^-116 (e5m2: 2^-102) values under 2^-126 are rounded to multiples of 2^-133, and a value of 2^128, to which
+ * magnitudes from 2^128 (1 - 2^-5) on (e5m2: 2^-4) round, is an infinity.
  * dtype of unquantised tensors: 0 fp32, 1 bf16, 2 fp16. Values, outputs and workspaces 16-byte aligned, scales 4. */
 
 #define SIREN_FP8_TILES 1  /* an operand's layout: one scale per 128 x 128 instead of per 1 x 128 */

@@ -40,7 +40,7 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, fl
     return __builtin_bit_cast(uint32_t, r);
 }
 
-// two codes to bf16, times scale (a power of two: exact)
+// two codes to bf16, times scale (a power of two: exact down to bf16's smallest number, 2^-133, and below 2^128)
 template <bool E5M2, int HI>
 __device__ __forceinline__ bf16x2 widen2(uint32_t w, float scale) {
     if constexpr (E5M2)

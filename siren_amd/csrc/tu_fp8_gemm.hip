@@ -7,6 +7,11 @@
 // value times a power of two is a bf16 number exactly, and v_cvt_scalef32_pk_bf16_fp8 makes two of them at once. So the
 // operands travel as bytes through HBM and LDS, are scaled and widened in registers, and the bf16 matrix pipe sums them,
 // for 16-bit results too (an output that nearly cancels would show the fp8 instructions' missing bits there as well).
+// Exactly, that is, where bf16 reaches: of scale bytes 3 and more (e5m2: 10) every code is a bf16 number, its subnormal ones,
+// which the pipe keeps, among them. Below, in blocks whose magnitudes stay under 2^-116 (e5m2: 2^-102), values under 2^-126 are
+// rounded to multiples of 2^-133, the nearest, ties to even: off by 2^-134 at most. Above, a block whose largest magnitude
+// rounds to 2^128 (from 2^128 (1 - 2^-5) on; e5m2: 2^-4) holds an infinity there, in fp32 as in bf16. A scale that is carried
+// apart, into the 32-bit sums, would lose neither, for a multiplication of every sum in each block.
 //
 // A workgroup of 4 waves owns 256 x 128 of out (128 x 128 where rows are few), each wave 128 x 64 (64 x 64) in tiles of
 // 32 x 32. Half a block, 64 k of both operands, is one stage of LDS: 24 KiB by direct global-to-LDS loads, three stages, so

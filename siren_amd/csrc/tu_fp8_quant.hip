@@ -3,7 +3,8 @@
 //   s = 2^e, the smallest with which the block's largest finite magnitude is at most 448 s (e5m2: 57344 s), e >= -126
 //   q = x / s to the nearest e4m3 (e5m2) value, ties to even; infinities and NaN become NaN (e5m2 keeps infinities)
 //
-// A power of two divides exactly, so the one rounding is q's, and a dequantised value is a bf16 number exactly.
+// A power of two divides exactly, so the one rounding is q's, and a dequantised value is a bf16 number exactly (from 2^-133 to
+// below 2^128: what of the smallest and largest blocks lies beyond is said with the products).
 // A training step needs a tensor both as rows (blocks along the columns) and transposed (blocks along the rows, for
 // the product that sums over the rows): one workgroup holds a 128 x 128 tile in registers and writes both, with the
 // column sums of a bias's gradient on the way, so the tensor is read once. 64 values a thread: 16 rows x 4 columns, so

@@ -7,7 +7,8 @@
 A block is 128 values along the axis that a product sums over (activations, gradients: 'row') or 128 x 128 (weights:
 'tile', which serve both directions). Its scale is the smallest power of two with which the largest finite magnitude is
 at most 448; values are then rounded once, to the nearest e4m3 number. Sums, bias and sine are in 32 bits. NaN stays NaN
-and infinities become NaN. BatchLinear, FCBlock, SingleBVPNet and HyperNetwork take it as precision='fp8'.
+and infinities become NaN. The products are exact for blocks whose largest magnitude lies between 2^-116 and 2^128 (1 - 2^-5);
+smaller blocks are held to multiples of 2^-133 there, a value that rounds to 2^128 is an infinity. BatchLinear, FCBlock, SingleBVPNet and HyperNetwork take it as precision='fp8'.
 
 The kernels are gfx950 only (include/siren_amd.h, "8-bit training"): there is no CPU path. Calls are asynchronous on the
 current stream of x's device and allocate from torch's caching allocator, so they can be captured into a graph. A captured

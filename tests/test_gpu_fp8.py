@@ -671,3 +671,48 @@ def test_a_layer_whose_backward_would_not_fit_is_refused_at_once(cuda):
     assert bool((fp8.linear(x, w.detach()) == 1).all())
     y = fp8.linear(x[:rows], w)
     assert torch.autograd.grad(y, w, torch.ones_like(y))[0].tolist() == [[float(rows)]]  # whole numbers below 2^24
+
+
+@pytest.mark.parametrize('m', [3, 40, 300])
+@pytest.mark.parametrize('fmt', [E4M3, E5M2])
+def test_products_at_the_small_end(cuda, m, fmt):
+    """Blocks of magnitudes from 2^-139 to 2^-90 against others near 2^100: a bf16 operand holds values under 2^-126 to half of
+    2^-133, all others exactly; the sums are 32-bit ones of that. The scale bytes from which on nothing is lost are 3 and, for
+    e5m2, 10."""
+    from siren_amd import fp8
+    g = torch.Generator().manual_seed(m)
+    k, n, first = 384, 70, 3 if fmt is E4M3 else 10
+    a = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-137, -90, (m, 3), generator=g).float()).repeat_interleave(128, 1)
+    b = torch.randn(n, k, generator=g) * 2. ** 100
+    aq, byte = held(np64(a), fmt)
+    bq = held(np64(b), tiles=True)[0]
+    assert byte.min() == 1 and byte.max() > first
+    small = (np.abs(aq) < 2. ** -126) & np.repeat(byte < first, 128, 1)
+    want = aq @ bq.T
+    tol = product_tol(aq, bq, want, torch.float32) + (1 + 2. ** -10) * 2. ** -134 * (small @ np.abs(bq).T)
+    qa, qb = fp8.quantize(a.to(cuda), dtype=fmt), fp8.quantize(b.to(cuda), 'tile')
+    check(fp8.matmul(qa, qb), want, tol, 'small first operand')
+    lossless = torch.from_numpy((byte >= first).all(1))
+    check(fp8.matmul(qa, qb)[lossless.to(cuda)], want[lossless.numpy()], product_tol(aq, bq, want, torch.float32)[lossless.numpy()],
+          'bytes from %d on' % first)
+    if fmt is E4M3:
+        check(fp8.linear(a.to(cuda), qb), want, tol, 'layer')
+        check(fp8.matmul(qb, qa), want.T, tol.T, 'small second operand')
+
+
+@pytest.mark.parametrize('m', [3, 40])
+def test_products_at_the_large_end(cuda, m):
+    """A block whose largest value rounds to 2^128 holds an infinity there, as dequantize shows it, and spoils its own row; the
+    largest that does not, 2^128 (1 - 2^-4), is taken exactly."""
+    from siren_amd import fp8
+    a = torch.zeros(m, 200)
+    a[:, 0] = 2. ** 127 + 2. ** 126 + 2. ** 125 + 2. ** 124  # 2^128 (1 - 2^-4), an e4m3 number times a power of two
+    a[:, 1], a[1, 0] = 2. ** 121, torch.finfo(torch.float32).max
+    b = torch.zeros(5, 200)
+    b[:, :2], b[3, 0] = 2. ** -100, 0.
+    qa, qb = fp8.quantize(a.to(cuda)), fp8.quantize(b.to(cuda))
+    assert bool(torch.isinf(fp8.dequantize(qa)[1, 0]))
+    want = (fp8.dequantize(qa).double().cpu() @ fp8.dequantize(qb).double().cpu().t()).float()
+    assert torch.isinf(want[1, :3]).all() and torch.isnan(want[1, 3]) and torch.isfinite(want[0]).all()
+    for got in (fp8.matmul(qa, qb), fp8.linear(a.to(cuda), fp8.quantize(b.to(cuda), 'tile'))):
+        assert torch.equal(got.cpu().nan_to_num(1., 2.), want.nan_to_num(1., 2.))

@@ -716,3 +716,22 @@ def test_products_at_the_large_end(cuda, m):
     assert torch.isinf(want[1, :3]).all() and torch.isnan(want[1, 3]) and torch.isfinite(want[0]).all()
     for got in (fp8.matmul(qa, qb), fp8.linear(a.to(cuda), fp8.quantize(b.to(cuda), 'tile'))):
         assert torch.equal(got.cpu().nan_to_num(1., 2.), want.nan_to_num(1., 2.))
+
+
+@pytest.mark.parametrize('m', [7, 200, 1500])
+def test_sine_bias_gradient_is_the_formulas(cuda, m):
+    """db of a sine layer against dy omega cos(omega z) in 64 bits: its terms are products of dy and a bf16 cosine, off by half a
+    bf16 step (2^-8) and by the phase's error, nothing of them is in 8 bits, and their sum is a 32-bit one."""
+    from siren_amd import fp8
+    k, n = 192, 130
+    x, w, b = layer(m, k, n, torch.float32, cuda, 5)
+    dy = values((m, n), 6, 1 / 64).to(cuda)
+    b.requires_grad_(True)
+    db, = torch.autograd.grad(fp8.linear(x, w, b, 'sine'), b, dy)
+    xq, wq = held(np64(x))[0], held(np64(w), tiles=True)[0]
+    z = xq @ wq.T + np64(b)
+    d = 30 * np.cos(30 * z)
+    phase = 30 * product_tol(xq, wq, 0 * z, torch.float32, np.abs(np64(b))) + np.abs(30 * z) * 2. ** -23 + 2. ** -22
+    off = 30 * phase + 2. ** -8 * np.abs(d)
+    want, mag = (np64(dy) * d).sum(0), (np.abs(np64(dy)) * (np.abs(d) + off)).sum(0)
+    check(db, want, (np.abs(np64(dy)) * off).sum(0) + 24 * 2. ** -24 * mag + 2. ** -149, 'db')

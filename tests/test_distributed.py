@@ -180,3 +180,68 @@ def test_dp_closure_loss_is_global():
     lf = float(loss.detach())
     assert ret['l0'] == ret['l1'] and abs(ret['l0'] - lf) <= 1e-6 * lf
     assert torch.equal(ret['g0'], ret['g1']) and torch.allclose(ret['g0'], p.grad, rtol=1e-5, atol=0)
+
+
+# ---- training.train(optimizer=...) under DP: an optimiser that clips by itself -------------------------------------------
+class _SelfClipping:
+    """Gradient descent that clips as optim.FusedAdamW does: by itself, to max_norm, all its gradients as one."""
+
+    def __init__(self, params, lr):
+        self.params, self.lr, self.max_norm, self.norms = list(params), lr, None, []
+
+    def zero_grad(self):
+        for p in self.params:
+            p.grad = None
+
+    @torch.no_grad()
+    def step(self):
+        norm = torch.stack([p.grad.norm() for p in self.params]).norm()
+        self.norms.append(float(norm))
+        c = min(1., self.max_norm / (float(norm) + 1e-6)) if self.max_norm else 1.
+        for p in self.params:
+            p.sub_(self.lr * c * p.grad)
+
+
+def _train_self_clipping(x, t, n_steps=3):
+    from siren_amd.modules import SingleBVPNet
+    from siren_amd.training import train
+    torch.manual_seed(3)
+    m = SingleBVPNet(type='tanh', hidden_features=32, num_hidden_layers=1, verbose=False)
+    opt = _SelfClipping(m.parameters(), 0.5)
+    with tempfile.TemporaryDirectory() as d:
+        train(m, [({'coords': x}, {'img': t})], epochs=n_steps, lr=1., steps_til_summary=1000, epochs_til_checkpoint=1000,
+              model_dir=d, loss_fn=lambda out, gt: {'img_loss': ((out['model_out'] - gt['img']) ** 2).mean()}, clip_grad=0.05,
+              device='cpu', log=lambda *a: None, optimizer=opt)
+    return torch.cat([p.detach().reshape(-1) for p in m.parameters()]), opt
+
+
+def _self_clipping_worker(rank, world, port, ret, n):
+    _env(rank, world, port)
+    from siren_amd import distributed as sd
+    sd.init('gloo')
+    x, t = _self_clipping_data(n)
+    a, b = sd.shard(n, world, rank, align=64)
+    p, opt = _train_self_clipping(x[:, a:b], t[:, a:b])
+    ret[rank], ret['norms%d' % rank], ret['n%d' % rank] = p, opt.norms, b - a
+    torch.distributed.destroy_process_group()
+
+
+def _self_clipping_data(n):
+    g = torch.Generator().manual_seed(1)
+    x = torch.rand(1, n, 2, generator=g) * 2 - 1
+    return x, torch.sin(3 * x[..., :1])
+
+
+@pytest.mark.parametrize('n', [1000, 70, 40])
+def test_an_optimiser_that_clips_itself_world2_equals_full_batch(n):
+    """Each rank's optimiser sees the reduced gradient once and clips that, not its shard's and not twice; with 40 coordinates
+    one rank's shard is empty."""
+    world, port = 2, _free_port()
+    ret = mp.Manager().dict()
+    mp.spawn(_self_clipping_worker, args=(world, port, ret, n), nprocs=world, join=True)
+    full, opt = _train_self_clipping(*_self_clipping_data(n))
+    assert opt.max_norm == 0.05 and max(opt.norms) > 0.05
+    assert ret['n0'] + ret['n1'] == n and (n != 40 or 0 in (ret['n0'], ret['n1']))
+    assert torch.equal(ret[0], ret[1]) and torch.allclose(ret[0], full, atol=1e-6, rtol=1e-5)
+    for r in (0, 1):  # norms of whole gradients: what a loop that clipped first would not show
+        assert torch.allclose(torch.tensor(ret['norms%d' % r]), torch.tensor(opt.norms), rtol=1e-4)

@@ -537,3 +537,45 @@ def test_counts_are_checked_saved_and_made_up(cuda):
         with pytest.raises(ValueError, match='counts'):
             adamw_step(ps, [p.clone() for p in ps], opt.exp_avg, opt.exp_avg_sq, opt.steps, counts=bad)
     assert int(opt.steps) == 2
+
+
+def test_second_moment_in_8_bits_does_not_drift(cuda):
+    """The 8-bit sqrt(v) under a constant gradient, within what its rounding's variance allows. While u <= 0.7, u only grows: a
+    step from a code q to u' = q + D, D <= 0.001 (w - q^2) / 2 q with w = 0.49, is rounded to q or to the next code d <= q / 8
+    above, with a variance of at most D d <= 0.001 (w - q^2) / 16. v's mean gains just that variance a step, so it grows as if
+    1 - b2 were 17 / 16 of itself at most (1 / 256 more in the first step, whose d^2 / 4 is the bound), and as fast as in 32 bits
+    at least. The variances add up to 0.3 w / 16 at most, so that v's deviation is below 2 0.7 sqrt(0.0092) = 0.134, a mean's of
+    2^16 elements below 0.41 % of 0.127; five of those are 2 %."""
+    from siren_amd.optim import FusedAdamW
+    n, steps, w = 1 << 16, 300, 0.49
+    p = torch.zeros(n, device=cuda, requires_grad=True)
+    opt = FusedAdamW([p], lr=0., weight_decay=0., state_bits=8, seed=3)
+    p.grad = torch.full((n,), 0.7, device=cuda)
+    for _ in range(steps):
+        opt.step()
+    v = (opt.exp_avg_sq.float() * torch.exp2(opt.scales[1].float() - 127).repeat_interleave(128)).double().square()
+    assert bool((v <= w).all())  # and so in every step before
+    exact = w * (1 - 0.999 ** steps)
+    most = w * (1 - (1 - 0.001 * 17 / 16) ** steps) * (1 + 1 / 256)
+    assert 0.98 * exact <= float(v.mean()) <= 1.02 * most, (float(v.mean()) / exact, most / exact)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_parameters_without_a_gradient_stay(cuda, bits):
+    """Of many tensors of mixed types those without a gradient keep their starting values, byte for byte, and so do their
+    moments; clipping or not."""
+    from siren_amd.optim import FusedAdamW
+    types = [torch.float32, torch.bfloat16, torch.float16]
+    for max_norm in (None, 0.5):
+        ps = [t.to(types[i % 3]).to(cuda).requires_grad_(True) for i, t in enumerate(make(list(range(1, 331)), torch.float32, 8, 0.1))]
+        for i, p in enumerate(ps):
+            p.grad = None if i % 7 == 3 else torch.ones_like(p)
+        start = [p.detach().clone() for p in ps]
+        opt = FusedAdamW(ps, lr=1e-2, state_bits=bits, max_norm=max_norm)
+        opt.step(), opt.step()
+        off = 0
+        for i, (p, s) in enumerate(zip(ps, start)):
+            span = slice(off, off + (p.numel() + 127) // 128 * 128)
+            off = span.stop
+            assert torch.equal(p, s) == (i % 7 == 3), i
+            assert bool(opt.exp_avg[span].float().any()) != (i % 7 == 3) and bool(opt.exp_avg_sq[span].float().any()) != (i % 7 == 3)

@@ -247,3 +247,33 @@ def test_activations_of_an_8_bit_network_refuse_what_it_refuses(cuda):
         net.forward_with_activations(torch.zeros(1, 4, 2, device=cuda), params={k: v[None] for k, v in net.named_parameters()})
     with pytest.raises(RuntimeError, match='ROCm'):
         net.cpu().forward_with_activations(torch.zeros(1, 4, 2))
+
+
+def test_relu_block_trains_on_3d_inputs(cuda):
+    """Its relu works in place on what the layer returned, a view of its rows where the input has three dimensions: value and
+    gradients are those of the layers with a relu that copies."""
+    from siren_amd import fp8
+    from siren_amd.modules import FCBlock
+    torch.manual_seed(0)
+    net = FCBlock(96, 70, 2, 128, outermost_linear=False, nonlinearity='relu', precision='fp8').to(cuda)
+    x = torch.randn(7, 50, 96, device=cuda)
+    dy = torch.randn(7, 50, 70, device=cuda)
+    for shape in ((7, 50), (350,)):
+        leaf = x.view(*shape, 96).clone().requires_grad_(True)
+        got = torch.autograd.grad(net(leaf), [leaf] + list(net.parameters()), dy.view(*shape, 70))
+        a = leaf
+        for l in net.net:
+            a = torch.relu(fp8.linear(a, l[0].weight, l[0].bias))
+        want = torch.autograd.grad(a, [leaf] + list(net.parameters()), dy.view(*shape, 70))
+        assert all(torch.equal(g, v) for g, v in zip(got, want))
+
+
+def test_function_transforms_are_refused(cuda):
+    """torch.func's wrappers have no memory of their own: an error, not a wrong result."""
+    from siren_amd import fp8
+    w, x = torch.randn(64, 96, device=cuda), torch.randn(4, 5, 96, device=cuda)
+    w8 = fp8.quantize(w, 'tile')
+    for call in (lambda: torch.vmap(lambda r: fp8.linear(r, w))(x), lambda: torch.vmap(lambda r: fp8.linear(r, w8))(x),
+                 lambda: torch.func.grad(lambda r: fp8.linear(r, w).sum())(x[0]), lambda: torch.vmap(lambda r: fp8.quantize(r).data)(x)):
+        with pytest.raises(RuntimeError):
+            call()

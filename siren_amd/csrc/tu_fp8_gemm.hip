@@ -2,11 +2,12 @@
 //
 //   out[m][n] = sum_b sa[m][b] sb[n][b] sum_{k in block b} a[m][k] b[n][k], 32-bit sums
 //
-// The card's fp8 matrix instructions keep about 17 bits of the products that one instruction sums (errors of 1e-5 of
-// the result on random operands, whatever the length), the bf16 ones lose nothing of these operands' products; an e4m3
-// value times a power of two is a bf16 number exactly, and v_cvt_scalef32_pk_bf16_fp8 makes two of them at once. So the
-// operands travel as bytes through HBM and LDS, are scaled and widened in registers, and the bf16 matrix pipe sums them,
-// for 16-bit results too (an output that nearly cancels would show the fp8 instructions' missing bits there as well).
+// The card's fp8 matrix instructions keep about 17 bits of the products that one instruction sums (rms errors of 1.5e-5 of
+// the result on random operands, whatever the length; the bf16 ones 1e-8 to 1e-7: tools/micro/fp8_sum_accuracy.hip), the bf16
+// ones lose nothing of these operands' products; an e4m3 value times a power of two is a bf16 number exactly, and
+// v_cvt_scalef32_pk_bf16_fp8 makes two of them at once. So the operands travel as bytes through HBM and LDS, are scaled and
+// widened in registers, and the bf16 matrix pipe sums them, for 16-bit results too (an output that nearly cancels would show the
+// fp8 instructions' missing bits there as well).
 // Exactly, that is, where bf16 reaches: of scale bytes 3 and more (e5m2: 10) every code is a bf16 number, its subnormal ones,
 // which the pipe keeps, among them. Below, in blocks whose magnitudes stay under 2^-116 (e5m2: 2^-102), values under 2^-126 are
 // rounded to multiples of 2^-133, the nearest, ties to even: off by 2^-134 at most. Above, a block whose largest magnitude

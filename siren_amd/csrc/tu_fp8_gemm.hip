@@ -16,7 +16,8 @@
 //
 // A workgroup of 4 waves owns 256 x 128 of out (128 x 128 where rows are few), each wave 128 x 64 (64 x 64) in tiles of
 // 32 x 32. Half a block, 64 k of both operands, is one stage of LDS: 24 KiB by direct global-to-LDS loads, three stages, so
-// the loads run two half blocks ahead; two workgroups share a CU, and one's stores run behind the other's products. With 128
+// the loads run two half blocks ahead; two workgroups share a CU, and one's stores run behind the other's products (where there
+// are more tiles than the 512 that the card holds at once: 512 begin, sum and store together). With 128
 // rows two stages of 16 KiB, so that four workgroups share a CU (50001 x 832 x 320: 44 us with three stages, 42 with two).
 // A half block of padding alone, and a wave whose rows or columns do not exist, take no products (42 -> 37 us).
 //
@@ -88,7 +89,8 @@ constexpr float MANY_TURNS = 4194304.f;  // 2^22: beyond, fp32 holds no whole nu
 // with the factor in two parts, so that neither omega z nor the product is rounded on the way. Of phases past MANY_TURNS the
 // fraction is taken in 64 bits: in a branch that the wave takes if any lane has one, where the others keep their result, so that
 // no output depends on its neighbours. Chosen for each element, the 64-bit steps were issued whether a lane needed them or not
-// (262144 x 1024 x 1024 with the sine 692 us, 670 then; 16384 x 1024 x 1024 bf16 40.2 with the phase first, 38.9).
+// (262144 x 1024 x 1024 with the sine 692 us, 670 then, both in the first passes after an idle card, which are slower than the
+// later 590; 16384 x 1024 x 1024 bf16 40.2 with the phase first, 38.9).
 __device__ __forceinline__ f32x4 turns4(const f32x4& z, const GemmArgs& g) {
     f32x4 u;
     float most = 0.f;
@@ -536,7 +538,10 @@ void launch_join(hipStream_t stream, const GemmArgs& g, const void* part, int sp
 int64_t tiles_of(int64_t m, int64_t n, int rows) { return (m + rows - 1) / rows * ((n + TN - 1) / TN); }
 bool less_waste(int64_t m) { return 10 * ((m + 255) / 256 * 256) > 11 * ((m + 127) / 128 * 128); }  // by 128 rows, over 10 %
 
-// 262144 x 1024 x 1024: 590 us with 256 rows, 607 with 128; 16384 x 4096 x 4096: 453 and 491; 50001 x 832 x 320: 48 and 37
+// 262144 x 1024 x 1024: 590 us with 256 rows, 607 with 128; 16384 x 4096 x 4096: 453 and 491; 50001 x 832 x 320: 48 and 37.
+// At the borders, whole layers of bf16 rows with their rounding: 16384 x 1024 x 1024 (512 tiles) 46.3 and 48.0 us, 12288 rows of
+// it (384 tiles) 41.1 and 38.2; k = 768 37.7 and 38.4, of 65536 rows 134 and 134, with the sine 41.3 and 41.1, 146 and 142; k =
+// 512 of 65536 rows 99 and 97, with the sine 111 and 106
 bool tall(int64_t m, int64_t n, int64_t k) { return k >= 1024 && tiles_of(m, n, 256) >= 512 && !less_waste(m); }
 
 // A product whose tiles do not fill the card splits its k axis, where that pays for the partial results' way through memory

@@ -175,8 +175,9 @@ def _check_fp8_network(coords, weights_biases):
 
 def _fp8_sine_apply(coords, weights_biases, outermost_linear):
     """A sine network with its hidden products in 8 bits (fp8.linear with the sine in its epilogue), activations between
-    them in bf16 (8 bits of mantissa for values that the next layer rounds to 4). The first layer, and a last one with
-    fewer than FP8_MIN_FEATURES outputs, are plain fp32. Trains on values; its gradients are not differentiable again."""
+    them in bf16 (8 bits of mantissa for values that the next layer rounds to 4). Layers with fewer than FP8_MIN_FEATURES
+    inputs or outputs, as a network's first and last mostly are, are plain fp32. Trains on values; its gradients are not
+    differentiable again."""
     _check_fp8_network(coords, weights_biases)
     a = coords
     for i, (W, b) in enumerate(weights_biases):
@@ -389,8 +390,10 @@ class SingleBVPNet(MetaModule):
     split W0 forward plus the bf16x6 W2 backward (siren_backward_split: split-bf16 recompute + reverse, fp32 MFMA
     wgrad). A backward through the jet node recomputes on the fp32 kernels.
     precision='fp8' runs the products of every layer with 64 inputs and outputs at least on 8-bit operands with a scale
-    per block of 128, forward and backward (fp8.linear): values to some 2^-5 a layer, any hidden width, losses on
-    model_out only (a loss on gradient() raises in its backward).
+    per block of 128, forward and backward (fp8.linear): sine activations with an rms error of 2^-5 of theirs after one such
+    layer and 2^-4 after three, any hidden width, losses on model_out only (a loss on gradient() raises in its backward). It
+    is for wide networks: a training step of 5 x 1024 takes a third of fp32's time, one of 5 x 256, whose fp32 and bf16x6
+    kernels keep activations on the chip, 1.3 times it.
     """
 
     def __init__(self, out_features=1, type='sine', in_features=2, mode='mlp', hidden_features=256,

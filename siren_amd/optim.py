@@ -143,7 +143,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
 
 class FusedAdamW:
     """AdamW over parameters where they lie (any mix of fp32, bf16, fp16; .grad may be replaced freely, and be missing: the
-    parameter and its moments then stay, and its bias corrections count its own steps), two launches a step. state_bits 8 keeps the moments in 8 bits (2 bytes a parameter instead of 8), rounded at random from seed."""
+    parameter and its moments then stay, and its bias corrections count its own steps), two launches a step. state_bits 8 keeps the moments in 8 bits (2 bytes a parameter instead of 8), rounded at random from seed. One
+    set of hyperparameters (attributes: opt.lr = ... between steps) for all parameters; no torch.optim.Optimizer."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32,
                  seed=0):

@@ -475,7 +475,7 @@ MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Mayb
     std::vector<int64_t> numels(n);
     std::vector<int32_t> types(n);
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-    spans.reserve(n);
+    spans.reserve(n + 6);
     std::vector<Tensor> keep;
     int64_t size = 0;
     for (size_t i = 0; i < n; ++i) {
@@ -504,9 +504,6 @@ MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Mayb
         if (numels[i] > 0) spans.emplace_back((uintptr_t)ps[i], (uintptr_t)ps[i] + p.nbytes());
         size += padded(numels[i]);
     }
-    std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); ++i)
-        TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first, "adamw_step: parameters overlap (is one listed twice?)");
     TORCH_CHECK_VALUE(bool(sm) == bool(sv), "scales must be two tensors");
     const auto want = sm ? at::kFloat8_e4m3fn : at::kFloat;
     const std::pair<const char*, const Tensor*> states[2] = {{"exp_avg", &m}, {"exp_avg_sq", &v}};
@@ -523,6 +520,17 @@ MaybeTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Mayb
     TORCH_CHECK_VALUE(!counts || (counts->scalar_type() == at::kLong && counts->numel() == (int64_t)n && counts->device() == dev &&
                                   counts->is_contiguous()),
                       "counts must be ", n, " contiguous int64 on ", dev);
+    // what is written lies apart: one thread's store must not be another's load
+    const auto span = [&](const Tensor& t) {
+        if (t.numel() > 0) spans.emplace_back((uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + t.nbytes());
+    };
+    span(m), span(v), span(step);
+    if (sm) span(*sm), span(*sv);
+    if (counts) span(*counts);
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first,
+                          "adamw_step: parameters or states overlap (is a parameter listed twice, a state given for two?)");
     TORCH_CHECK_VALUE(!max_norm || *max_norm > 0., "max_norm must be positive or None; got ", max_norm.value_or(0.));
     int64_t need = 0;
     check(lib.adamw_scratch_bytes((int64_t)n, &need), "siren_adamw_scratch_bytes");

@@ -12,10 +12,10 @@
 // inputs. The update of p uses the moments before they are rounded.
 //
 // Bytes bound it: 28 a parameter with fp32 moments, 16 with 8-bit ones (p read and written, g read, moments read and
-// written), 4 more for the norm. 35 million fp32 parameters: the norm 44 us (3.2 TB/s; twice the workgroups or twice the
-// loads in flight gained nothing), 32-bit moments 170 us (5.8 TB/s), 8-bit ones 100 to 112 us by the
-// state (5.6 to 5.0 TB/s). Ten tensors of 198 thousand: 9 us, two launches. The tensors' pointers travel as kernel arguments (no table in device memory, so a captured step holds
-// what it needs), ADAMW_TENSORS a launch.
+// written), 4 more for the norm. 35 million fp32 parameters: the norm 44 us (3.2 TB/s; twice the workgroups or twice
+// the loads in flight gained nothing), 32-bit moments 170 us (5.8 TB/s), 8-bit ones 100 to 112 us by the state (5.6 to
+// 5.0 TB/s). Ten tensors of 198 thousand: 9 us, two launches. The tensors' pointers travel as kernel arguments (no
+// table in device memory, so a captured step holds what it needs), ADAMW_TENSORS a launch.
 #include <cmath>
 
 #include "adamw.h"

@@ -579,3 +579,23 @@ def test_parameters_without_a_gradient_stay(cuda, bits):
             off = span.stop
             assert torch.equal(p, s) == (i % 7 == 3), i
             assert bool(opt.exp_avg[span].float().any()) != (i % 7 == 3) and bool(opt.exp_avg_sq[span].float().any()) != (i % 7 == 3)
+
+
+def test_states_that_overlap_are_refused(cuda):
+    """Two states in the same memory, a state inside a parameter, counts that are the step: each would be written by one thread
+    and read by another."""
+    from siren_amd.optim import FusedAdamW, adamw_step
+    p = [torch.ones(128, device=cuda)]
+    g = [torch.ones(128, device=cuda)]
+    a, b = FusedAdamW(p), FusedAdamW(p, state_bits=8)
+    one = dict(params=p, grads=g, exp_avg=a.exp_avg, exp_avg_sq=a.exp_avg_sq, step=a.steps, counts=a.counts)
+    eight = dict(params=p, grads=g, exp_avg=b.exp_avg, exp_avg_sq=b.exp_avg_sq, step=b.steps, scales=b.scales)
+    shared = torch.zeros(192, device=cuda)
+    for ok, change in ((one, dict(exp_avg_sq=a.exp_avg)), (one, dict(counts=a.steps)), (one, dict(exp_avg=p[0])),
+                       (one, dict(exp_avg=shared[:128], exp_avg_sq=shared[64:])), (one, dict(step=a.exp_avg[:2].view(torch.int64))),
+                       (eight, dict(scales=(b.scales[0],) * 2)), (eight, dict(exp_avg=b.exp_avg_sq)),
+                       (eight, dict(scales=(b.scales[0], b.exp_avg[:1].view(torch.uint8))))):
+        with pytest.raises(ValueError, match='overlap'):
+            adamw_step(**{**ok, **change})
+    assert bool((p[0] == 1).all()) and int(a.steps) == 0 and int(b.steps) == 0
+    adamw_step(**one), adamw_step(**eight)

@@ -599,3 +599,33 @@ def test_states_that_overlap_are_refused(cuda):
             adamw_step(**{**ok, **change})
     assert bool((p[0] == 1).all()) and int(a.steps) == 0 and int(b.steps) == 0
     adamw_step(**one), adamw_step(**eight)
+
+
+def test_elements_past_2_to_the_31(cuda):
+    """A tensor of 2^31 elements and more, and one behind it: their last elements and moments are those of a short list, the
+    zeros before them stay zeros."""
+    from siren_amd.optim import FusedAdamW
+    n, tail = (1 << 31) + 777, 5000
+    for bits in (32, 8):
+        big = [torch.zeros(n, dtype=torch.bfloat16, device=cuda), torch.zeros(300, dtype=torch.bfloat16, device=cuda)]
+        for p in big:
+            p.grad = torch.zeros_like(p)
+        g = make([tail, 300], torch.bfloat16, 3)
+        start = make([tail, 300], torch.bfloat16, 4)
+        short = [s.to(cuda) for s in start]
+        for p, q, s, x in zip(big, short, start, g):
+            p[-s.numel():], p.grad[-s.numel():] = s.to(cuda), x.to(cuda)
+            q.grad = x.to(cuda)
+        a, b = (FusedAdamW(ps, lr=1e-2, weight_decay=0.1, max_norm=1., state_bits=bits) for ps in (big, short))
+        a.step(), b.step()
+        assert torch.equal(a.grad_norm(), b.grad_norm())
+        assert all(torch.equal(p[-q.numel():], q) for p, q in zip(big, short))
+        assert not big[0][:-tail].any()
+        if bits == 32:
+            for s, t in ((a.exp_avg, b.exp_avg), (a.exp_avg_sq, b.exp_avg_sq)):
+                assert torch.equal(s[n - tail:n], t[:tail]) and torch.equal(s[-384:], t[-384:]) and not s[:n - tail].any()
+        else:
+            u = lambda o, k: (o.exp_avg_sq[k].float().view(-1, 128) * torch.exp2(o.scales[1].float()[:, None] - 127)[k.start // 128:k.stop // 128])
+            x, y = u(a, slice(a.exp_avg.numel() - 384, a.exp_avg.numel())), u(b, slice(b.exp_avg.numel() - 384, b.exp_avg.numel()))
+            assert ((x - y).abs() <= torch.maximum(x, y) / 8 + torch.exp2(b.scales[1][-3:].float() - 127)[:, None] * 2. ** -9).all()  # by other random bits
+            assert not a.exp_avg[:n - tail - 128].view(torch.uint8).any()

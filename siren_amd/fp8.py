@@ -92,8 +92,8 @@ def linear(x, weight, bias=None, activation=None, omega=30., grad_dtype=torch.fl
 
     weight: a tensor (out, in) of any of the three types, quantised on the way and differentiable, or Blocks from
     quantize(weight, 'tile') (a weight that stays in 8 bits: forward only). activation: None or 'sine', sin(omega z).
-    A layer has fewer than 2^22 outputs and, where x or the weight need gradients, fewer than 2^22 inputs (2^24 otherwise); a
-    weight's gradient sums over at most 2^24 - 128 rows.
+    A layer has fewer than 2^22 outputs and, where x or the weight need gradients, fewer than 2^22 inputs (2^24 - 128 at
+    most otherwise); a weight's gradient sums over at most 2^24 - 128 rows.
     The backward gives dx, dW and db; its gradients are rounded to grad_dtype (e4m3 or e5m2) and are not differentiable
     again. dW is quantised products of gradients and activations, so its relative error is that of e4m3's 3 bits. The sine's
     derivative omega cos(omega z) is kept in bf16 from the forward to the backward: each term of db is dy times that, off by
